@@ -141,8 +141,9 @@ def _stored(x):
     pad = -n % BLOCK
     b = torch.cat([x, x.new_zeros(m, pad)], 1).view(m, -1, BLOCK)
     most = b.abs().amax(-1, keepdim=True)
-    codes = torch.round(b * torch.where(most > 0, 127.0 / most, 0.0))
-    return (codes * (most / 127.0)).view(m, -1)[:, :n]
+    top = torch.full_like(most, 127.0)                 # (a tensor: torch multiplies by the inverse of a number, which moves ties)
+    codes = torch.round(b * top / torch.where(most > 0, most, 1.0))
+    return (codes * (most / top)).view(m, -1)[:, :n]
 
 
 def _act(g, kind):
@@ -245,8 +246,8 @@ def exact(case, seed):
             out = torch.empty_like(v)
             for at in range(0, v.shape[1], BLOCK):
                 part = v[:, at:at + BLOCK]
-                step = part.abs().max(dim=1, keepdim=True).values / 127
-                out[:, at:at + BLOCK] = torch.where(step > 0, torch.round(part / step.clamp_min(1e-300)), 0) * step
+                largest = part.abs().max(dim=1, keepdim=True).values
+                out[:, at:at + BLOCK] = torch.round(127 * part / largest.clamp_min(1e-300)) * largest / 127
             return out
 
         if case["op"] == "store":
