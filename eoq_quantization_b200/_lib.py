@@ -48,6 +48,8 @@ EXPORTS = [
     "eoq_b200_dequant_packed", "eoq_b200_gemv_packed", "eoq_b200_gemv_polar_codes",
     "eoq_b200_linear_packed", "eoq_b200_linear_polar_codes", "eoq_b200_weight_linear", "eoq_b200_weight_linear_scratch",
     "eoq_b200_linear_status", "eoq_b200_weight_status",
+    "eoq_b200_gated_scratch", "eoq_b200_gated_packed", "eoq_b200_gated_grad_scratch", "eoq_b200_gated_grad",
+    "eoq_b200_packed_input_grad_scratch", "eoq_b200_packed_input_grad", "eoq_b200_store_8bit", "eoq_b200_load_8bit",
 ]
 #: exported for this project's benchmarks and tests only (declared in csrc/eoq_internal.h, not in the public header)
 INTERNAL_EXPORTS = ["eoq_b200_ordered_launches", "eoq_b200_linear_packed_preferred", "eoq_b200_weight_linear_preferred", "eoq_b200_tune", "eoq_b200_launch_count", "eoq_b200_weight_read"]
@@ -107,6 +109,15 @@ class TilesView(C.Structure):
                 ("precision_bits", C.c_uint32), ("num_tiles", C.c_uint32), ("num_col_segments", C.c_uint32),
                 ("table", C.POINTER(C.c_uint32)), ("tiles", C.POINTER(C.c_uint32)), ("stream", C.POINTER(C.c_uint8)),
                 ("stream_bytes", C.c_uint64), ("max_lane_drift", C.c_uint32), ("head_bytes", C.c_uint32)]
+
+
+class Gated(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("gate", "up", "gate_scales", "up_scales", "gate_bias", "up_bias")] + \
+               [(n, C.c_uint32) for n in ("rows", "cols", "bits", "group")] + [("activation", C.c_int)]
+
+
+class Kept(C.Structure):
+    _fields_ = [("form", C.c_int), ("gate", C.c_void_p), ("up", C.c_void_p), ("gate_scales", C.c_void_p), ("up_scales", C.c_void_p)]
 
 
 _LIB: Optional[C.CDLL] = None
@@ -184,6 +195,14 @@ def lib() -> C.CDLL:
         "eoq_b200_weight_linear_scratch": (C.c_size_t, [vp, C.c_uint32, C.c_int]),
         "eoq_b200_linear_status": (C.c_uint32, []),
         "eoq_b200_weight_status": (C.c_int, [vp, vp]),
+        "eoq_b200_gated_scratch": (C.c_size_t, [C.POINTER(Gated), C.POINTER(Kept), C.c_int, C.c_uint32]),
+        "eoq_b200_gated_packed": (C.c_int, [C.POINTER(Gated), vp, C.c_int, C.c_uint32, vp, vp, C.POINTER(Kept), vp]),
+        "eoq_b200_gated_grad_scratch": (C.c_size_t, [C.POINTER(Gated), C.POINTER(Kept), C.c_int, C.c_uint32]),
+        "eoq_b200_gated_grad": (C.c_int, [C.POINTER(Gated), C.POINTER(Kept), vp, C.c_int, C.c_uint32, vp, vp, vp, vp, vp]),
+        "eoq_b200_packed_input_grad_scratch": (C.c_size_t, [C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_int, C.c_uint32]),
+        "eoq_b200_packed_input_grad": (C.c_int, [vp, vp, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, vp, C.c_int, C.c_uint32, vp, vp, vp]),
+        "eoq_b200_store_8bit": (C.c_int, [vp, C.c_int, C.c_size_t, C.c_uint32, vp, vp, vp]),
+        "eoq_b200_load_8bit": (C.c_int, [vp, vp, C.c_size_t, C.c_uint32, vp, C.c_int, vp]),
         "eoq_b200_tune": (C.c_int, [C.c_char_p, C.c_int]),
         "eoq_b200_ordered_launches": (C.c_int, [C.c_int]),
         "eoq_b200_linear_packed_preferred": (C.c_int, [vp, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, vp, C.c_int, C.c_uint32]),

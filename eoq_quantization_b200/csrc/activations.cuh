@@ -1,0 +1,68 @@
+// Activations of a gated block and their derivatives in fp32, the power of two that brings a row into fp16's range, and the 8-bit
+// storage of a block.
+#pragma once
+
+#include <cstdint>
+#include <cuda_runtime.h>
+
+#include "gated.h"
+
+namespace eoq {
+
+// value and derivative: silu g s(g), s(g) (1 + g (1 - s(g))); gelu g P(g), P(g) + g p(g) of the normal distribution; gelu_tanh with
+// P(g) = (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))) / 2
+__device__ __forceinline__ void activation_and_slope(float g, int act, float &value, float &slope)
+{
+    if (act == kActSilu) {
+        const float s = 1.0f / (1.0f + __expf(-g));
+        value = g * s;
+        slope = s * (1.0f + g * (1.0f - s));
+    } else if (act == kActGelu) {
+        const float p = 0.5f * (1.0f + erff(g * 0.70710678f));
+        value = g * p;
+        slope = p + g * __expf(-0.5f * g * g) * 0.39894228f;
+    } else {
+        const float t = tanhf(0.79788456f * (g + 0.044715f * g * g * g)), p = 0.5f * (1.0f + t);
+        value = g * p;
+        slope = p + g * 0.5f * (1.0f - t * t) * 0.79788456f * (1.0f + 0.134145f * g * g);
+    }
+}
+
+__device__ __forceinline__ float activation(float g, int act)
+{
+    float value, slope;
+    activation_and_slope(g, act, value, slope);
+    return value;
+}
+
+__device__ __forceinline__ float finite_magnitude(float v) { return fabsf(v) < __int_as_float(0x7f800000) ? fabsf(v) : 0.0f; }
+
+// e with 2^14 <= most 2^e < 2^15, within what a float holds; rows without a finite value other than zero stay as they are
+__device__ __forceinline__ int half_exponent(float most) { return most > 0.0f ? min(120, 141 - (int)(__float_as_uint(most) >> 23)) : 0; }
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+
+// A block's scale and codes from the bits of its largest magnitude (as a whole number, so that NaN is above infinity).  A code is
+// the quotient 127 v / largest to the nearest whole number: the product with the inverse, corrected by what is left of 127 v
+// (Markstein's step), so that quotients halfway between two codes, which 16-bit values often have, come out as such and go to
+// the even one.
+struct Storer {
+    float scale, most, inv;
+    __device__ __forceinline__ explicit Storer(uint32_t bits)
+    {
+        most = __uint_as_float(bits);
+        const bool fine = bits < 0x7f800000u, zero = most < 1e-30f;
+        scale = !fine ? __uint_as_float(0x7fffffffu) : zero ? 0.0f : __fdiv_rn(most, 127.0f);
+        inv = !fine || zero ? 0.0f : __fdiv_rn(1.0f, most);
+        if (!fine || zero) most = 0.0f;
+    }
+    __device__ __forceinline__ int8_t code(float v) const
+    {
+        if (inv == 0.0f) return 0;
+        // (1e-30 and more; above 2^120 in 128ths, so that neither 127 v nor the products leave the range)
+        const float f = most > 1e36f ? 0.0078125f : 1.0f, w = 127.0f * (v * f), q = w * inv, p = most * f;
+        const float t = f == 1.0f ? q : q * 128.0f;
+        return (int8_t)__float2int_rn(fmaf(fmaf(-t, p, w), f == 1.0f ? inv : inv * 128.0f, t));
+    }
+};
+
+}  // namespace eoq

@@ -388,6 +388,206 @@ PyObject *polar_linear(PyObject *, PyObject *const *a, Py_ssize_t n)
     GUARD_END
 }
 
+// -- the gated block on packed weights ------------------------------------------
+
+// A packed weight beside x: codes in the layout of `bits`, scales that cover the flattened matrix, converted to fp16 where a cast
+// of the module left them in another type.
+struct Packed {
+    const uint8_t *codes = nullptr;
+    const uint16_t *scales = nullptr;
+    bool converted = false;
+    bool open(PyObject *codes_, PyObject *scales_, const Tensor &x, int64_t N, int64_t K, int64_t bits, int64_t group)
+    {
+        const Tensor *pk = tensor_of(codes_);
+        const int64_t row_bytes = bits == 4 ? (K + 1) / 2 : bits == 2 ? (K + 3) / 4 : K;
+        if (N < 1 || N > 0x7fffffff || K < 1 || K > 0x7fffffff || bits < 2 || bits > 8 || group < 1 || group > 0x7fffffff ||
+            !resident(pk, x, bits == 4 || bits == 2 ? at::kByte : at::kChar) || pk->numel() != N * row_bytes || !sc.open(scales_, x, at::kHalf) ||
+            sc.t->numel() < (N * K + group - 1) / group)
+            return false;
+        codes = static_cast<const uint8_t *>(pk->data_ptr());
+        scales = static_cast<const uint16_t *>(sc.t->data_ptr());
+        converted = sc.converted;
+        return true;
+    }
+
+  private:
+    Parameter sc;
+};
+
+Tensor bytes_beside(const Tensor &x, size_t n) { return at::detail::empty_cuda({(int64_t)n}, at::kByte, x.device(), std::nullopt); }
+
+constexpr int64_t kStoreBlock = 64;
+
+// Tensors that the forward pass leaves: values of x's type, or signed codes and fp32 scales.
+struct KeptTensors {
+    Tensor v[2], scale[2];
+    eoq_b200_kept_t c = {};
+    KeptTensors(int form, const Tensor &x, int64_t rows, int64_t N)
+    {
+        c.form = form;
+        if (form == EOQ_B200_KEEP_NONE) return;
+        for (int i = 0; i < 2; i++) {
+            v[i] = at::detail::empty_cuda({rows, N}, form == EOQ_B200_KEEP_FULL ? x.scalar_type() : at::kChar, x.device(), std::nullopt);
+            if (form == EOQ_B200_KEEP_8BIT) scale[i] = at::detail::empty_cuda({rows, (N + kStoreBlock - 1) / kStoreBlock}, at::kFloat, x.device(), std::nullopt);
+        }
+        c.gate = v[0].data_ptr(); c.up = v[1].data_ptr();
+        if (form == EOQ_B200_KEEP_8BIT) { c.gate_scales = static_cast<float *>(scale[0].data_ptr()); c.up_scales = static_cast<float *>(scale[1].data_ptr()); }
+    }
+};
+
+bool wrap_into(PyObject *tuple, Py_ssize_t i, Tensor &&t)
+{
+    PyObject *o = THPVariable_Wrap(std::move(t));
+    if (!o) return false;
+    PyTuple_SET_ITEM(tuple, i, o);
+    return true;
+}
+
+// gated_packed(gate, gate_scales, up, up_scales, N, K, bits, group, x, gate_bias, up_bias, activation, form): h, or with a form of
+// keeping (h, gate, up[, gate_scales, up_scales]).
+PyObject *gated_packed(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    if (n != 13) { PyErr_SetString(PyExc_TypeError, "gated_packed takes 13 arguments"); return nullptr; }
+    GUARD_BEGIN
+    const int64_t N = PyLong_AsLongLong(a[4]), K = PyLong_AsLongLong(a[5]), bits = PyLong_AsLongLong(a[6]), group = PyLong_AsLongLong(a[7]);
+    const int form = (int)PyLong_AsLong(a[12]);
+    Activations act;
+    Packed gate, up;
+    Bias bias[2];
+    if (!act.open(a[8], K) || !gate.open(a[0], a[1], *act.x, N, K, bits, group) || !up.open(a[2], a[3], *act.x, N, K, bits, group) ||
+        !bias[0].open(a[9], *act.x, N) || !bias[1].open(a[10], *act.x, N))
+        Py_RETURN_NONE;
+    const Tensor &x = *act.x;
+    const Ordered ordered(gate.converted || up.converted);
+    const eoq_b200_gated_t w = {gate.codes, up.codes, gate.scales, up.scales, bias[0].p, bias[1].p, (uint32_t)N, (uint32_t)K, (uint32_t)bits, (uint32_t)group,
+                                (int)PyLong_AsLong(a[11])};
+    if (PyErr_Occurred()) return nullptr;
+    KeptTensors kept(form, x, act.rows, N);
+    Tensor h = result(x, N, x.scalar_type()), scratch;
+    if (const size_t bytes = eoq_b200_gated_scratch(&w, &kept.c, act.code, (uint32_t)act.rows)) scratch = bytes_beside(x, bytes);
+    const eoq_error_t rc = eoq_b200_gated_packed(&w, x.data_ptr(), act.code, (uint32_t)act.rows, scratch.defined() ? scratch.data_ptr() : nullptr, h.data_ptr(),
+                                                 &kept.c, stream_of(x));
+    if (rc != EOQ_OK) return failed(rc, "eoq_b200_gated_packed");
+    if (form == EOQ_B200_KEEP_NONE) return THPVariable_Wrap(std::move(h));
+    PyObject *out = PyTuple_New(form == EOQ_B200_KEEP_FULL ? 3 : 5);
+    if (!out) return nullptr;
+    bool ok = wrap_into(out, 0, std::move(h)) && wrap_into(out, 1, std::move(kept.v[0])) && wrap_into(out, 2, std::move(kept.v[1]));
+    if (form == EOQ_B200_KEEP_8BIT) ok = ok && wrap_into(out, 3, std::move(kept.scale[0])) && wrap_into(out, 4, std::move(kept.scale[1]));
+    if (ok) return out;
+    Py_DECREF(out);
+    return nullptr;
+    GUARD_END
+}
+
+// gated_grad(gate, gate_scales, up, up_scales, N, K, bits, group, activation, dh, kept gate, kept up, their scales or None x 2, want dx,
+// want the gate's bias, want the up's): (dx or None, fp32 or None, fp32 or None).
+PyObject *gated_grad(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    if (n != 17) { PyErr_SetString(PyExc_TypeError, "gated_grad takes 17 arguments"); return nullptr; }
+    GUARD_BEGIN
+    const int64_t N = PyLong_AsLongLong(a[4]), K = PyLong_AsLongLong(a[5]), bits = PyLong_AsLongLong(a[6]), group = PyLong_AsLongLong(a[7]);
+    Activations act;
+    Packed gate, up;
+    if (!act.open(a[9], N) || !gate.open(a[0], a[1], *act.x, N, K, bits, group) || !up.open(a[2], a[3], *act.x, N, K, bits, group)) Py_RETURN_NONE;
+    const Tensor &dh = *act.x;
+    eoq_b200_kept_t kept = {};
+    kept.form = a[12] == Py_None ? EOQ_B200_KEEP_FULL : EOQ_B200_KEEP_8BIT;
+    const Tensor *kg = tensor_of(a[10]), *ku = tensor_of(a[11]);
+    const at::ScalarType type = kept.form == EOQ_B200_KEEP_FULL ? dh.scalar_type() : at::kChar;
+    if (!resident(kg, dh, type) || !resident(ku, dh, type) || kg->numel() != act.rows * N || ku->numel() != act.rows * N) Py_RETURN_NONE;
+    kept.gate = kg->data_ptr(); kept.up = ku->data_ptr();
+    if (kept.form == EOQ_B200_KEEP_8BIT) {
+        const Tensor *gs = tensor_of(a[12]), *us = tensor_of(a[13]);
+        const int64_t blocks = act.rows * ((N + kStoreBlock - 1) / kStoreBlock);
+        if (!resident(gs, dh, at::kFloat) || !resident(us, dh, at::kFloat) || gs->numel() != blocks || us->numel() != blocks) Py_RETURN_NONE;
+        kept.gate_scales = static_cast<float *>(gs->data_ptr()); kept.up_scales = static_cast<float *>(us->data_ptr());
+    }
+    const Ordered ordered(gate.converted || up.converted);
+    const eoq_b200_gated_t w = {gate.codes, up.codes, gate.scales, up.scales, nullptr, nullptr, (uint32_t)N, (uint32_t)K, (uint32_t)bits, (uint32_t)group,
+                                (int)PyLong_AsLong(a[8])};
+    const bool want[3] = {PyObject_IsTrue(a[14]) == 1, PyObject_IsTrue(a[15]) == 1, PyObject_IsTrue(a[16]) == 1};
+    if (PyErr_Occurred()) return nullptr;
+    Tensor scratch = bytes_beside(dh, eoq_b200_gated_grad_scratch(&w, &kept, act.code, (uint32_t)act.rows)), out[3];
+    if (want[0]) out[0] = result(dh, K, dh.scalar_type());
+    for (int i = 1; i < 3; i++) if (want[i]) out[i] = at::detail::empty_cuda({N}, at::kFloat, dh.device(), std::nullopt);
+    const eoq_error_t rc = eoq_b200_gated_grad(&w, &kept, dh.data_ptr(), act.code, (uint32_t)act.rows, scratch.data_ptr(), want[0] ? out[0].data_ptr() : nullptr,
+                                               want[1] ? static_cast<float *>(out[1].data_ptr()) : nullptr,
+                                               want[2] ? static_cast<float *>(out[2].data_ptr()) : nullptr, stream_of(dh));
+    if (rc != EOQ_OK) return failed(rc, "eoq_b200_gated_grad");
+    PyObject *r = PyTuple_New(3);
+    if (!r) return nullptr;
+    for (int i = 0; i < 3; i++) {
+        if (!want[i]) { Py_INCREF(Py_None); PyTuple_SET_ITEM(r, i, Py_None); }
+        else if (!wrap_into(r, i, std::move(out[i]))) { Py_DECREF(r); return nullptr; }
+    }
+    return r;
+    GUARD_END
+}
+
+// input_grad(packed, scales, N, K, bits, group, dy): dx.
+PyObject *input_grad(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    if (n != 7) { PyErr_SetString(PyExc_TypeError, "input_grad takes 7 arguments"); return nullptr; }
+    GUARD_BEGIN
+    const int64_t N = PyLong_AsLongLong(a[2]), K = PyLong_AsLongLong(a[3]), bits = PyLong_AsLongLong(a[4]), group = PyLong_AsLongLong(a[5]);
+    Activations act;
+    Packed w;
+    if (!act.open(a[6], N) || !w.open(a[0], a[1], *act.x, N, K, bits, group)) Py_RETURN_NONE;
+    const Tensor &dy = *act.x;
+    const Ordered ordered(w.converted);
+    Tensor dx = result(dy, K, dy.scalar_type());
+    Tensor scratch = bytes_beside(dy, eoq_b200_packed_input_grad_scratch((uint32_t)N, (uint32_t)K, (uint32_t)bits, (uint32_t)group, act.code, (uint32_t)act.rows));
+    return done(eoq_b200_packed_input_grad(w.codes, w.scales, (uint32_t)N, (uint32_t)K, (uint32_t)bits, (uint32_t)group, dy.data_ptr(), act.code,
+                                           (uint32_t)act.rows, scratch.data_ptr(), dx.data_ptr(), stream_of(dy)),
+                std::move(dx), "eoq_b200_packed_input_grad");
+    GUARD_END
+}
+
+// store_8bit(x): (codes, scales) of the rows of x.
+PyObject *store_8bit(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    if (n != 1) { PyErr_SetString(PyExc_TypeError, "store_8bit takes 1 argument"); return nullptr; }
+    GUARD_BEGIN
+    const Tensor *t = tensor_of(a[0]);
+    if (!t || t->dim() < 1) Py_RETURN_NONE;
+    const int64_t N = t->size(-1);
+    Activations act;
+    if (!act.open(a[0], N) || N > 0x7fffffff) Py_RETURN_NONE;
+    const Tensor &x = *act.x;
+    Tensor codes = result(x, N, at::kChar), scales = result(x, (N + kStoreBlock - 1) / kStoreBlock, at::kFloat);
+    const eoq_error_t rc = eoq_b200_store_8bit(x.data_ptr(), act.code, (size_t)act.rows, (uint32_t)N, static_cast<int8_t *>(codes.data_ptr()),
+                                               static_cast<float *>(scales.data_ptr()), stream_of(x));
+    if (rc != EOQ_OK) return failed(rc, "eoq_b200_store_8bit");
+    PyObject *out = PyTuple_New(2);
+    if (!out) return nullptr;
+    if (wrap_into(out, 0, std::move(codes)) && wrap_into(out, 1, std::move(scales))) return out;
+    Py_DECREF(out);
+    return nullptr;
+    GUARD_END
+}
+
+// load_8bit(codes, scales, type): the values, 0 fp16, 1 bf16, 2 fp32.
+PyObject *load_8bit(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    if (n != 3) { PyErr_SetString(PyExc_TypeError, "load_8bit takes 3 arguments"); return nullptr; }
+    GUARD_BEGIN
+    const Tensor *codes = tensor_of(a[0]), *scales = tensor_of(a[1]);
+    const int type = (int)PyLong_AsLong(a[2]);
+    if (PyErr_Occurred()) return nullptr;
+    if (!codes || !scales || !codes->is_cuda() || codes->dim() < 1 || thread_is_watched() || kind_of(*codes) != kPlain || kind_of(*scales) != kPlain) Py_RETURN_NONE;
+    const int64_t N = codes->size(-1), rows = N ? codes->numel() / N : 0;
+    if (N < 1 || rows < 1 || N > 0x7fffffff || type < 0 || type > 2 || !resident(codes, *codes, at::kChar) || !resident(scales, *codes, at::kFloat) ||
+        scales->numel() != rows * ((N + kStoreBlock - 1) / kStoreBlock))
+        Py_RETURN_NONE;
+    std::optional<c10::cuda::CUDAGuard> guard;
+    if (codes->get_device() != c10::cuda::current_device()) guard.emplace(codes->device());
+    Tensor y = result(*codes, N, type == EOQ_B200_F16 ? at::kHalf : type == EOQ_B200_BF16 ? at::kBFloat16 : at::kFloat);
+    return done(eoq_b200_load_8bit(static_cast<const int8_t *>(codes->data_ptr()), static_cast<const float *>(scales->data_ptr()), (size_t)rows, (uint32_t)N,
+                                   y.data_ptr(), type, stream_of(*codes)),
+                std::move(y), "eoq_b200_load_8bit");
+    GUARD_END
+}
+
 // -- codec ---------------------------------------------------------------------
 
 // A C-contiguous buffer for as long as it is in scope.
@@ -609,6 +809,11 @@ PyMethodDef methods[] = {
     {"weight_linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(weight_linear)), METH_FASTCALL, nullptr},
     {"packed_linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(packed_linear)), METH_FASTCALL, nullptr},
     {"polar_linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(polar_linear)), METH_FASTCALL, nullptr},
+    {"gated_packed", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(gated_packed)), METH_FASTCALL, nullptr},
+    {"gated_grad", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(gated_grad)), METH_FASTCALL, nullptr},
+    {"input_grad", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(input_grad)), METH_FASTCALL, nullptr},
+    {"store_8bit", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(store_8bit)), METH_FASTCALL, nullptr},
+    {"load_8bit", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(load_8bit)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -526,6 +526,61 @@ eoq_error_t eoq_b200_gemv_polar_codes(const uint8_t *d_codes, const uint16_t *d_
                                       uint32_t batch, void *d_scratch, void *y, int y_dtype, const float *bias,
                                       int tensor_cores, void *stream);
 
+/* The gated feed-forward block on packed weights,
+ *   h = act(x Wg^T + bg) * (x Wu^T + bu),
+ * with its backward pass.  Both weights as QuantizedLinear packs them (core/quantized_linear.py:49-66; 2 and 4 bits packed low
+ * bits first, any other width one signed code per byte), rows x cols each, scales in fp16 over the flattened matrix; biases
+ * NULL or fp32 [rows].  Device pointers. */
+typedef struct eoq_b200_gated {
+    const uint8_t *gate, *up;
+    const uint16_t *gate_scales, *up_scales;
+    const float *gate_bias, *up_bias;
+    uint32_t rows, cols, bits, group;
+    int activation;
+} eoq_b200_gated_t;
+
+#define EOQ_B200_SILU      0
+#define EOQ_B200_GELU      1   /* g P(g), P of the normal distribution */
+#define EOQ_B200_GELU_TANH 2
+
+/* What the forward pass leaves for the backward one: g = x Wg^T + bg and u = x Wu^T + bu, [batch, rows] each, in x's type
+ * (EOQ_B200_KEEP_FULL) or as eoq_b200_store_8bit keeps them (EOQ_B200_KEEP_8BIT: codes, and scales [batch, ceil(rows / 64)]). */
+typedef struct eoq_b200_kept {
+    int form;
+    void *gate, *up;
+    float *gate_scales, *up_scales;
+} eoq_b200_kept_t;
+
+#define EOQ_B200_KEEP_NONE 0
+#define EOQ_B200_KEEP_FULL 1
+#define EOQ_B200_KEEP_8BIT 2
+
+/* x [batch, cols] to h [batch, rows], both of type dtype (EOQ_B200_F16 / BF16 / F32), sums in fp32; kept may be NULL.  d_scratch:
+ * eoq_b200_gated_scratch() bytes, 16-byte aligned (may be NULL where that is 0).  Any shape; 16-byte aligned pointers, whole
+ * groups per row, groups that are multiples of 32 and packed rows that are multiples of 16 bytes take the tensor-core forms.
+ * There (more than eight rows) 16-bit activations go in as fp16, bf16 ones times a power of two per row, which is exact for all
+ * but what is 2^-24 below the row's largest, and code x scale is rounded to fp16 once.  Asynchronous. */
+size_t eoq_b200_gated_scratch(const eoq_b200_gated_t *w, const eoq_b200_kept_t *kept, int dtype, uint32_t batch);
+eoq_error_t eoq_b200_gated_packed(const eoq_b200_gated_t *w, const void *x, int dtype, uint32_t batch, void *d_scratch, void *h,
+                                  const eoq_b200_kept_t *kept, void *stream);
+
+/* The backward pass: dh [batch, rows] to dx [batch, cols] (NULL: not wanted) and to the biases' gradients (NULL, or fp32 [rows]).
+ * The sums over rows have a fixed order: two calls give the same bits. */
+size_t eoq_b200_gated_grad_scratch(const eoq_b200_gated_t *w, const eoq_b200_kept_t *kept, int dtype, uint32_t batch);
+eoq_error_t eoq_b200_gated_grad(const eoq_b200_gated_t *w, const eoq_b200_kept_t *kept, const void *dh, int dtype, uint32_t batch,
+                                void *d_scratch, void *dx, float *d_gate_bias, float *d_up_bias, void *stream);
+
+/* dx = dy W, the gradient that a packed weight passes on: dy [batch, rows], dx [batch, cols], both of type dtype. */
+size_t eoq_b200_packed_input_grad_scratch(uint32_t rows, uint32_t cols, uint32_t bits, uint32_t group, int dtype, uint32_t batch);
+eoq_error_t eoq_b200_packed_input_grad(const uint8_t *d_packed, const uint16_t *d_scales_fp16, uint32_t rows, uint32_t cols, uint32_t bits,
+                                       uint32_t group, const void *dy, int dtype, uint32_t batch, void *d_scratch, void *dx, void *stream);
+
+/* Activations [rows, cols] to 8 bits: blocks of 64 values of a row, code = round(127 x / largest magnitude of the block), half to
+ * even, scale = largest / 127 in fp32, [rows, ceil(cols / 64)].  A block that holds a NaN or an infinity stands for NaN, one whose
+ * largest magnitude is below 1e-30 for zeros.  eoq_b200_load_8bit gives code * scale in any of the three types. */
+eoq_error_t eoq_b200_store_8bit(const void *x, int dtype, size_t rows, uint32_t cols, int8_t *d_codes, float *d_scales, void *stream);
+eoq_error_t eoq_b200_load_8bit(const int8_t *d_codes, const float *d_scales, size_t rows, uint32_t cols, void *y, int dtype, void *stream);
+
 /* Synchronises `stream` and reports whether any kernel that used this weight gave up on a
  * bounded wait for its staged data (EOQ_ERR_CUDA; outputs of that launch are then invalid).
  * The kernels never spin without a limit, so a fault in the copy engine ends in this error
