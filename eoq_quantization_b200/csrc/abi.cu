@@ -2,6 +2,7 @@
 // Host-side validation mirrors the reference's checks and error codes; all
 // decoding runs on the GPU.
 #include "eoq_internal.h"
+#include "gated.h"
 
 #include <algorithm>
 #include <atomic>
@@ -2328,7 +2329,11 @@ extern "C" int eoq_b200_weight_linear_preferred(const eoq_b200_weight_t *w, cons
     return qmm_preferred(c, (double)w->N * w->K / 1.5e6 - 1.0, 0.0) ? 1 : 0;
 }
 
-extern "C" uint32_t eoq_b200_linear_status(void) { return qmm_status(); }
+extern "C" uint32_t eoq_b200_linear_status(void)
+{
+    const uint32_t linear = qmm_status(), gated = gated_status();
+    return linear | gated;
+}
 
 extern "C" eoq_error_t eoq_b200_gemv_polar_codes(const uint8_t *d_codes, const uint16_t *d_norms_fp16, const float *d_centroids,
                                                  uint32_t rows, uint32_t cols, uint32_t bits, uint32_t block, const void *x, int x_dtype,
@@ -2398,7 +2403,7 @@ extern "C" int eoq_b200_tune(const char *key, int value)
     if (std::strcmp(key, "v1_lanes") == 0) { set_v1_lanes(value); return 0; }
     if (std::strcmp(key, "packed_warps") == 0) { set_packed_warps(value); return 0; }
     if (std::strcmp(key, "dequant_vec") == 0) { set_dequant_vec(value); return 0; }
-    if (std::strcmp(key, "qmm_wait_us") == 0) { set_qmm_wait_us(value); return 0; }
+    if (std::strcmp(key, "qmm_wait_us") == 0) { set_qmm_wait_us(value); set_gated_wait_us(value); return 0; }
     if (std::strcmp(key, "pinned_refused") == 0) { g_pinned_refused.store(value); return 0; }
     if (std::strcmp(key, "release_scratch") == 0) { DeviceArena::trim(); PinnedBlock::trim(); return 0; }
     if (std::strcmp(key, "symbols_refused") == 0) { g_symbols_refused.store(value); return 0; }

@@ -57,6 +57,14 @@ int launch_rows_to_half(const void *x, int dtype, uint32_t M, uint32_t K, uint32
 
 // h = act(g) u of fp32 [M][N].
 int launch_gate_apply(const float *g, const float *u, size_t count, int act, void *h, int dtype, void *stream);
+// The tensor-core forms (gated_product.cu): whole groups per row, groups of 32 columns and their multiples, rows of codes that are
+// multiples of 16 bytes, everything 16-byte aligned.  x, dy: fp16, [M][K] and [nw][M][pitch], pitch a multiple of 8.
+bool product_takes(const PackedPair &w, int nw);
+int launch_gated_product(const GatedCall &c, const uint16_t *x, const float *factor, void *stream);
+int launch_input_grad_product(const PackedPair &w, int nw, const uint16_t *dy, uint32_t pitch, const float *factor, uint32_t M, void *dx, int dtype, void *stream);
+uint32_t gated_status();
+void set_gated_wait_us(int v);
+
 int launch_store_8bit(const void *x, int dtype, size_t M, uint32_t N, int8_t *codes, float *scales, void *stream);
 int launch_load_8bit(const int8_t *codes, const float *scales, size_t M, uint32_t N, void *y, int dtype, void *stream);
 

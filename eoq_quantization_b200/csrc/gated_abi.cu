@@ -56,6 +56,12 @@ bool exact_products(const PackedPair &w, int dtype, const void *codes, const voi
     return dtype == EOQ_B200_F32 && qmm_takes(w.K, w.bits, w.group, codes, x) && split_rows_takes(w.K, 1);
 }
 
+// 16-bit activations on the tensor cores: fp16 rows as they are, where copies of them can be aligned; others as fp16 times a
+// power of two a row.
+uint32_t pitch_of(uint32_t n) { return (n + 7u) & ~7u; }
+bool as_it_is(const void *x, int dtype, uint32_t n) { return dtype == EOQ_B200_F16 && n % 8u == 0 && (reinterpret_cast<uintptr_t>(x) & 15u) == 0; }
+size_t half_bytes(uint32_t batch, uint32_t n) { return values(batch, pitch_of(n)) * 2; }
+
 }  // namespace
 }  // namespace eoq
 
@@ -69,6 +75,11 @@ extern "C" size_t eoq_b200_gated_scratch(const eoq_b200_gated_t *w, const eoq_b2
     if (dtype == EOQ_B200_F32) {
         c.take<float>(values(batch, w->cols + 1) * 4);
         if (form != kKeepFull) c.take<float>(2 * values(batch, w->rows) * 4);
+        return c.at;
+    }
+    if (product_takes(pair_of(w), 2)) {
+        c.take<void>(half_bytes(batch, w->cols));
+        c.take<float>((size_t)batch * 4);
     } else if (form == kKeep8bit) {
         c.take<float>(2 * values(batch, w->rows) * 4);
     }
@@ -91,6 +102,18 @@ extern "C" eoq_error_t eoq_b200_gated_packed(const eoq_b200_gated_t *w, const vo
     Carve scratch{static_cast<uint8_t *>(d_scratch)};
     const size_t n = values(batch, w->rows);
     int e = 0;
+    if (dtype != EOQ_B200_F32 && product_takes(c.w, 2)) {
+        uint16_t *half = scratch.take<uint16_t>(half_bytes(batch, w->cols));
+        float *factor = scratch.take<float>((size_t)batch * 4);
+        if (as_it_is(x, dtype, w->cols)) {
+            half = static_cast<uint16_t *>(const_cast<void *>(x));
+            factor = nullptr;
+        } else {
+            e = launch_rows_to_half(x, dtype, batch, w->cols, pitch_of(w->cols), half, factor, stream);
+        }
+        if (e == 0) e = launch_gated_product(c, half, factor, stream);
+        return launched(e, where);
+    }
     if (exact_products(c.w, dtype, w->gate, d_scratch) && exact_products(c.w, dtype, w->up, d_scratch)) {
         void *planes = scratch.take<void>(values(batch, w->cols + 1) * 4);
         float *factors = reinterpret_cast<float *>(static_cast<uint8_t *>(planes) + values(batch, w->cols) * 4);
@@ -126,8 +149,13 @@ extern "C" eoq_error_t eoq_b200_gated_packed(const eoq_b200_gated_t *w, const vo
 extern "C" size_t eoq_b200_gated_grad_scratch(const eoq_b200_gated_t *w, const eoq_b200_kept_t *, int dtype, uint32_t batch)
 {
     if (!w || !fine(w->rows, w->cols, w->bits, w->group)) return 0;
-    (void)dtype;
     Carve c{nullptr};
+    if (dtype != EOQ_B200_F32 && product_takes(pair_of(w), 2)) {
+        c.take<void>(2 * half_bytes(batch, w->rows));
+        c.take<float>((size_t)batch * 4);
+        c.take<void>(column_sums_scratch(batch, w->rows));
+        return c.at;
+    }
     c.take<float>(2 * values(batch, w->rows) * 4);
     c.take<void>(std::max(column_sums_scratch(batch, w->rows), input_grad_general_scratch(pair_of(w), batch)));
     return c.at;
@@ -145,26 +173,38 @@ extern "C" eoq_error_t eoq_b200_gated_grad(const eoq_b200_gated_t *w, const eoq_
     const size_t n = values(batch, w->rows);
     const PackedPair pair = pair_of(w);
     Carve scratch{static_cast<uint8_t *>(d_scratch)};
+    const char *where = "eoq_b200_gated_grad";
+    float *to[2] = {d_gate_bias, d_up_bias};
+    if (dtype != EOQ_B200_F32 && product_takes(pair, 2)) {
+        const uint32_t pitch = pitch_of(w->rows);
+        uint16_t *half = scratch.take<uint16_t>(2 * half_bytes(batch, w->rows));
+        float *factor = scratch.take<float>((size_t)batch * 4), *sums = scratch.take<float>(0);
+        int e = launch_gate_grad(kept_of(kept), dh, dtype, w->activation, batch, w->rows, nullptr, half, pitch, factor, stream);
+        if (e == 0 && (d_gate_bias || d_up_bias)) e = launch_column_sums(nullptr, half, pitch, factor, batch, w->rows, sums, to, stream);
+        if (e == 0 && dx) e = launch_input_grad_product(pair, 2, half, pitch, factor, batch, dx, dtype, stream);
+        return launched(e, where);
+    }
     float *d = scratch.take<float>(2 * n * 4), *out[2] = {d, d + n};
     void *sums = scratch.take<void>(0);
     int e = launch_gate_grad(kept_of(kept), dh, dtype, w->activation, batch, w->rows, out, nullptr, 0, nullptr, stream);
-    if (e == 0 && (d_gate_bias || d_up_bias)) {
-        float *to[2] = {d_gate_bias, d_up_bias};
-        e = launch_column_sums(out, nullptr, 0, nullptr, batch, w->rows, static_cast<float *>(sums), to, stream);
-    }
+    if (e == 0 && (d_gate_bias || d_up_bias)) e = launch_column_sums(out, nullptr, 0, nullptr, batch, w->rows, static_cast<float *>(sums), to, stream);
     if (e == 0 && dx) {
         const void *dy[2] = {out[0], out[1]};
         e = launch_input_grad_general(pair, 2, dy, EOQ_B200_F32, batch, sums, dx, dtype, stream);
     }
-    return launched(e, "eoq_b200_gated_grad");
+    return launched(e, where);
 }
 
 extern "C" size_t eoq_b200_packed_input_grad_scratch(uint32_t rows, uint32_t cols, uint32_t bits, uint32_t group, int dtype, uint32_t batch)
 {
     if (!fine(rows, cols, bits, group)) return 0;
-    (void)dtype;
-    PackedPair p = {{nullptr, nullptr}, {nullptr, nullptr}, rows, cols, bits, group, row_bytes(cols, bits)};
-    return input_grad_general_scratch(p, batch);
+    const PackedPair p = {{nullptr, nullptr}, {nullptr, nullptr}, rows, cols, bits, group, row_bytes(cols, bits)};
+    const size_t any = input_grad_general_scratch(p, batch);        // (codes that are not aligned)
+    if (dtype == EOQ_B200_F32 || !product_takes(p, 1)) return any;
+    Carve c{nullptr};
+    c.take<void>(half_bytes(batch, rows));
+    c.take<float>((size_t)batch * 4);
+    return std::max(c.at, any);
 }
 
 extern "C" eoq_error_t eoq_b200_packed_input_grad(const uint8_t *d_packed, const uint16_t *d_scales_fp16, uint32_t rows, uint32_t cols, uint32_t bits,
@@ -176,6 +216,20 @@ extern "C" eoq_error_t eoq_b200_packed_input_grad(const uint8_t *d_packed, const
     if (!fine(rows, cols, bits, group)) return EOQ_ERR_INVALID_HEADER;
     if (!have_device()) return EOQ_ERR_CUDA;
     const PackedPair p = {{d_packed, d_packed}, {d_scales_fp16, d_scales_fp16}, rows, cols, bits, group, row_bytes(cols, bits)};
+    if (dtype != EOQ_B200_F32 && product_takes(p, 1)) {
+        Carve scratch{static_cast<uint8_t *>(d_scratch)};
+        uint16_t *half = scratch.take<uint16_t>(half_bytes(batch, rows));
+        float *factor = scratch.take<float>((size_t)batch * 4);
+        int e = 0;
+        if (as_it_is(dy, dtype, rows)) {
+            half = static_cast<uint16_t *>(const_cast<void *>(dy));
+            factor = nullptr;
+        } else {
+            e = launch_rows_to_half(dy, dtype, batch, rows, pitch_of(rows), half, factor, stream);
+        }
+        if (e == 0) e = launch_input_grad_product(p, 1, half, pitch_of(rows), factor, batch, dx, dtype, stream);
+        return launched(e, "eoq_b200_packed_input_grad");
+    }
     const void *d[2] = {dy, dy};
     return launched(launch_input_grad_general(p, 1, d, dtype, batch, d_scratch, dx, dtype, stream), "eoq_b200_packed_input_grad");
 }

@@ -746,32 +746,6 @@ void set_qmm_wait_us(int v) { g_qmm_limit.store(std::min(std::max(v, 0), 6000000
 
 namespace {
 
-// CTAs of a kernel in clusters of `split` that fit on the device at once, asked once per kernel, size and shared memory.
-uint32_t resident_ctas(const void *kern, uint32_t threads, size_t smem, uint32_t split)
-{
-    struct Known { const void *k; size_t smem; uint32_t split; int dev; uint32_t n; };
-    static std::mutex mu;
-    static std::vector<Known> known;
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-    std::lock_guard<std::mutex> lock(mu);
-    for (const Known &k : known) if (k.k == kern && k.smem == smem && k.split == split && k.dev == dev) return k.n;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(split);
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = split; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    int n = 0;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess ||
-        cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) { (void)cudaGetLastError(); n = 0; }
-    known.push_back(Known{kern, smem, split, dev, (uint32_t)std::max(n, 0) * split});
-    return known.back().n;
-}
-
 struct Shape { uint32_t T, nw, ns, nd, a_base; size_t smem; uint32_t at_x, at_bar; };
 
 // Stages and shared memory of a kernel variant for a token tile T.  A producer set has to come by every stage on every lap

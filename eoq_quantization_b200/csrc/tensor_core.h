@@ -7,6 +7,9 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <algorithm>
+#include <mutex>
+#include <vector>
 
 namespace eoq {
 namespace {
@@ -217,6 +220,32 @@ bool map_2d(CUtensorMap &m, CUtensorMapDataType type, const void *p, uint64_t in
     EncodeFn fn = encode_fn();
     return fn && fn(&m, type, 2, const_cast<void *>(p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
                     CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// CTAs of a kernel in clusters of `split` that fit on the device at once, asked once per kernel, size and shared memory.
+uint32_t resident_ctas(const void *kern, uint32_t threads, size_t smem, uint32_t split)
+{
+    struct Known { const void *k; size_t smem; uint32_t split; int dev; uint32_t n; };
+    static std::mutex mu;
+    static std::vector<Known> known;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+    std::lock_guard<std::mutex> lock(mu);
+    for (const Known &k : known) if (k.k == kern && k.smem == smem && k.split == split && k.dev == dev) return k.n;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(split);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = split; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) { (void)cudaGetLastError(); n = 0; }
+    known.push_back(Known{kern, smem, split, dev, (uint32_t)std::max(n, 0) * split});
+    return known.back().n;
 }
 
 }  // namespace
