@@ -3,6 +3,8 @@
 #include "gated.h"
 
 #include <algorithm>
+#include <type_traits>
+
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -23,6 +25,65 @@ __device__ __forceinline__ void store_from_float(void *p, size_t i, float v, int
     if (dtype == EOQ_B200_F32) reinterpret_cast<float *>(p)[i] = v;
     else if (dtype == EOQ_B200_F16) reinterpret_cast<__half *>(p)[i] = __float2half_rn(v);
     else reinterpret_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(v);
+}
+
+// Eight values in a row of a type, as they lie in memory: four words, or eight.
+template <int DTYPE> struct Raw8 { uint4 v[DTYPE == EOQ_B200_F32 ? 2 : 1]; };
+
+template <int DTYPE>
+__device__ __forceinline__ Raw8<DTYPE> load8(const void *p, size_t i)
+{
+    Raw8<DTYPE> r;
+    const uint4 *at = reinterpret_cast<const uint4 *>(reinterpret_cast<const uint8_t *>(p) + i * (DTYPE == EOQ_B200_F32 ? 4 : 2));
+    r.v[0] = __ldg(at);
+    if constexpr (DTYPE == EOQ_B200_F32) r.v[1] = __ldg(at + 1);
+    return r;
+}
+__device__ __forceinline__ float2 pair_of(uint32_t w, bool half)
+{
+    if (half) return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+template <int DTYPE>
+__device__ __forceinline__ void values_of(const Raw8<DTYPE> &r, float (&f)[8])
+{
+    const uint32_t w[4] = {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w};
+    if constexpr (DTYPE == EOQ_B200_F32) {
+        const uint32_t u[4] = {r.v[1].x, r.v[1].y, r.v[1].z, r.v[1].w};
+#pragma unroll
+        for (int j = 0; j < 4; j++) { f[j] = __uint_as_float(w[j]); f[4 + j] = __uint_as_float(u[j]); }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++) { const float2 p = pair_of(w[j], DTYPE == EOQ_B200_F16); f[2 * j] = p.x; f[2 * j + 1] = p.y; }
+    }
+}
+__device__ __forceinline__ uint32_t half_pair(float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t *>(&h); }
+__device__ __forceinline__ uint32_t bf16_pair(float a, float b) { const __nv_bfloat162 h = __floats2bfloat162_rn(a, b); return *reinterpret_cast<const uint32_t *>(&h); }
+template <int DTYPE>
+__device__ __forceinline__ void store8(void *p, size_t i, const float (&f)[8])
+{
+    uint4 *at = reinterpret_cast<uint4 *>(reinterpret_cast<uint8_t *>(p) + i * (DTYPE == EOQ_B200_F32 ? 4 : 2));
+    if constexpr (DTYPE == EOQ_B200_F32) {
+        at[0] = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+        at[1] = make_uint4(__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]), __float_as_uint(f[7]));
+    } else if constexpr (DTYPE == EOQ_B200_F16) {
+        at[0] = make_uint4(half_pair(f[0], f[1]), half_pair(f[2], f[3]), half_pair(f[4], f[5]), half_pair(f[6], f[7]));
+    } else {
+        at[0] = make_uint4(bf16_pair(f[0], f[1]), bf16_pair(f[2], f[3]), bf16_pair(f[4], f[5]), bf16_pair(f[6], f[7]));
+    }
+}
+
+// The largest value of a CTA's threads, in all of them.
+__device__ __forceinline__ float largest_of(float v, float *part)
+{
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
+    if ((threadIdx.x & 31u) == 0) part[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = 0.0f;
+    for (uint32_t w = 0; w < blockDim.x / 32u; w++) v = fmaxf(v, part[w]);
+    __syncthreads();
+    return v;
 }
 
 // Weight (n, k) in fp32: any width and any group of the flattened matrix, rows that end inside a group among them.
@@ -203,7 +264,6 @@ __device__ __forceinline__ void kept_at(const GateGradArgs &a, uint32_t m, uint3
 __global__ void __launch_bounds__(512) gate_grad_kernel(const GateGradArgs a)
 {
     __shared__ float part[16];
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
     for (uint32_t m = blockIdx.x; m < a.M; m += gridDim.x) {
         auto at = [&](uint32_t n, float &dg, float &du) {
             float g, u, act, slope;
@@ -228,14 +288,7 @@ __global__ void __launch_bounds__(512) gate_grad_kernel(const GateGradArgs a)
             at(n, dg, du);
             most = fmaxf(most, fmaxf(finite_magnitude(dg), finite_magnitude(du)));
         }
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-        if (lane == 0) part[warp] = most;
-        __syncthreads();
-        most = 0.0f;
-        for (uint32_t w = 0; w < blockDim.x / 32u; w++) most = fmaxf(most, part[w]);
-        __syncthreads();
-        const int e = half_exponent(most);
+        const int e = half_exponent(largest_of(most, part));
         const float up = power_of_two(e);
         if (threadIdx.x == 0) a.factor[m] = power_of_two(-e);
         for (uint32_t n = threadIdx.x; n < a.pitch; n += blockDim.x) {
@@ -253,6 +306,82 @@ __global__ void __launch_bounds__(256) gate_apply_kernel(const float *__restrict
         store_from_float(h, i, activation(g[i], act) * u[i], dtype);
 }
 
+// The same to fp16 where rows are multiples of eight values and aligned: a row's inputs are read once and stay in registers, as they
+// came (KEEP8: with their scales), eight values a thread ROUNDS times.  The row's power of two comes from a bound of its largest
+// gradient that takes no exponential, |dh| max(1.13 |u|, |g|): a slope is below 1.13 in magnitude and |act(g)| is at most |g|.  It
+// can be some bits above the largest, of which fp16 has enough (a row's largest is at 2^14, the smallest normal number at 2^-14).
+template <int DTYPE, bool KEEP8, int ROUNDS>
+__global__ void __launch_bounds__(512) gate_grad_rows_kernel(const GateGradArgs a)
+{
+    __shared__ float part[16];
+    struct Kept8 { uint2 v; float s; };
+    struct Kept16 { Raw8<DTYPE> v; };
+    using K = std::conditional_t<KEEP8, Kept8, Kept16>;
+    auto load_kept = [&](int which, size_t m, uint32_t n) {
+        K k;
+        if constexpr (KEEP8) {
+            k.v = __ldg(reinterpret_cast<const uint2 *>(reinterpret_cast<const int8_t *>(a.k.v[which]) + m * a.N + n));
+            k.s = __ldg(a.k.scale[which] + m * ((a.N + kStoreBlock - 1) / kStoreBlock) + n / kStoreBlock);
+        } else {
+            k.v = load8<DTYPE>(a.k.v[which], m * a.N + n);
+        }
+        return k;
+    };
+    auto kept_values = [&](const K &k, float (&f)[8]) {
+        if constexpr (KEEP8) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) f[j] = (float)(int8_t)((j < 4 ? k.v.x : k.v.y) >> (8 * (j & 3))) * k.s;
+        } else {
+            values_of<DTYPE>(k.v, f);
+        }
+    };
+    for (uint32_t m = blockIdx.x; m < a.M; m += gridDim.x) {
+        Raw8<DTYPE> rd[ROUNDS];
+        K rg[ROUNDS], ru[ROUNDS];
+        float most = 0.0f;
+#pragma unroll
+        for (int r = 0; r < ROUNDS; r++) {
+            const uint32_t n = (r * 512u + threadIdx.x) * 8u;
+            if (n >= a.N) continue;
+            rd[r] = load8<DTYPE>(a.dh, (size_t)m * a.N + n);
+            rg[r] = load_kept(0, m, n);
+            ru[r] = load_kept(1, m, n);
+        }
+#pragma unroll
+        for (int r = 0; r < ROUNDS; r++) {
+            const uint32_t n = (r * 512u + threadIdx.x) * 8u;
+            if (n >= a.N) continue;
+            float d[8], g[8], u[8];
+            values_of<DTYPE>(rd[r], d);
+            kept_values(rg[r], g);
+            kept_values(ru[r], u);
+#pragma unroll
+            for (int j = 0; j < 8; j++) most = fmaxf(most, finite_magnitude(d[j] * fmaxf(1.13f * fabsf(u[j]), fabsf(g[j]))));
+        }
+        const int e = half_exponent(largest_of(most, part));
+        const float up = power_of_two(e);
+        if (threadIdx.x == 0) a.factor[m] = power_of_two(-e);
+#pragma unroll
+        for (int r = 0; r < ROUNDS; r++) {
+            const uint32_t n = (r * 512u + threadIdx.x) * 8u;
+            if (n >= a.N) continue;
+            float d[8], g[8], u[8];
+            values_of<DTYPE>(rd[r], d);
+            kept_values(rg[r], g);
+            kept_values(ru[r], u);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                float value, slope;
+                activation_and_slope(g[j], a.act, value, slope);
+                g[j] = d[j] * u[j] * slope * up;
+                u[j] = d[j] * value * up;
+            }
+            store8<EOQ_B200_F16>(a.half, (size_t)m * a.pitch + n, g);
+            store8<EOQ_B200_F16>(a.half, ((size_t)a.M + m) * a.pitch + n, u);
+        }
+    }
+}
+
 // Sums over the rows in two steps, so that their order is fixed: 256 rows a CTA and column, then the parts in order.
 constexpr uint32_t kSumRows = 256;
 
@@ -267,19 +396,32 @@ struct SumArgs {
 
 __global__ void __launch_bounds__(256) column_parts_kernel(const SumArgs a)
 {
-    __shared__ float sums[8][32];
-    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, n = blockIdx.x * 32u + lane, which = blockIdx.z;
+    __shared__ float2 sums[8][32];
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, n = blockIdx.x * 64u + lane * 2u, which = blockIdx.z;
     for (uint32_t chunk = blockIdx.y; chunk < a.chunks; chunk += gridDim.y) {
-        float v = 0.0f;
+        float2 v = make_float2(0.0f, 0.0f);
         const uint32_t last = min(a.M, (chunk + 1) * kSumRows);
-        if (n < a.N)
-            for (uint32_t m = chunk * kSumRows + warp; m < last; m += 8u)
-                v += a.half ? __half2float(a.half[((size_t)which * a.M + m) * a.pitch + n]) * __ldg(a.factor + m) : a.in32[which][(size_t)m * a.N + n];
+        if (n < a.N) {
+#pragma unroll 4
+            for (uint32_t m = chunk * kSumRows + warp; m < last; m += 8u) {
+                if (a.half) {              // (rows are padded to eight)
+                    const float f = __ldg(a.factor + m);
+                    const float2 p = __half22float2(*reinterpret_cast<const __half2 *>(a.half + ((size_t)which * a.M + m) * a.pitch + n));
+                    v.x = fmaf(p.x, f, v.x);
+                    v.y = fmaf(p.y, f, v.y);
+                } else {
+                    v.x += a.in32[which][(size_t)m * a.N + n];
+                    if (n + 1 < a.N) v.y += a.in32[which][(size_t)m * a.N + n + 1];
+                }
+            }
+        }
         sums[warp][lane] = v;
         __syncthreads();
         if (warp == 0 && n < a.N) {
-            for (int w = 1; w < 8; w++) v += sums[w][lane];
-            a.part[((size_t)chunk * 2 + which) * a.N + n] = v;
+            for (int w = 1; w < 8; w++) { v.x += sums[w][lane].x; v.y += sums[w][lane].y; }
+            float *to = a.part + ((size_t)chunk * 2 + which) * a.N + n;
+            to[0] = v.x;
+            if (n + 1 < a.N) to[1] = v.y;
         }
         __syncthreads();
     }
@@ -294,22 +436,53 @@ __global__ void __launch_bounds__(256) column_sums_kernel(const SumArgs a)
     a.out[which][n] = v;
 }
 
+// bf16 or fp16 rows of multiples of eight values, aligned: read once, kept in registers.
+template <int DTYPE, int ROUNDS>
+__global__ void __launch_bounds__(256) rows_to_half_vector_kernel(const void *__restrict__ x, uint32_t M, uint32_t K, __half *__restrict__ out, float *__restrict__ factor)
+{
+    __shared__ float part[8];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    for (uint32_t m = blockIdx.x; m < M; m += gridDim.x) {
+        Raw8<DTYPE> raw[ROUNDS];
+        float most = 0.0f;
+#pragma unroll
+        for (int r = 0; r < ROUNDS; r++) {
+            const uint32_t k = (r * 256u + threadIdx.x) * 8u;
+            if (k < K) raw[r] = load8<DTYPE>(x, (size_t)m * K + k);
+        }
+#pragma unroll
+        for (int r = 0; r < ROUNDS; r++) {
+            float f[8];
+            if ((r * 256u + threadIdx.x) * 8u >= K) continue;
+            values_of<DTYPE>(raw[r], f);
+#pragma unroll
+            for (int j = 0; j < 8; j++) most = fmaxf(most, finite_magnitude(f[j]));
+        }
+        const int e = half_exponent(largest_of(most, part));
+        const float up = power_of_two(e);
+        if (threadIdx.x == 0) factor[m] = power_of_two(-e);
+#pragma unroll
+        for (int r = 0; r < ROUNDS; r++) {
+            const uint32_t k = (r * 256u + threadIdx.x) * 8u;
+            if (k >= K) continue;
+            float f[8];
+            values_of<DTYPE>(raw[r], f);
+#pragma unroll
+            for (int j = 0; j < 8; j++) f[j] *= up;
+            store8<EOQ_B200_F16>(out, (size_t)m * K + k, f);
+        }
+    }
+}
+
 __global__ void __launch_bounds__(256) rows_to_half_kernel(const void *__restrict__ x, int dtype, uint32_t M, uint32_t K, uint32_t pitch, __half *__restrict__ out,
                                                            float *__restrict__ factor)
 {
     __shared__ float part[8];
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
     for (uint32_t m = blockIdx.x; m < M; m += gridDim.x) {
         float most = 0.0f;
         for (uint32_t k = threadIdx.x; k < K; k += 256u) most = fmaxf(most, finite_magnitude(load_as_float(x, (size_t)m * K + k, dtype)));
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-        if (lane == 0) part[warp] = most;
-        __syncthreads();
-        most = 0.0f;
-        for (uint32_t w = 0; w < 8; w++) most = fmaxf(most, part[w]);
-        __syncthreads();
-        const int e = half_exponent(most);
+        const int e = half_exponent(largest_of(most, part));
         const float up = power_of_two(e);
         if (threadIdx.x == 0) factor[m] = power_of_two(-e);
         for (uint32_t k = threadIdx.x; k < pitch; k += 256u)
@@ -323,46 +496,71 @@ __global__ void __launch_bounds__(256) rows_to_half_kernel(const void *__restric
 // lanes each, eight values a lane.  A block that holds a NaN or an infinity stands for NaN throughout, so that it shows; one
 // whose largest is below 1e-30 for zeros (127 / largest would be infinite at 3.7e-37).  Bound by HBM.
 // ---------------------------------------------------------------------------
-__global__ void __launch_bounds__(256) store_8bit_kernel(const void *__restrict__ x, int dtype, size_t blocks, uint32_t N, int8_t *__restrict__ codes,
-                                                         float *__restrict__ scales)
+// VEC: rows are multiples of eight values and 16-byte aligned, a lane's eight lie together; else they are eight apart.
+template <int DTYPE, bool VEC>
+__global__ void __launch_bounds__(256) store_8bit_kernel(const void *__restrict__ x, size_t blocks, uint32_t N, int8_t *__restrict__ codes, float *__restrict__ scales)
 {
     const uint32_t per_row = (N + kStoreBlock - 1) / kStoreBlock, lane8 = threadIdx.x & 7u;
     for (size_t b0 = ((size_t)blockIdx.x * 256u + (threadIdx.x & ~31u)) / 8u; b0 < blocks; b0 += (size_t)gridDim.x * 32u) {
         const size_t b = b0 + ((threadIdx.x & 31u) >> 3);
         const bool here = b < blocks;
-        const size_t m = here ? b / per_row : 0;
-        const uint32_t n0 = here ? (uint32_t)(b - m * per_row) * kStoreBlock + lane8 * 8u : N;
-        float v[8];
+        const size_t m = !here ? 0 : blocks <= 0xffffffffu ? (uint32_t)b / per_row : b / per_row;
+        const uint32_t first = here ? (uint32_t)(b - m * per_row) * kStoreBlock : N;
+        float v[8] = {};
+        if constexpr (VEC) {
+            if (first + lane8 * 8u < N) values_of<DTYPE>(load8<DTYPE>(x, m * N + first + lane8 * 8u), v);
+        } else {
+#pragma unroll
+            for (uint32_t j = 0; j < 8; j++) if (first + j * 8u + lane8 < N) v[j] = load_as_float(x, m * N + first + j * 8u + lane8, DTYPE);
+        }
         uint32_t most = 0u;
 #pragma unroll
-        for (uint32_t j = 0; j < 8; j++) {
-            v[j] = n0 + j < N ? load_as_float(x, m * N + n0 + j, dtype) : 0.0f;
-            most = max(most, __float_as_uint(v[j]) & 0x7fffffffu);      // as whole numbers: infinity and then NaN are the largest
-        }
+        for (uint32_t j = 0; j < 8; j++) most = max(most, __float_as_uint(v[j]) & 0x7fffffffu);      // as whole numbers: infinity and then NaN are the largest
 #pragma unroll
         for (int d = 4; d > 0; d >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
         const Storer to(most);
         if (!here) continue;
         if (lane8 == 0) scales[b] = to.scale;
+        if constexpr (VEC) {
+            if (first + lane8 * 8u >= N) continue;
+            uint32_t p[2] = {0u, 0u};
 #pragma unroll
-        for (uint32_t j = 0; j < 8; j++)
-            if (n0 + j < N) codes[m * N + n0 + j] = to.code(v[j]);
+            for (int j = 0; j < 8; j++) p[j >> 2] |= (uint32_t)(uint8_t)to.code(v[j]) << (8 * (j & 3));
+            *reinterpret_cast<uint2 *>(codes + m * N + first + lane8 * 8u) = make_uint2(p[0], p[1]);
+        } else {
+#pragma unroll
+            for (uint32_t j = 0; j < 8; j++) if (first + j * 8u + lane8 < N) codes[m * N + first + j * 8u + lane8] = to.code(v[j]);
+        }
     }
 }
 
-__global__ void __launch_bounds__(256) load_8bit_kernel(const int8_t *__restrict__ codes, const float *__restrict__ scales, size_t M, uint32_t N, void *__restrict__ y, int dtype)
+// VEC: eight values a thread (a row's eights are whole and lie in one block).
+template <int DTYPE, bool VEC>
+__global__ void __launch_bounds__(256) load_8bit_kernel(const int8_t *__restrict__ codes, const float *__restrict__ scales, size_t M, uint32_t N, void *__restrict__ y)
 {
-    const uint32_t per_row = (N + kStoreBlock - 1) / kStoreBlock;
-    for (size_t i = (size_t)blockIdx.x * 256u + threadIdx.x; i < M * N; i += (size_t)gridDim.x * 256u) {
-        const size_t m = i / N;
-        const uint32_t n = (uint32_t)(i - m * N);
-        store_from_float(y, i, (float)codes[i] * scales[m * per_row + n / kStoreBlock], dtype);
+    const uint32_t per_row = (N + kStoreBlock - 1) / kStoreBlock, width = VEC ? N / 8u : N;
+    const size_t count = M * width;
+    for (size_t i = (size_t)blockIdx.x * 256u + threadIdx.x; i < count; i += (size_t)gridDim.x * 256u) {
+        const size_t m = count <= 0xffffffffu ? (uint32_t)i / width : i / width;
+        const uint32_t n = (uint32_t)(i - m * width) * (VEC ? 8u : 1u);
+        const float s = __ldg(scales + m * per_row + n / kStoreBlock);
+        if constexpr (VEC) {
+            const uint2 w = __ldg(reinterpret_cast<const uint2 *>(codes) + i);
+            float f[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) f[j] = (float)(int8_t)((j < 4 ? w.x : w.y) >> (8 * (j & 3))) * s;
+            store8<DTYPE>(y, i * 8u, f);
+        } else {
+            store_from_float(y, i, (float)codes[i] * s, DTYPE);
+        }
     }
 }
 
 uint32_t ctas_for(size_t work, uint32_t per) { return (uint32_t)std::min<size_t>((work + per - 1) / per, (size_t)device_sm_count() * 16u); }
 
 }  // namespace
+
+static bool aligned(const void *p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
 int launch_gated_general(const GatedCall &c, void *stream)
 {
@@ -400,7 +598,17 @@ int launch_gate_grad(const Kept &k, const void *dh, int dtype, int act, uint32_t
                      void *stream)
 {
     GateGradArgs a = {k, dh, {out32 ? out32[0] : nullptr, out32 ? out32[1] : nullptr}, (__half *)half, factor, M, N, pitch, dtype, act};
-    gate_grad_kernel<<<std::min(M, 65535u), 512, 0, (cudaStream_t)stream>>>(a);
+    const bool k8 = k.form == kKeep8bit;
+    if (half && dtype != EOQ_B200_F32 && N % 8u == 0 && pitch == N && N <= 7u * 4096u && aligned(dh, 16) && aligned(k.v[0], 16) && aligned(k.v[1], 16) && aligned(half, 16)) {
+#define EOQ_GATE(D, R) (k8 ? gate_grad_rows_kernel<D, true, R> : gate_grad_rows_kernel<D, false, R>)
+#define EOQ_GATE_ROUNDS(D) (N <= 4096u ? EOQ_GATE(D, 1) : N <= 12288u ? EOQ_GATE(D, 3) : EOQ_GATE(D, 7))
+        auto kern = dtype == EOQ_B200_F16 ? EOQ_GATE_ROUNDS(EOQ_B200_F16) : EOQ_GATE_ROUNDS(EOQ_B200_BF16);
+#undef EOQ_GATE_ROUNDS
+#undef EOQ_GATE
+        kern<<<std::min(M, 65535u), N <= 4096u ? (N / 8u + 31u) / 32u * 32u : 512u, 0, (cudaStream_t)stream>>>(a);
+    } else {
+        gate_grad_kernel<<<std::min(M, 65535u), 512, 0, (cudaStream_t)stream>>>(a);
+    }
     count_launch();
     return (int)cudaGetLastError();
 }
@@ -413,7 +621,7 @@ int launch_column_sums(const float *const in32[2], const uint16_t *half, uint32_
 {
     cudaStream_t st = (cudaStream_t)stream;
     SumArgs a = {{in32 ? in32[0] : nullptr, in32 ? in32[1] : nullptr}, (const __half *)half, factor, scratch, {out[0], out[1]}, M, N, pitch, sum_chunks(M)};
-    column_parts_kernel<<<dim3((N + 31u) / 32u, std::min(a.chunks, 65535u), 2), 256, 0, st>>>(a);
+    column_parts_kernel<<<dim3((N + 63u) / 64u, std::min(a.chunks, 65535u), 2), 256, 0, st>>>(a);
     count_launch();
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return (int)e;
@@ -424,6 +632,23 @@ int launch_column_sums(const float *const in32[2], const uint16_t *half, uint32_
 
 int launch_rows_to_half(const void *x, int dtype, uint32_t M, uint32_t K, uint32_t pitch, uint16_t *out, float *factor, void *stream)
 {
+    if (dtype != EOQ_B200_F32 && K % 8u == 0 && pitch == K && K <= 16384u && aligned(x, 16)) {
+#define EOQ_ROWS(D) (K <= 2048u ? rows_to_half_vector_kernel<D, 1> : K <= 4096u ? rows_to_half_vector_kernel<D, 2> : rows_to_half_vector_kernel<D, 8>)
+        auto kern = dtype == EOQ_B200_F16 ? EOQ_ROWS(EOQ_B200_F16) : EOQ_ROWS(EOQ_B200_BF16);
+#undef EOQ_ROWS
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(std::min(M, 65535u));
+        cfg.blockDim = dim3(256);
+        cfg.stream = (cudaStream_t)stream;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = programmatic_launches();
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, x, M, K, (__half *)out, factor);
+        count_launch();
+        return (int)(e != cudaSuccess ? e : cudaGetLastError());
+    }
     rows_to_half_kernel<<<std::min(M, 65535u), 256, 0, (cudaStream_t)stream>>>(x, dtype, M, K, pitch, (__half *)out, factor);
     count_launch();
     return (int)cudaGetLastError();
@@ -432,14 +657,22 @@ int launch_rows_to_half(const void *x, int dtype, uint32_t M, uint32_t K, uint32
 int launch_store_8bit(const void *x, int dtype, size_t M, uint32_t N, int8_t *codes, float *scales, void *stream)
 {
     const size_t blocks = M * ((N + kStoreBlock - 1) / kStoreBlock);
-    store_8bit_kernel<<<ctas_for(blocks, 32u), 256, 0, (cudaStream_t)stream>>>(x, dtype, blocks, N, codes, scales);
+    const bool vec = N % 8u == 0 && aligned(x, 16) && aligned(codes, 8);
+    auto kern = dtype == EOQ_B200_F32 ? (vec ? store_8bit_kernel<EOQ_B200_F32, true> : store_8bit_kernel<EOQ_B200_F32, false>)
+              : dtype == EOQ_B200_F16 ? (vec ? store_8bit_kernel<EOQ_B200_F16, true> : store_8bit_kernel<EOQ_B200_F16, false>)
+                                      : (vec ? store_8bit_kernel<EOQ_B200_BF16, true> : store_8bit_kernel<EOQ_B200_BF16, false>);
+    kern<<<ctas_for(blocks, 32u), 256, 0, (cudaStream_t)stream>>>(x, blocks, N, codes, scales);
     count_launch();
     return (int)cudaGetLastError();
 }
 
 int launch_load_8bit(const int8_t *codes, const float *scales, size_t M, uint32_t N, void *y, int dtype, void *stream)
 {
-    load_8bit_kernel<<<ctas_for(M * N, 256u), 256, 0, (cudaStream_t)stream>>>(codes, scales, M, N, y, dtype);
+    const bool vec = N % 8u == 0 && aligned(y, 16) && aligned(codes, 8);
+    auto kern = dtype == EOQ_B200_F32 ? (vec ? load_8bit_kernel<EOQ_B200_F32, true> : load_8bit_kernel<EOQ_B200_F32, false>)
+              : dtype == EOQ_B200_F16 ? (vec ? load_8bit_kernel<EOQ_B200_F16, true> : load_8bit_kernel<EOQ_B200_F16, false>)
+                                      : (vec ? load_8bit_kernel<EOQ_B200_BF16, true> : load_8bit_kernel<EOQ_B200_BF16, false>);
+    kern<<<ctas_for(M * (vec ? N / 8u : N), 256u), 256, 0, (cudaStream_t)stream>>>(codes, scales, M, N, y);
     count_launch();
     return (int)cudaGetLastError();
 }

@@ -62,6 +62,10 @@ int launch_gate_apply(const float *g, const float *u, size_t count, int act, voi
 bool product_takes(const PackedPair &w, int nw);
 int launch_gated_product(const GatedCall &c, const uint16_t *x, const float *factor, void *stream);
 int launch_input_grad_product(const PackedPair &w, int nw, const uint16_t *dy, uint32_t pitch, const float *factor, uint32_t M, void *dx, int dtype, void *stream);
+// Up to eight rows of 16-bit activations, 16-byte aligned; kept in full or in fp32 (gated_rows.cu).
+bool gated_rows_takes(const PackedPair &w, uint32_t batch);
+int launch_gated_rows(const GatedCall &c, void *stream);
+void set_gated_rows(int warps, int ctas);
 uint32_t gated_status();
 void set_gated_wait_us(int v);
 

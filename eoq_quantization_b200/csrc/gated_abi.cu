@@ -56,6 +56,9 @@ bool exact_products(const PackedPair &w, int dtype, const void *codes, const voi
     return dtype == EOQ_B200_F32 && qmm_takes(w.K, w.bits, w.group, codes, x) && split_rows_takes(w.K, 1);
 }
 
+// Up to eight rows of 16-bit activations: one pass over the codes.
+bool few_rows(const PackedPair &w, int dtype, uint32_t batch) { return dtype != EOQ_B200_F32 && gated_rows_takes(w, batch); }
+
 // 16-bit activations on the tensor cores: fp16 rows as they are, where copies of them can be aligned; others as fp16 times a
 // power of two a row.
 uint32_t pitch_of(uint32_t n) { return (n + 7u) & ~7u; }
@@ -80,10 +83,10 @@ extern "C" size_t eoq_b200_gated_scratch(const eoq_b200_gated_t *w, const eoq_b2
     if (product_takes(pair_of(w), 2)) {
         c.take<void>(half_bytes(batch, w->cols));
         c.take<float>((size_t)batch * 4);
-    } else if (form == kKeep8bit) {
-        c.take<float>(2 * values(batch, w->rows) * 4);
+        if (!few_rows(pair_of(w), dtype, batch)) return c.at;
     }
-    return c.at;
+    const size_t sums = form == kKeep8bit ? 2 * values(batch, w->rows) * 4 : 0;
+    return std::max(c.at, sums);
 }
 
 extern "C" eoq_error_t eoq_b200_gated_packed(const eoq_b200_gated_t *w, const void *x, int dtype, uint32_t batch, void *d_scratch, void *h,
@@ -102,6 +105,17 @@ extern "C" eoq_error_t eoq_b200_gated_packed(const eoq_b200_gated_t *w, const vo
     Carve scratch{static_cast<uint8_t *>(d_scratch)};
     const size_t n = values(batch, w->rows);
     int e = 0;
+    const Kept keep = c.keep;
+    if (few_rows(c.w, dtype, batch) && (reinterpret_cast<uintptr_t>(x) & 15u) == 0) {
+        if (form == kKeep8bit) {
+            float *g = scratch.take<float>(2 * n * 4);
+            c.keep = Kept{kKeepF32, {g, g + n}, {nullptr, nullptr}};
+        }
+        e = launch_gated_rows(c, stream);
+        for (int i = 0; i < 2 && e == 0 && form == kKeep8bit; i++)
+            e = launch_store_8bit(c.keep.v[i], EOQ_B200_F32, batch, w->rows, static_cast<int8_t *>(keep.v[i]), keep.scale[i], stream);
+        return launched(e, where);
+    }
     if (dtype != EOQ_B200_F32 && product_takes(c.w, 2)) {
         uint16_t *half = scratch.take<uint16_t>(half_bytes(batch, w->cols));
         float *factor = scratch.take<float>((size_t)batch * 4);
@@ -135,7 +149,6 @@ extern "C" eoq_error_t eoq_b200_gated_packed(const eoq_b200_gated_t *w, const vo
         scratch.at = 0;
     }
     if (dtype == EOQ_B200_F32) scratch.take<void>(values(batch, w->cols + 1) * 4);
-    const Kept keep = c.keep;
     if (form == kKeep8bit) {
         float *g = scratch.take<float>(2 * n * 4);
         c.keep = Kept{kKeepF32, {g, g + n}, {nullptr, nullptr}};
