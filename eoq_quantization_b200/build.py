@@ -15,7 +15,7 @@ OBJ = os.path.join(HERE, "build")
 LIB = os.path.join(HERE, "libeoq_b200.so")
 NATIVE = os.path.join(HERE, "_native.so")
 SOURCES = ["abi.cu", "kernels.cu", "qmm.cu", "gated.cu", "gated_product.cu", "gated_rows.cu", "gated_abi.cu", "wire_encode.cu", "rans_host.cpp", "wire_host.cpp"]
-HEADERS = ["eoq_internal.h", "tensor_core.h", "packed_mma.h", "gated.h", "activations.cuh", os.path.join("..", "..", "include", "eoq_b200.h")]
+HEADERS = ["eoq_internal.h", "tensor_core.h", "and_or.h", "packed_mma.h", "gated.h", "activations.cuh", os.path.join("..", "..", "include", "eoq_b200.h")]
 
 
 def nvcc() -> str:

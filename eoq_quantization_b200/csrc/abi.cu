@@ -2403,7 +2403,6 @@ extern "C" int eoq_b200_tune(const char *key, int value)
     if (std::strcmp(key, "v1_lanes") == 0) { set_v1_lanes(value); return 0; }
     if (std::strcmp(key, "packed_warps") == 0) { set_packed_warps(value); return 0; }
     if (std::strcmp(key, "dequant_vec") == 0) { set_dequant_vec(value); return 0; }
-    if (std::strcmp(key, "gated_rows") == 0) { set_gated_rows(value & 31, value >> 5); return 0; }
     if (std::strcmp(key, "qmm_wait_us") == 0) { set_qmm_wait_us(value); set_gated_wait_us(value); return 0; }
     if (std::strcmp(key, "pinned_refused") == 0) { g_pinned_refused.store(value); return 0; }
     if (std::strcmp(key, "release_scratch") == 0) { DeviceArena::trim(); PinnedBlock::trim(); return 0; }

@@ -65,7 +65,8 @@ int launch_input_grad_product(const PackedPair &w, int nw, const uint16_t *dy, u
 // Up to eight rows of 16-bit activations, 16-byte aligned; kept in full or in fp32 (gated_rows.cu).
 bool gated_rows_takes(const PackedPair &w, uint32_t batch);
 int launch_gated_rows(const GatedCall &c, void *stream);
-void set_gated_rows(int warps, int ctas);
+long long gated_wait_limit();
+uint32_t *gated_status_word();       // of the current device
 uint32_t gated_status();
 void set_gated_wait_us(int v);
 

@@ -647,6 +647,21 @@ int launch_input_grad_product(const PackedPair &w, int nw, const uint16_t *dy, u
 
 void set_gated_wait_us(int v) { g_limit.store(std::min(std::max(v, 0), 60000000) * 2000ll); }
 
+long long gated_wait_limit() { return g_limit.load(std::memory_order_relaxed); }
+
+uint32_t *gated_status_word()
+{
+    static std::atomic<uint32_t *> known[16];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return nullptr;
+    uint32_t *p = dev < 16 ? known[dev].load() : nullptr;
+    if (!p) {
+        if (cudaGetSymbolAddress(reinterpret_cast<void **>(&p), g_gated_status) != cudaSuccess) return nullptr;
+        if (dev < 16) known[dev].store(p);
+    }
+    return p;
+}
+
 uint32_t gated_status()
 {
     uint32_t v = 0, zero = 0;

@@ -6,17 +6,16 @@
 // dummy: a lane feeds its codes in the order in which they leave their words cheapest (packed_mma.h), and the activations, brought
 // to shared memory in that order once per CTA, follow.
 //
-// A CTA takes a run of neighbouring eights of features ("tiles"), and its warps equal runs of the tiles' 128-column spans, whichever
-// tile these belong to; a warp leaves its sums of a tile in shared memory where it goes on to the next one, and what the warps left is
-// added up in their order.
+// A CTA takes a run of neighbouring eights of features ("tiles"), and its warps equal runs of the tiles' chunks, 128 bytes of all
+// sixteen rows, whichever tile these belong to; a warp leaves its sums of a tile in shared memory where it goes on to the next one,
+// and what the warps left is added up in their order.  Each warp has a ring of chunks of its own, which TMA fills some chunks ahead:
+// what has to be under way to keep HBM busy (50 KB an SM) would not fit the registers.
+//   Waits are bounded: a warp whose copy does not come marks the CTA, whose results become NaN, and sets the status word.
 #include "gated.h"
 #include "packed_mma.h"
+#include "tensor_core.h"
 
 #include <algorithm>
-#include <atomic>
-#include <cuda_fp16.h>
-#include <mutex>
-#include <vector>
 
 #include "activations.cuh"
 
@@ -24,18 +23,23 @@ namespace eoq {
 namespace {
 
 struct RowsArgs {
-    const uint8_t *codes[2];
     const uint16_t *scales[2];
     const float *bias[2];
     const void *x;
     void *h;
     void *kept[2];               // [batch][N] of x's type, fp32 (kept32), or null
-    uint32_t N, K, group, row_bytes, batch, tiles;
+    uint32_t N, K, group, batch, per, more;      // tiles a CTA takes, and how many CTAs take one more
+    uint32_t most, pitch, slots; // tiles at a time, words that a row's scales take in shared memory, chunks of a warp's ring
     int act, kept32;
+    long long limit;             // clock ticks a wait may take
+    uint32_t *status;            // set when one runs out
 };
 
-constexpr uint32_t kMostThreads = 768;
+constexpr int most_threads(int bt) { return bt == 1 ? 1024 : 768; }        // 64 or 80 registers a thread
 constexpr int kParts = 3;        // tiles that a warp's run touches at most, for up to two tiles a warp
+
+// A unit (half of one, where that has 128 bytes) in bytes and columns: a lane takes a quarter of it.
+template <int BITS, int U> struct Part { static constexpr int kBytes = U * BITS / 8 < 64 ? U * BITS / 8 : 64, kCols = kBytes * 8 / BITS; };
 
 // x in the order of the codes: sixteen-byte pieces [span][i][row][t], piece i of lane (row, t) the columns of its registers 4 i .. 4 i + 3.
 template <int BITS, int U>
@@ -53,131 +57,183 @@ __device__ __forceinline__ uint4 piece_of(const uint16_t *x, uint32_t span, uint
     }
 }
 
-// U: columns of a unit whose scale is applied on its own, the largest of 128, 64 and 32 that divides a group.  Of a span's units a lane
-// takes an equal part each, 32 columns in all.  BT: rows of x, of which `batch` are there.
-template <int BITS, bool BF16, int U, int BT>
-__global__ void __launch_bounds__(kMostThreads, 1) gated_rows_kernel(const RowsArgs a)
+// U: columns of a unit whose scale is applied on its own.
+// EXACT: units are groups, and a chunk's scales lie together; else a group is several units.
+// BT: rows of x that shared memory has room for.
+//   Lane (g, t) takes the tile's row whose number is g's three bits reversed: with the copies' 128-byte swizzle the rows that a load's
+// phase covers then lie in different banks, for loads of 16, 8 and 4 bytes.
+//   What it takes 128 columns (2048 codes a warp): at four bits 72 instructions for the codes, 8 products, 6 loads of codes and activations.
+template <int BITS, bool BF16, int U, bool EXACT, int BT>
+__global__ void __launch_bounds__(most_threads(BT), 1) gated_rows_kernel(const RowsArgs a, const __grid_constant__ CUtensorMap gmap, const __grid_constant__ CUtensorMap umap)
 {
     static_assert(BITS != 2 || U >= 64, "a unit of 32 two-bit codes is no whole word of a lane");
-    constexpr int kUnits = 128 / U, kWords = BITS / kUnits;        // of a lane's part of a unit
-    constexpr int kSets = BITS == 8 || U < 128 ? 2 : 3;            // register sets of codes and scales, all but one on their way (more spill)
-    extern __shared__ uint4 xs[];
-    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, nwarps = blockDim.x >> 5, g = lane >> 2, t = lane & 3u;
-    const uint32_t sgroups = a.K / a.group, nspans = a.K >> 7, gunits = a.group / U;
-    float (*red)[kParts][16][BT] = reinterpret_cast<float (*)[kParts][16][BT]>(xs + (size_t)nspans * 16u * BT);
-    const uint32_t last = (uint32_t)((uint64_t)a.tiles * (blockIdx.x + 1) / gridDim.x);
-    uint32_t tile0 = (uint32_t)((uint64_t)a.tiles * blockIdx.x / gridDim.x), ntiles = min(last - tile0, 2u * nwarps);
+    using P = Part<BITS, U>;
+    constexpr int CH = 8 / BITS;                                   // spans of 128 columns a chunk has
+    constexpr int kUnits = 128 / U, kParts128 = 128 / P::kBytes, kWords = P::kBytes / 16;      // units of a span, parts of a chunk, words of a lane's share of a part
+    constexpr int kScales = (CH * kUnits + 1) / 2;                 // words of a chunk's scales (EXACT)
+    constexpr uint32_t kHalf = 1024u, kSlot = 2048u;               // a chunk's codes of one weight, of both
+    extern __shared__ uint8_t raw[];
+    const uint32_t lane = threadIdx.x & 31u, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), nwarps = blockDim.x >> 5, g = lane >> 2, t = lane & 3u;
+    const uint32_t sgroups = a.K / a.group, chunks = a.K / (128u * CH), gunits = a.group / U, myrow = (g & 1u) << 2 | (g & 2u) | g >> 2;
+    constexpr uint32_t kPieces = 16u * BT * CH;                    // of a chunk of x
+    // shared memory: rings, activations, scales [gate, up][row of the tiles][pitch], sums, barriers and the mark
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023u) & ~(uintptr_t)1023u);
+    uint4 *xs = reinterpret_cast<uint4 *>(smem + (size_t)nwarps * a.slots * kSlot);
+    uint32_t *scales = reinterpret_cast<uint32_t *>(xs + (size_t)chunks * kPieces);
+    float (*red)[kParts][16][BT] = reinterpret_cast<float (*)[kParts][16][BT]>(scales + (size_t)a.most * 16u * a.pitch);
+    const uint32_t ring = saddr(smem) + warp * a.slots * kSlot, bars = saddr(red + nwarps) + warp * a.slots * 8u, mark = saddr(red + nwarps) + nwarps * a.slots * 8u;
+    uint32_t tile0 = blockIdx.x * a.per + min(blockIdx.x, a.more), ntiles;
+    const uint32_t last = tile0 + a.per + (blockIdx.x < a.more);
 
-    // a warp's run of spans of the tiles at hand, and what one load of it brings: both rows' codes and scales
-    uint32_t next, end, load_tile, load_span;
-    const uint8_t *pw[2];
-    const uint16_t *ps[2];
-    auto at_tile = [&]() {
-        const uint32_t row = min((tile0 + load_tile) * 8u + g, a.N - 1u);
-#pragma unroll
-        for (int r = 0; r < 2; r++) {
-            pw[r] = a.codes[r] + (size_t)row * a.row_bytes + t * (4u * BITS / kUnits);
-            ps[r] = a.scales[r] + (size_t)row * sgroups;
+    // a warp's run of chunks of the tiles at hand; copies are requested `slots` chunks ahead
+    uint32_t next, end, to_load = 0, load_tile, load_chunk;
+    bool gave_up = false;
+    auto begin = [&]() {
+        ntiles = min(last - tile0, a.most);
+        const uint32_t n = ntiles * chunks;
+        next = to_load = n * warp / nwarps;
+        end = n * (warp + 1) / nwarps;
+        load_tile = next / chunks;
+        load_chunk = next - load_tile * chunks;
+    };
+    auto load = [&](uint32_t slot) {
+        if (to_load >= end || gave_up) return;
+        to_load++;
+        if (lane == 0) {
+            const uint32_t bar = bars + slot * 8u, to = ring + slot * kSlot, row = (tile0 + load_tile) * 8u, at = load_chunk * 128u;
+            bar_expect(bar, kSlot);
+            tma_2d(to, &gmap, at, row, bar);
+            tma_2d(to + kHalf, &umap, at, row, bar);
+        }
+        if (++load_chunk == chunks) { load_chunk = 0; load_tile++; }
+    };
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+        if (bar_try(bar, parity)) return;
+        const long long t0 = clock64();
+        while (!bar_try(bar, parity)) {
+            if (clock64() - t0 <= a.limit && !gave_up) continue;
+            gave_up = true;                        // (of all lanes or none: the loop is left together, below)
+            break;
+        }
+        gave_up = __any_sync(0xffffffffu, gave_up);
+        if (gave_up && lane == 0) {
+            asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(mark), "r"(1u) : "memory");
+            *reinterpret_cast<volatile uint32_t *>(a.status) = 1u;
         }
     };
-    auto begin = [&]() {
-        const uint32_t n = ntiles * nspans;
-        next = (uint32_t)((uint64_t)n * warp / nwarps);
-        end = (uint32_t)((uint64_t)n * (warp + 1) / nwarps);
-        load_tile = next / nspans;
-        load_span = next - load_tile * nspans;
-        at_tile();
-    };
-    struct Loaded { uint32_t w[2][BITS]; uint16_t sc[2][kUnits]; };
-    uint32_t to_load = 0;
-    auto load = [&](Loaded &l) {
-        if (to_load >= end) return;
-#pragma unroll
-        for (int r = 0; r < 2; r++)
-#pragma unroll
-            for (int u = 0; u < kUnits; u++) {
-                const uint8_t *p = pw[r] + load_span * (16u * BITS) + u * (U * BITS / 8);
-                if constexpr (kWords == 1) {
-                    l.w[r][u] = __ldg(reinterpret_cast<const uint32_t *>(p));
-                } else if constexpr (kWords == 2) {
-                    const uint2 v = __ldg(reinterpret_cast<const uint2 *>(p));
-                    l.w[r][2 * u] = v.x; l.w[r][2 * u + 1] = v.y;
-                } else {
-#pragma unroll
-                    for (int h = 0; h < kWords / 4; h++) {
-                        const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p) + h);
-                        uint32_t *d = &l.w[r][u * kWords + 4 * h];
-                        d[0] = v.x; d[1] = v.y; d[2] = v.z; d[3] = v.w;
-                    }
-                }
-                const uint32_t at = load_span * kUnits + u;
-                l.sc[r][u] = __ldg(ps[r] + (gunits == 1u ? at : at / gunits));
-            }
-        to_load++;
-        if (++load_span == nspans) { load_span = 0; load_tile++; at_tile(); }
+    // Scales by whole rows to shared memory: a load of a few of each row would touch as many lines as one of their codes.
+    auto fetch_scales = [&]() {
+        for (uint32_t row = warp; row < ntiles * 16u; row += nwarps) {
+            const uint32_t which = row >= ntiles * 8u, n = min(tile0 * 8u + row - which * ntiles * 8u, a.N - 1u);
+            const uint16_t *from = (which ? a.scales[1] : a.scales[0]) + (size_t)n * sgroups;
+            if (EXACT && CH * kUnits > 1) for (uint32_t j = lane; j < sgroups / 2u; j += 32u) scales[row * a.pitch + j] = __ldg(reinterpret_cast<const uint32_t *>(from) + j);
+            else for (uint32_t j = lane; j < sgroups; j += 32u) reinterpret_cast<uint16_t *>(scales + row * a.pitch)[j] = __ldg(from + j);
+        }
     };
 
     // codes and scales do not depend on the kernel before this one in the stream, the activations may
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (lane == 0) for (uint32_t i = 0; i < a.slots; i++) bar_init(bars + i * 8u, 1);
+    if (threadIdx.x == 0) asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(mark), "r"(0u) : "memory");
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    __syncwarp();
     begin();
-    to_load = next;
-    Loaded buf[kSets];
-#pragma unroll
-    for (int d = 0; d < kSets - 1; d++) load(buf[d]);
+    for (uint32_t i = 0; i < a.slots; i++) load(i);
+    fetch_scales();
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    for (uint32_t e = threadIdx.x; e < nspans * 16u * BT; e += blockDim.x) {
+    for (uint32_t e = threadIdx.x; e < chunks * kPieces; e += blockDim.x) {
         const uint32_t tt = e & 3u, b = (e >> 2) % BT, i = (e >> 2) / BT & 3u, s = e / (16u * BT);
-        xs[e] = b < a.batch ? piece_of<BITS, U>(reinterpret_cast<const uint16_t *>(a.x) + (size_t)b * a.K, s, i, tt) : make_uint4(0u, 0u, 0u, 0u);
+        if (b < a.batch) xs[e] = piece_of<BITS, P::kCols>(reinterpret_cast<const uint16_t *>(a.x) + (size_t)b * a.K, s, i, tt);
     }
     __syncthreads();
 
+    // (columns of the products behind the last row of x are left: what lanes of such rows read is any other row)
+    const uint32_t x0 = (uint32_t)__cvta_generic_to_shared(xs) + (min(g, a.batch - 1u) * 4u + t) * 16u;
+    const uint32_t s0 = (uint32_t)__cvta_generic_to_shared(scales) + myrow * a.pitch * 4u;
+    const uint32_t w0 = ring + myrow * 128u + ((((t * (P::kBytes / 4)) >> 4) ^ myrow) << 4) + ((t * (P::kBytes / 4)) & 15u);
     float tot[4];
-    auto multiply = [&](const Loaded &l, uint32_t span) {
-        const uint4 *xp = xs + (size_t)span * 16u * BT + g * 4u + t;
-        // four registers of codes a row at a time, and their piece of the activations: two products, whose accumulators alternate, so
-        // that consecutive ones do not wait for one another
-        float c[4], d[4];
+    // w, x, s: shared addresses of the lane's share of the chunk's codes, of the activations, and of the gate row's scales
+    auto multiply = [&](uint32_t w, uint32_t x, uint32_t s, uint32_t chunk) {
+        uint32_t code[2][8];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            uint4 q = make_uint4(0u, 0u, 0u, 0u);
-            if (BT == 8 || g < BT) q = xp[i * 4 * BT];
-            uint32_t h0[4], h1[4];
-            if constexpr (BITS == 4) {
-                unpack_word<BITS, BF16>(l.w[0][i], h0);
-                unpack_word<BITS, BF16>(l.w[1][i], h1);
-            } else if constexpr (BITS == 2) {
-                uint32_t e0[8], e1[8];
-                unpack_word<BITS, BF16>(l.w[0][i / 2], e0);
-                unpack_word<BITS, BF16>(l.w[1][i / 2], e1);
+        for (int r = 0; r < 2; r++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) { h0[j] = e0[4 * (i & 1) + j]; h1[j] = e1[4 * (i & 1) + j]; }
-            } else {
-                uint32_t e[2];
-#pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    unpack_word<BITS, BF16>(l.w[0][2 * i + j], e);
-                    h0[2 * j] = e[0]; h0[2 * j + 1] = e[1];
-                    unpack_word<BITS, BF16>(l.w[1][2 * i + j], e);
-                    h1[2 * j] = e[0]; h1[2 * j + 1] = e[1];
-                }
+            for (int p = 0; p < kParts128; p++) {
+                const uint32_t at = (w ^ (p * P::kBytes)) + r * kHalf;
+                uint32_t *d = &code[r][p * kWords];
+                if constexpr (kWords == 1) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(d[0]) : "r"(at));
+                else if constexpr (kWords == 2) asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(d[0]), "=r"(d[1]) : "r"(at));
+                else asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]) : "r"(at));
             }
-            constexpr int kPieces = 4 / kUnits;                    // of a unit
-            if (i % kPieces == 0) {
-                mma_m16n8k16_first<BF16>(c, h0[0], h1[0], h0[1], h1[1], q.x, q.y);
-                mma_m16n8k16_first<BF16>(d, h0[2], h1[2], h0[3], h1[3], q.z, q.w);
-            } else {
-                mma_m16n8k16<BF16>(c, h0[0], h1[0], h0[1], h1[1], q.x, q.y);
-                mma_m16n8k16<BF16>(d, h0[2], h1[2], h0[3], h1[3], q.z, q.w);
-            }
-            if (i % kPieces == kPieces - 1) {
-                const float fa = __half2float(__ushort_as_half(l.sc[0][i / kPieces])), fb = __half2float(__ushort_as_half(l.sc[1][i / kPieces]));
-                tot[0] = fmaf(fa, c[0] + d[0], tot[0]); tot[1] = fmaf(fa, c[1] + d[1], tot[1]);
-                tot[2] = fmaf(fb, c[2] + d[2], tot[2]); tot[3] = fmaf(fb, c[3] + d[3], tot[3]);
+        uint32_t sc[2][kScales] = {};
+        if constexpr (EXACT) {
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+                const uint32_t at = s + r * ntiles * 32u * a.pitch;
+                if constexpr (CH * kUnits == 1) asm volatile("ld.shared.u16 %0, [%1];" : "=r"(sc[r][0]) : "r"(at));
+                else if constexpr (kScales == 1) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(sc[r][0]) : "r"(at));
+                else if constexpr (kScales == 2) asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(sc[r][0]), "=r"(sc[r][1]) : "r"(at));
+                else asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(sc[r][0]), "=r"(sc[r][1]), "=r"(sc[r][2]), "=r"(sc[r][3]) : "r"(at));
             }
         }
+        auto scale = [&](int r, int u) {
+            uint32_t v;
+            if (EXACT) v = sc[r][u / 2] >> (16 * (u & 1));
+            else asm volatile("ld.shared.u16 %0, [%1];" : "=r"(v) : "r"(s + r * ntiles * 32u * a.pitch + (chunk * (uint32_t)(CH * kUnits) + u) / gunits * 2u));
+            return __half2float(__ushort_as_half((uint16_t)v));
+        };
+        // four registers of codes a row and span at a time, and their piece of the activations: two products.  The accumulators of the
+        // chunk's spans (of one span: two) alternate, so that consecutive products do not wait for one another.
+        float c[CH == 1 ? 2 : CH][4];
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int sp = 0; sp < CH; sp++) {
+                uint4 q;
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "r"(x + (sp * 4 + i) * (BT * 64)));
+                uint32_t h[2][4];
+#pragma unroll
+                for (int r = 0; r < 2; r++) {
+                    if constexpr (BITS == 4) {
+                        unpack_word<BITS, BF16>(code[r][sp * 4 + i], h[r]);
+                    } else if constexpr (BITS == 2) {
+                        uint32_t e[8];
+                        unpack_word<BITS, BF16>(code[r][sp * 2 + i / 2], e);
+#pragma unroll
+                        for (int j = 0; j < 4; j++) h[r][j] = e[4 * (i & 1) + j];
+                    } else {
+                        uint32_t e[2];
+#pragma unroll
+                        for (int j = 0; j < 2; j++) {
+                            unpack_word<BITS, BF16>(code[r][2 * i + j], e);
+                            h[r][2 * j] = e[0]; h[r][2 * j + 1] = e[1];
+                        }
+                    }
+                }
+                constexpr int kOfUnit = 4 / kUnits;                    // pieces
+                float (&one)[4] = c[CH == 1 ? 0 : sp], (&two)[4] = c[CH == 1 ? 1 : sp];
+                if (i % kOfUnit == 0) {
+                    mma_m16n8k16_first<BF16>(one, h[0][0], h[1][0], h[0][1], h[1][1], q.x, q.y);
+                    if (CH > 1) mma_m16n8k16<BF16>(two, h[0][2], h[1][2], h[0][3], h[1][3], q.z, q.w);
+                    else mma_m16n8k16_first<BF16>(two, h[0][2], h[1][2], h[0][3], h[1][3], q.z, q.w);
+                } else {
+                    mma_m16n8k16<BF16>(one, h[0][0], h[1][0], h[0][1], h[1][1], q.x, q.y);
+                    mma_m16n8k16<BF16>(two, h[0][2], h[1][2], h[0][3], h[1][3], q.z, q.w);
+                }
+                if (i % kOfUnit == kOfUnit - 1) {
+                    const int u = sp * kUnits + i / kOfUnit;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) tot[j] = fmaf(scale(j >> 1, u), CH > 1 ? one[j] : one[j] + two[j], tot[j]);
+                }
+            }
     };
+    Ring at_slot, lost;                            // (laps go on over the rounds of tiles)
+    uint32_t owing = 0;
     for (;;) {
-        uint32_t span = next % nspans, part = 0;
+        const uint32_t first_tile = next / chunks;
+        uint32_t chunk = next - first_tile * chunks, part = 0, x = x0 + chunk * (kPieces * 16u);
+        constexpr uint32_t kStep = EXACT ? CH * kUnits * 2u : 0u;
+        uint32_t sc = s0 + first_tile * 32u * a.pitch + chunk * kStep;
         tot[0] = tot[1] = tot[2] = tot[3] = 0.0f;
         auto leave = [&]() {
             if (2u * t < BT) {
@@ -188,31 +244,46 @@ __global__ void __launch_bounds__(kMostThreads, 1) gated_rows_kernel(const RowsA
             part++;
             tot[0] = tot[1] = tot[2] = tot[3] = 0.0f;
         };
-        while (next < end) {
-#pragma unroll
-            for (int d = 0; d < kSets; d++) {                       // register sets in rotation: every index is static
-                if (next >= end) break;
-                load(buf[(d + kSets - 1) % kSets]);
-                multiply(buf[d], span);
-                next++;
-                if (++span == nspans) { leave(); span = 0; }
+        for (; next < end; next++) {
+            if (!gave_up) {
+                wait(bars + at_slot.at * 8u, at_slot.lap);
+                if (gave_up) { lost = at_slot; owing = to_load - next; }
+            }
+            multiply(w0 + at_slot.at * kSlot, x, sc, chunk);
+            // every lane's codes have gone into products: the slot is free
+            __syncwarp();
+            load(at_slot.at);
+            at_slot.next(a.slots);
+            x += kPieces * 16u;
+            sc += kStep;
+            if (++chunk == chunks) {
+                leave();
+                chunk = 0;
+                x = x0;
+                sc += 32u * a.pitch - chunks * kStep;
             }
         }
-        if (span) leave();
+        if (chunk) leave();
+        if (owing) {                               // no copy may be under way when the CTA ends
+            const long long t0 = clock64();
+            for (; owing; owing--, lost.next(a.slots)) while (!bar_try(bars + lost.at * 8u, lost.lap) && clock64() - t0 < 20000000ll) {}
+        }
         __syncthreads();
+        uint32_t stopped;
+        asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(stopped) : "r"(mark) : "memory");
         // every (tile, row of x, feature): the parts of the warps whose runs touch the tile, in their order
-        const uint32_t n = ntiles * nspans;
+        const uint32_t n = ntiles * chunks;
         for (uint32_t i = threadIdx.x; i < ntiles * 8u * BT; i += blockDim.x) {
-            const uint32_t f = i & 7u, b = (i >> 3) % BT, tile = i / (8u * BT), feature = (tile0 + tile) * 8u + f;
+            const uint32_t f = i & 7u, b = (i >> 3) % BT, tile = i / (8u * BT), feature = (tile0 + tile) * 8u + ((f & 1u) << 2 | (f & 2u) | f >> 2);
             if (feature >= a.N || b >= a.batch) continue;
-            const uint32_t first = tile * nspans, behind = first + nspans;
-            // the warp that has span s: the last w with n w / nwarps <= s
-            uint32_t w = (uint32_t)(((uint64_t)(first + 1) * nwarps - 1) / n);
+            const uint32_t first = tile * chunks, behind = first + chunks;
+            // the warp that has chunk s: the last w with n w / nwarps <= s
+            uint32_t w = ((first + 1) * nwarps - 1) / n;
             float gs = 0.0f, us = 0.0f;
-            for (uint32_t from = (uint32_t)((uint64_t)n * w / nwarps); w < nwarps && from < behind; w++) {
-                const uint32_t to = (uint32_t)((uint64_t)n * (w + 1) / nwarps);
+            for (uint32_t from = n * w / nwarps; w < nwarps && from < behind; w++) {
+                const uint32_t to = n * (w + 1) / nwarps;
                 if (to > from) {
-                    const uint32_t part_of = tile - from / nspans;
+                    const uint32_t part_of = tile - from / chunks;
                     gs += red[w][part_of][f][b];
                     us += red[w][part_of][8 + f][b];
                 }
@@ -220,6 +291,7 @@ __global__ void __launch_bounds__(kMostThreads, 1) gated_rows_kernel(const RowsA
             }
             if (a.bias[0]) gs += __ldg(a.bias[0] + feature);
             if (a.bias[1]) us += __ldg(a.bias[1] + feature);
+            if (stopped) gs = us = __uint_as_float(0x7fffffffu);
             const size_t at = (size_t)b * a.N + feature;
             auto put = [&](void *to, float value) {
                 if (BF16) reinterpret_cast<__nv_bfloat16 *>(to)[at] = __float2bfloat16_rn(value);
@@ -237,76 +309,114 @@ __global__ void __launch_bounds__(kMostThreads, 1) gated_rows_kernel(const RowsA
         }
         tile0 += ntiles;
         if (tile0 >= last) break;
-        ntiles = min(last - tile0, 2u * nwarps);
         __syncthreads();
+        gave_up = stopped != 0;
         begin();
-        to_load = next;
-#pragma unroll
-        for (int d = 0; d < kSets - 1; d++) load(buf[d]);
+        // (the slots in the order in which the ring comes by them)
+        for (uint32_t i = 0, slot = at_slot.at; i < a.slots; i++, slot = slot + 1 == a.slots ? 0 : slot + 1) load(slot);
+        fetch_scales();
+        __syncthreads();
     }
 }
 
-std::atomic<int> g_warps{0}, g_ctas{0};        // 0: by shape
+uint32_t rounded(uint32_t batch) { return batch <= 1 ? 1u : batch <= 4 ? 4u : 8u; }
 
-uint32_t rounded(uint32_t batch) { return batch <= 1 ? 1u : batch <= 2 ? 2u : batch <= 4 ? 4u : 8u; }
-size_t rows_smem(uint32_t K, uint32_t bt, uint32_t warps) { return (size_t)K * bt * 2 + (size_t)warps * kParts * 16 * bt * 4; }
-
-template <int BITS, bool BF16, int U>
-void (*by_batch(uint32_t bt))(RowsArgs)
+// How a call is laid out: CTAs to an SM, warps, chunks of a warp's ring, tiles whose scales are in shared memory at a time (up to two a
+// warp, see kParts, and 64 KB of scales).  A row's scales are an odd number of their loads' sizes apart, so that the rows of a tile lie in
+// different banks.
+struct Room { uint32_t warps, slots, most, pitch; size_t smem; };
+Room room_for(const PackedPair &w, uint32_t bt, uint32_t warps, uint32_t slots, uint32_t tiles)
 {
-    return bt == 1 ? gated_rows_kernel<BITS, BF16, U, 1> : bt == 2 ? gated_rows_kernel<BITS, BF16, U, 2> : bt == 4 ? gated_rows_kernel<BITS, BF16, U, 4>
-                                                                                                                   : gated_rows_kernel<BITS, BF16, U, 8>;
+    // groups of a chunk (1024 bits of a row), whose scales one load of as many halves of a word fetches where that is a whole number
+    const uint32_t groups = w.K / w.group, chunk = 1024u / (w.bits == 2 || w.bits == 4 ? w.bits : 8u) / w.group, load = std::max(1u, chunk / 2u);
+    Room r;
+    r.warps = warps;
+    r.slots = slots;
+    r.pitch = ((groups + 1) / 2 + load - 1) / load * load;
+    if (r.pitch / load % 2 == 0) r.pitch += load;
+    r.most = std::max(1u, std::min({2u * warps, tiles, 65536u / (64u * r.pitch)}));
+    r.smem = 1024 + (size_t)warps * slots * (2048 + 8) + (size_t)w.K * bt * 2 + (size_t)r.most * 64 * r.pitch + (size_t)warps * kParts * 16 * bt * 4 + 16;
+    return r;
+}
+
+typedef void (*Kernel)(RowsArgs, CUtensorMap, CUtensorMap);
+
+template <int BITS, bool BF16, int U, bool EXACT>
+Kernel by_batch(uint32_t bt)
+{
+    return bt == 1 ? (Kernel)gated_rows_kernel<BITS, BF16, U, EXACT, 1> : bt == 4 ? (Kernel)gated_rows_kernel<BITS, BF16, U, EXACT, 4> : (Kernel)gated_rows_kernel<BITS, BF16, U, EXACT, 8>;
+}
+
+// Groups that are several units go one scale at a time.
+template <int BITS, bool BF16>
+Kernel by_group(uint32_t group, uint32_t bt)
+{
+    constexpr int kLeast = BITS == 2 ? 64 : 32;
+    if (group == 128u) return by_batch<BITS, BF16, 128, true>(bt);
+    if (group == 64u) return by_batch<BITS, BF16, 64, true>(bt);
+    if (group == 32u && kLeast == 32) return by_batch<BITS, BF16, kLeast, true>(bt);
+    if (group % 128u == 0) return by_batch<BITS, BF16, 128, false>(bt);
+    return by_batch<BITS, BF16, kLeast, false>(bt);
 }
 
 }  // namespace
 
-void set_gated_rows(int warps, int ctas) { g_warps.store(warps); g_ctas.store(ctas); }
-
-// Whole spans a row, whole units a group, activations that fit beside the warps' sums.
+// Rows of whole 128-byte lines, whole units a group, scales that can be loaded two at a time, activations that fit beside two chunks a warp.
 bool gated_rows_takes(const PackedPair &w, uint32_t batch)
 {
-    return batch <= 8 && product_takes(w, 2) && w.K % 128u == 0 && (w.bits != 2 || w.group % 64u == 0) && rows_smem(w.K, rounded(batch), kMostThreads / 32) <= 226u * 1024u;
+    const uintptr_t scales = reinterpret_cast<uintptr_t>(w.scales[0]) | reinterpret_cast<uintptr_t>(w.scales[1]);
+    return batch <= 8 && (scales & 3u) == 0 && product_takes(w, 2) && w.row_bytes % 128u == 0 && (w.bits != 2 || w.group % 64u == 0) &&
+           room_for(w, rounded(batch), 16, 2, 1u << 20).smem <= 226u * 1024u;
 }
 
 int launch_gated_rows(const GatedCall &c, void *stream)
 {
-    RowsArgs a = {{c.w.codes[0], c.w.codes[1]}, {c.w.scales[0], c.w.scales[1]}, {c.bias[0], c.bias[1]}, c.x, c.h, {c.keep.v[0], c.keep.v[1]},
-                  c.w.N, c.w.K, c.w.group, c.w.row_bytes, c.M, (c.w.N + 7u) / 8u, c.act, c.keep.form == kKeepF32};
-    const uint32_t bt = rounded(c.M), unit = a.group % 128u == 0 ? 128u : a.group % 64u == 0 ? 64u : 32u;
-    void (*kern)(RowsArgs) = nullptr;
-#define EOQ_ROWS(B, U) (c.dtype == EOQ_B200_BF16 ? by_batch<B, true, U>(bt) : by_batch<B, false, U>(bt))
-    if (c.w.bits == 4) kern = unit == 128u ? EOQ_ROWS(4, 128) : unit == 64u ? EOQ_ROWS(4, 64) : EOQ_ROWS(4, 32);
-    else if (c.w.bits == 2) kern = unit == 128u ? EOQ_ROWS(2, 128) : EOQ_ROWS(2, 64);
-    else kern = unit == 128u ? EOQ_ROWS(8, 128) : unit == 64u ? EOQ_ROWS(8, 64) : EOQ_ROWS(8, 32);
-#undef EOQ_ROWS
-    const uint32_t sms = (uint32_t)device_sm_count();
-    uint32_t warps = g_warps.load() ? (uint32_t)g_warps.load() : 12u, per_sm = g_ctas.load() ? (uint32_t)g_ctas.load() : 2u;
-    const size_t smem = rows_smem(a.K, bt, warps);
-    static std::mutex mu;                          // kernels whose shared-memory limit has been raised, per device
-    static std::vector<std::pair<const void *, int>> raised;
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return (int)e;
-    {
-        std::lock_guard<std::mutex> lock(mu);
-        const std::pair<const void *, int> key(reinterpret_cast<const void *>(kern), dev);
-        if (std::find(raised.begin(), raised.end(), key) == raised.end()) {
-            e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
-            if (e != cudaSuccess) return (int)e;
-            raised.push_back(key);
-        }
+    RowsArgs a = {};
+    for (int i = 0; i < 2; i++) { a.scales[i] = c.w.scales[i]; a.bias[i] = c.bias[i]; a.kept[i] = c.keep.v[i]; }
+    a.x = c.x; a.h = c.h; a.N = c.w.N; a.K = c.w.K; a.group = c.w.group; a.batch = c.M; a.act = c.act; a.kept32 = c.keep.form == kKeepF32;
+    a.limit = gated_wait_limit();
+    a.status = gated_status_word();
+    if (!a.status) return (int)cudaErrorInvalidDevice;
+    const uint32_t bt = rounded(c.M);
+    const bool bf = c.dtype == EOQ_B200_BF16;
+    const Kernel kern = c.w.bits == 4   ? (bf ? by_group<4, true>(a.group, bt) : by_group<4, false>(a.group, bt))
+                        : c.w.bits == 2 ? (bf ? by_group<2, true>(a.group, bt) : by_group<2, false>(a.group, bt))
+                                        : (bf ? by_group<8, true>(a.group, bt) : by_group<8, false>(a.group, bt));
+    const uint32_t sms = (uint32_t)device_sm_count(), tiles = (a.N + 7u) / 8u;
+    // One row: 32 warps an SM, in four CTAs where a call is short, so that the next one's start comes under the end of this one's (11008 x
+    // 4096, four bits 13.4 us with 4 x 8 warps, 13.6 with 2 x 16, 15.8 with 1 x 24; 28672 x 8192 62.0, 51.5, 54.3); more rows: 24, whose
+    // activations leave no room for more.  Rings of three chunks are no quicker than of two.
+    const bool brief = (uint64_t)tiles * (c.w.row_bytes / 128u) < 400ull * sms;
+    uint32_t per_sm = bt == 1 && brief ? 4u : 2u, warps = bt > 1 ? 12u : brief ? 8u : 16u, slots = 2u;
+    uint32_t grid = std::min(tiles, sms * per_sm);
+    Room room = room_for(c.w, bt, warps, slots, (tiles + grid - 1) / grid);
+    while (room.smem > 226u * 1024u / per_sm) {
+        if (per_sm > 1) { per_sm /= 2; warps = std::min(24u, warps * 2); }
+        else if (warps > 16) warps -= 4;
+        else return (int)cudaErrorNotSupported;
+        grid = std::min(tiles, sms * per_sm);
+        room = room_for(c.w, bt, warps, slots, (tiles + grid - 1) / grid);
     }
+    a.per = tiles / grid;
+    a.more = tiles % grid;
+    a.most = room.most;
+    a.pitch = room.pitch;
+    a.slots = room.slots;
+    CUtensorMap maps[2];
+    for (int i = 0; i < 2; i++)
+        if (!map_2d(maps[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, c.w.codes[i], c.w.row_bytes, c.w.N, c.w.row_bytes, 128, 8, CU_TENSOR_MAP_SWIZZLE_128B)) return (int)cudaErrorNotSupported;
+    if (resident_ctas(reinterpret_cast<const void *>(kern), warps * 32u, room.smem, 1) == 0) return (int)cudaErrorNotSupported;      // (raises the kernel's limit of shared memory)
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(std::min(a.tiles, sms * per_sm));
+    cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(warps * 32u);
-    cfg.dynamicSmemBytes = smem;
+    cfg.dynamicSmemBytes = room.smem;
     cfg.stream = (cudaStream_t)stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = programmatic_launches();
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, kern, a);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a, maps[0], maps[1]);
     count_launch();
     return (int)(e != cudaSuccess ? e : cudaGetLastError());
 }

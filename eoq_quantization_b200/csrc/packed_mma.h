@@ -6,6 +6,8 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
+#include "and_or.h"
+
 namespace eoq {
 namespace {
 
@@ -30,15 +32,6 @@ __device__ __forceinline__ void mma_m16n8k16_first(float (&c)[4], uint32_t a0, u
     else
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
                      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
-}
-
-// (a & b) | c in one instruction: from two immediate operands the compiler makes two, of the half-rate integer pipe (103 of its
-// instructions a warp and span before, 89 now)
-__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c)
-{
-    uint32_t r;
-    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
-    return r;
 }
 
 // two codes, already sitting in the low bits of the two halves of v, to two exact signed 16-bit floats

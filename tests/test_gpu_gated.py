@@ -174,7 +174,7 @@ def test_rows_of_any_magnitude(m, spread):
     inside(gated.packed_input_grad(pg, sg, n, k, 4, 128, dy), dy.double() @ wg, off + 2.0 ** -8 * ((dy.double() @ wg).abs() + off) + 1e-38, "dx")
 
 
-@pytest.mark.parametrize("how", ["strided", "transposed", "misaligned", "three dimensions", "scales cast", "weights off 16 bytes", "no rows"])
+@pytest.mark.parametrize("how", ["strided", "transposed", "misaligned", "three dimensions", "scales cast", "weights off 16 bytes", "scales off 16 bytes", "no rows"])
 @pytest.mark.parametrize("m", [4, 36])
 def test_layouts(how, m):
     n, k = 96, 256
@@ -193,6 +193,8 @@ def test_layouts(how, m):
         sg, su = sg.float(), su.double()
     elif how == "weights off 16 bytes":
         pg, pu, sg, su = off(pg), off(pu), off(sg), off(su)
+    elif how == "scales off 16 bytes":
+        sg, su = off(sg), off(su)
     elif how == "no rows":
         x, dh = x[:0], dh[:0]
     x.requires_grad_()
