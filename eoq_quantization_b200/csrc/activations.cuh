@@ -14,7 +14,7 @@ namespace eoq {
 __device__ __forceinline__ void activation_and_slope(float g, int act, float &value, float &slope)
 {
     if (act == kActSilu) {
-        const float s = 1.0f / (1.0f + __expf(-g));
+        const float s = __fdividef(1.0f, 1.0f + __expf(-g));      // (0 where the sum is beyond 2^126)
         value = g * s;
         slope = s * (1.0f + g * (1.0f - s));
     } else if (act == kActGelu) {

@@ -238,6 +238,11 @@ uint32_t grad_splits(const PackedPair &w, uint32_t M)
 // halves of a row, so that the largest is at 2^14 .. 2^15 and a gradient of any size keeps eleven bits (bf16 would keep eight).
 // The row is gone over twice then, first for its largest value.  Bound by the exponentials at two passes.
 // ---------------------------------------------------------------------------
+__device__ __forceinline__ void set_zeros(const Zeros &z)
+{
+    for (uint32_t i = blockIdx.x * blockDim.x + threadIdx.x; i < z.n; i += gridDim.x * blockDim.x) z.p[i] = 0u;
+}
+
 struct GateGradArgs {
     Kept k;
     const void *dh;
@@ -246,6 +251,7 @@ struct GateGradArgs {
     float *factor;
     uint32_t M, N, pitch;
     int dtype, act;
+    Zeros zeros;
 };
 
 __device__ __forceinline__ void kept_at(const GateGradArgs &a, uint32_t m, uint32_t n, float &g, float &u)
@@ -264,6 +270,7 @@ __device__ __forceinline__ void kept_at(const GateGradArgs &a, uint32_t m, uint3
 __global__ void __launch_bounds__(512) gate_grad_kernel(const GateGradArgs a)
 {
     __shared__ float part[16];
+    set_zeros(a.zeros);
     for (uint32_t m = blockIdx.x; m < a.M; m += gridDim.x) {
         auto at = [&](uint32_t n, float &dg, float &du) {
             float g, u, act, slope;
@@ -314,6 +321,7 @@ template <int DTYPE, bool KEEP8, int ROUNDS>
 __global__ void __launch_bounds__(512) gate_grad_rows_kernel(const GateGradArgs a)
 {
     __shared__ float part[16];
+    set_zeros(a.zeros);
     struct Kept8 { uint2 v; float s; };
     struct Kept16 { Raw8<DTYPE> v; };
     using K = std::conditional_t<KEEP8, Kept8, Kept16>;
@@ -438,11 +446,12 @@ __global__ void __launch_bounds__(256) column_sums_kernel(const SumArgs a)
 
 // bf16 or fp16 rows of multiples of eight values, aligned: read once, kept in registers.
 template <int DTYPE, int ROUNDS>
-__global__ void __launch_bounds__(256) rows_to_half_vector_kernel(const void *__restrict__ x, uint32_t M, uint32_t K, __half *__restrict__ out, float *__restrict__ factor)
+__global__ void __launch_bounds__(256) rows_to_half_vector_kernel(const void *__restrict__ x, uint32_t M, uint32_t K, __half *__restrict__ out, float *__restrict__ factor, const Zeros zeros)
 {
     __shared__ float part[8];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    set_zeros(zeros);
     for (uint32_t m = blockIdx.x; m < M; m += gridDim.x) {
         Raw8<DTYPE> raw[ROUNDS];
         float most = 0.0f;
@@ -476,9 +485,10 @@ __global__ void __launch_bounds__(256) rows_to_half_vector_kernel(const void *__
 }
 
 __global__ void __launch_bounds__(256) rows_to_half_kernel(const void *__restrict__ x, int dtype, uint32_t M, uint32_t K, uint32_t pitch, __half *__restrict__ out,
-                                                           float *__restrict__ factor)
+                                                           float *__restrict__ factor, const Zeros zeros)
 {
     __shared__ float part[8];
+    set_zeros(zeros);
     for (uint32_t m = blockIdx.x; m < M; m += gridDim.x) {
         float most = 0.0f;
         for (uint32_t k = threadIdx.x; k < K; k += 256u) most = fmaxf(most, finite_magnitude(load_as_float(x, (size_t)m * K + k, dtype)));
@@ -587,6 +597,29 @@ int launch_input_grad_general(const PackedPair &w, int nw, const void *const dy[
     return (int)cudaGetLastError();
 }
 
+__global__ void __launch_bounds__(256) zeros_kernel(const Zeros z)
+{
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    set_zeros(z);
+}
+
+int launch_zeros(Zeros zeros, void *stream)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(std::min((zeros.n + 255u) / 256u, 64u));
+    cfg.blockDim = dim3(256);
+    cfg.stream = (cudaStream_t)stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = programmatic_launches();
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, zeros_kernel, zeros);
+    count_launch();
+    return (int)(e != cudaSuccess ? e : cudaGetLastError());
+}
+
 int launch_gate_apply(const float *g, const float *u, size_t count, int act, void *h, int dtype, void *stream)
 {
     gate_apply_kernel<<<ctas_for(count, 256u), 256, 0, (cudaStream_t)stream>>>(g, u, count, act, h, dtype);
@@ -595,9 +628,9 @@ int launch_gate_apply(const float *g, const float *u, size_t count, int act, voi
 }
 
 int launch_gate_grad(const Kept &k, const void *dh, int dtype, int act, uint32_t M, uint32_t N, float *out32[2], uint16_t *half, uint32_t pitch, float *factor,
-                     void *stream)
+                     Zeros zeros, void *stream)
 {
-    GateGradArgs a = {k, dh, {out32 ? out32[0] : nullptr, out32 ? out32[1] : nullptr}, (__half *)half, factor, M, N, pitch, dtype, act};
+    GateGradArgs a = {k, dh, {out32 ? out32[0] : nullptr, out32 ? out32[1] : nullptr}, (__half *)half, factor, M, N, pitch, dtype, act, zeros};
     const bool k8 = k.form == kKeep8bit;
     if (half && dtype != EOQ_B200_F32 && N % 8u == 0 && pitch == N && N <= 7u * 4096u && aligned(dh, 16) && aligned(k.v[0], 16) && aligned(k.v[1], 16) && aligned(half, 16)) {
 #define EOQ_GATE(D, R) (k8 ? gate_grad_rows_kernel<D, true, R> : gate_grad_rows_kernel<D, false, R>)
@@ -630,7 +663,7 @@ int launch_column_sums(const float *const in32[2], const uint16_t *half, uint32_
     return (int)cudaGetLastError();
 }
 
-int launch_rows_to_half(const void *x, int dtype, uint32_t M, uint32_t K, uint32_t pitch, uint16_t *out, float *factor, void *stream)
+int launch_rows_to_half(const void *x, int dtype, uint32_t M, uint32_t K, uint32_t pitch, uint16_t *out, float *factor, Zeros zeros, void *stream)
 {
     if (dtype != EOQ_B200_F32 && K % 8u == 0 && pitch == K && K <= 16384u && aligned(x, 16)) {
 #define EOQ_ROWS(D) (K <= 2048u ? rows_to_half_vector_kernel<D, 1> : K <= 4096u ? rows_to_half_vector_kernel<D, 2> : rows_to_half_vector_kernel<D, 8>)
@@ -645,11 +678,11 @@ int launch_rows_to_half(const void *x, int dtype, uint32_t M, uint32_t K, uint32
         attr[0].val.programmaticStreamSerializationAllowed = programmatic_launches();
         cfg.attrs = attr;
         cfg.numAttrs = 1;
-        const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, x, M, K, (__half *)out, factor);
+        const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, x, M, K, (__half *)out, factor, zeros);
         count_launch();
         return (int)(e != cudaSuccess ? e : cudaGetLastError());
     }
-    rows_to_half_kernel<<<std::min(M, 65535u), 256, 0, (cudaStream_t)stream>>>(x, dtype, M, K, pitch, (__half *)out, factor);
+    rows_to_half_kernel<<<std::min(M, 65535u), 256, 0, (cudaStream_t)stream>>>(x, dtype, M, K, pitch, (__half *)out, factor, zeros);
     count_launch();
     return (int)cudaGetLastError();
 }

@@ -46,22 +46,30 @@ size_t input_grad_general_scratch(const PackedPair &w, uint32_t M);
 
 // dg = dh u act'(g), du = dh act(g): fp32 [M][N] each, or (half) fp16 [2][M][pitch] times a power of two of the row, whose inverse
 // goes to factor[m]; the pad of a row is zero.
+// zeros: words that are set to zero besides (a later kernel's counters).
+struct Zeros { uint32_t *p; uint32_t n; };
 int launch_gate_grad(const Kept &k, const void *dh, int dtype, int act, uint32_t M, uint32_t N, float *out32[2], uint16_t *half, uint32_t pitch, float *factor,
-                     void *stream);
+                     Zeros zeros, void *stream);
+int launch_zeros(Zeros zeros, void *stream);
 // Sums over the rows: of fp32 [M][N] x 2, or of the form above.  scratch: column_sums_scratch() bytes.
 int launch_column_sums(const float *const in32[2], const uint16_t *half, uint32_t pitch, const float *factor, uint32_t M, uint32_t N, float *scratch,
                        float *out[2], void *stream);
 size_t column_sums_scratch(uint32_t M, uint32_t N);
 // Rows to fp16, pitch values apart (a multiple of 8; the pad is zero), times a power of two that brings the largest to 2^14 .. 2^15.
-int launch_rows_to_half(const void *x, int dtype, uint32_t M, uint32_t K, uint32_t pitch, uint16_t *out, float *factor, void *stream);
+int launch_rows_to_half(const void *x, int dtype, uint32_t M, uint32_t K, uint32_t pitch, uint16_t *out, float *factor, Zeros zeros, void *stream);
 
 // h = act(g) u of fp32 [M][N].
 int launch_gate_apply(const float *g, const float *u, size_t count, int act, void *h, int dtype, void *stream);
 // The tensor-core forms (gated_product.cu): whole groups per row, groups of 32 columns and their multiples, rows of codes that are
-// multiples of 16 bytes, everything 16-byte aligned.  x, dy: fp16, [M][K] and [nw][M][pitch], pitch a multiple of 8.
+// multiples of 16 bytes, everything 16-byte aligned.  x, dy: fp16, [M][K] and [nw][M][pitch], pitch a multiple of 8.  Scratch: bytes,
+// of which the first `zeros` words are zero when the kernel before has ended.
+struct Scratch { size_t bytes; uint32_t zeros; };
 bool product_takes(const PackedPair &w, int nw);
-int launch_gated_product(const GatedCall &c, const uint16_t *x, const float *factor, void *stream);
-int launch_input_grad_product(const PackedPair &w, int nw, const uint16_t *dy, uint32_t pitch, const float *factor, uint32_t M, void *dx, int dtype, void *stream);
+Scratch gated_product_scratch(const PackedPair &w, uint32_t M);
+Scratch input_grad_product_scratch(const PackedPair &w, int nw, uint32_t M);
+int launch_gated_product(const GatedCall &c, const uint16_t *x, const float *factor, void *scratch, void *stream);
+int launch_input_grad_product(const PackedPair &w, int nw, const uint16_t *dy, uint32_t pitch, const float *factor, uint32_t M, void *dx, int dtype, void *scratch,
+                              void *stream);
 // Up to eight rows of 16-bit activations, 16-byte aligned; kept in full or in fp32 (gated_rows.cu).
 bool gated_rows_takes(const PackedPair &w, uint32_t batch);
 int launch_gated_rows(const GatedCall &c, void *stream);

@@ -83,6 +83,7 @@ extern "C" size_t eoq_b200_gated_scratch(const eoq_b200_gated_t *w, const eoq_b2
     if (product_takes(pair_of(w), 2)) {
         c.take<void>(half_bytes(batch, w->cols));
         c.take<float>((size_t)batch * 4);
+        c.take<void>(gated_product_scratch(pair_of(w), batch).bytes);
         if (!few_rows(pair_of(w), dtype, batch)) return c.at;
     }
     const size_t sums = form == kKeep8bit ? 2 * values(batch, w->rows) * 4 : 0;
@@ -119,13 +120,16 @@ extern "C" eoq_error_t eoq_b200_gated_packed(const eoq_b200_gated_t *w, const vo
     if (dtype != EOQ_B200_F32 && product_takes(c.w, 2)) {
         uint16_t *half = scratch.take<uint16_t>(half_bytes(batch, w->cols));
         float *factor = scratch.take<float>((size_t)batch * 4);
+        const Scratch s = gated_product_scratch(c.w, batch);
+        uint32_t *parts = scratch.take<uint32_t>(s.bytes);
         if (as_it_is(x, dtype, w->cols)) {
             half = static_cast<uint16_t *>(const_cast<void *>(x));
             factor = nullptr;
+            e = launch_zeros(Zeros{parts, s.zeros}, stream);
         } else {
-            e = launch_rows_to_half(x, dtype, batch, w->cols, pitch_of(w->cols), half, factor, stream);
+            e = launch_rows_to_half(x, dtype, batch, w->cols, pitch_of(w->cols), half, factor, Zeros{parts, s.zeros}, stream);
         }
-        if (e == 0) e = launch_gated_product(c, half, factor, stream);
+        if (e == 0) e = launch_gated_product(c, half, factor, parts, stream);
         return launched(e, where);
     }
     if (exact_products(c.w, dtype, w->gate, d_scratch) && exact_products(c.w, dtype, w->up, d_scratch)) {
@@ -166,6 +170,7 @@ extern "C" size_t eoq_b200_gated_grad_scratch(const eoq_b200_gated_t *w, const e
     if (dtype != EOQ_B200_F32 && product_takes(pair_of(w), 2)) {
         c.take<void>(2 * half_bytes(batch, w->rows));
         c.take<float>((size_t)batch * 4);
+        c.take<void>(input_grad_product_scratch(pair_of(w), 2, batch).bytes);
         c.take<void>(column_sums_scratch(batch, w->rows));
         return c.at;
     }
@@ -191,15 +196,18 @@ extern "C" eoq_error_t eoq_b200_gated_grad(const eoq_b200_gated_t *w, const eoq_
     if (dtype != EOQ_B200_F32 && product_takes(pair, 2)) {
         const uint32_t pitch = pitch_of(w->rows);
         uint16_t *half = scratch.take<uint16_t>(2 * half_bytes(batch, w->rows));
-        float *factor = scratch.take<float>((size_t)batch * 4), *sums = scratch.take<float>(0);
-        int e = launch_gate_grad(kept_of(kept), dh, dtype, w->activation, batch, w->rows, nullptr, half, pitch, factor, stream);
+        float *factor = scratch.take<float>((size_t)batch * 4);
+        const Scratch s = input_grad_product_scratch(pair, 2, batch);
+        uint32_t *parts = scratch.take<uint32_t>(s.bytes);
+        float *sums = scratch.take<float>(0);
+        int e = launch_gate_grad(kept_of(kept), dh, dtype, w->activation, batch, w->rows, nullptr, half, pitch, factor, Zeros{parts, s.zeros}, stream);
         if (e == 0 && (d_gate_bias || d_up_bias)) e = launch_column_sums(nullptr, half, pitch, factor, batch, w->rows, sums, to, stream);
-        if (e == 0 && dx) e = launch_input_grad_product(pair, 2, half, pitch, factor, batch, dx, dtype, stream);
+        if (e == 0 && dx) e = launch_input_grad_product(pair, 2, half, pitch, factor, batch, dx, dtype, parts, stream);
         return launched(e, where);
     }
     float *d = scratch.take<float>(2 * n * 4), *out[2] = {d, d + n};
     void *sums = scratch.take<void>(0);
-    int e = launch_gate_grad(kept_of(kept), dh, dtype, w->activation, batch, w->rows, out, nullptr, 0, nullptr, stream);
+    int e = launch_gate_grad(kept_of(kept), dh, dtype, w->activation, batch, w->rows, out, nullptr, 0, nullptr, Zeros{nullptr, 0}, stream);
     if (e == 0 && (d_gate_bias || d_up_bias)) e = launch_column_sums(out, nullptr, 0, nullptr, batch, w->rows, static_cast<float *>(sums), to, stream);
     if (e == 0 && dx) {
         const void *dy[2] = {out[0], out[1]};
@@ -217,6 +225,7 @@ extern "C" size_t eoq_b200_packed_input_grad_scratch(uint32_t rows, uint32_t col
     Carve c{nullptr};
     c.take<void>(half_bytes(batch, rows));
     c.take<float>((size_t)batch * 4);
+    c.take<void>(input_grad_product_scratch(p, 1, batch).bytes);
     return std::max(c.at, any);
 }
 
@@ -233,14 +242,17 @@ extern "C" eoq_error_t eoq_b200_packed_input_grad(const uint8_t *d_packed, const
         Carve scratch{static_cast<uint8_t *>(d_scratch)};
         uint16_t *half = scratch.take<uint16_t>(half_bytes(batch, rows));
         float *factor = scratch.take<float>((size_t)batch * 4);
+        const Scratch s = input_grad_product_scratch(p, 1, batch);
+        uint32_t *parts = scratch.take<uint32_t>(s.bytes);
         int e = 0;
         if (as_it_is(dy, dtype, rows)) {
             half = static_cast<uint16_t *>(const_cast<void *>(dy));
             factor = nullptr;
+            e = launch_zeros(Zeros{parts, s.zeros}, stream);
         } else {
-            e = launch_rows_to_half(dy, dtype, batch, rows, pitch_of(rows), half, factor, stream);
+            e = launch_rows_to_half(dy, dtype, batch, rows, pitch_of(rows), half, factor, Zeros{parts, s.zeros}, stream);
         }
-        if (e == 0) e = launch_input_grad_product(p, 1, half, pitch_of(rows), factor, batch, dx, dtype, stream);
+        if (e == 0) e = launch_input_grad_product(p, 1, half, pitch_of(rows), factor, batch, dx, dtype, parts, stream);
         return launched(e, "eoq_b200_packed_input_grad");
     }
     const void *d[2] = {dy, dy};

@@ -2,10 +2,12 @@
 //   forward   h[m][n] = act(g + bg) (u + bu),  g = sum over k of x[m][k] wg[n][k], u likewise
 //   gradient  dx[m][k] = sum over n of dg[m][n] wg[n][k] + du[m][n] wu[n][k]   (or of one weight)
 //
-// Both are products of a weight tile of 128 rows, which is the A operand and lives in tensor memory, with up to 256 tokens,
-// which are the B operand, brought by TMA (128-byte swizzle).  Packed codes come by TMA too; producer warps turn them into
-// code x scale, rounded to fp16 once, and store them to tensor memory, so that a dequantised weight touches neither global nor
-// shared memory.  Activations are fp16, with one power of two per row where they were something else.
+// Both are products of weight tiles of 256 rows, which are the A operand and live in the tensor memory of two SMs (cta_group::2,
+// 128 rows each), with up to 256 tokens, which are the B operand, brought by TMA (128-byte swizzle), half to each SM: alone, an SM
+// would need 64 bytes of activations a clock to keep its tensor cores busy, which is more than the L2 gives all of them.  Packed codes
+// come by TMA too; producer warps turn them into code x scale, rounded to fp16 once, and store them to tensor memory, so that a
+// dequantised weight touches neither global nor shared memory.  Activations are fp16, with one power of two per row where they were
+// something else.
 //
 //   forward: a CTA's 128 rows are 64 features of the gate and the same 64 of the up projection, so that h is made where both
 // sums are, on the way out.  A thread owns a row and turns 64 of its codes at a time into A's 32 columns.
@@ -15,14 +17,20 @@
 // half: what masking and a packed multiply-add make of it is a pair along the products' axis.  Its lanes are then sets of
 // columns, not neighbouring ones; tensor memory takes them in that order, and the way out puts them back (`place`).
 //
-// Few tiles: the products' axis is split over the CTAs of a cluster, which add their sums up through distributed shared memory,
-// in a fixed order.  Waits are bounded, as in the product kernel for one weight (qmm.cu): one that runs out marks the CTA,
-// whose results become NaN, and sets a status word.
+// The grid is as many CTA pairs as the device holds, and the work, tile after tile along the products' axis, is cut into as many equal
+// runs: a pair takes the end of one tile, whole ones, and the beginning of another, and nothing waits for a last, partly filled round.
+// Sums of a tile that several pairs share go to scratch; whoever comes last, by the tile's counter, adds them up in the order of the
+// pairs and finishes the tile, so results do not depend on who that is.  Copies, conversion and products run on from one tile to the next
+// while four warps bring the last one out; two accumulators take turns where tensor memory has room for them (192 tokens).
+//
+// Waits are bounded, as in the product kernel for one weight (qmm.cu): one that runs out marks the CTA, whose results become NaN,
+// and sets a status word.
 #include "gated.h"
 #include "tensor_core.h"
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cooperative_groups.h>
 
 #include "activations.cuh"
@@ -37,7 +45,8 @@ namespace {
 
 constexpr uint32_t kRows = 128;            // of a weight tile
 constexpr int kSets = 4;                   // producer sets of four warps, one per quadrant of tensor memory
-constexpr uint32_t kThreads = (4 * kSets + 4) * 32, kTmem = 512;
+constexpr int kWProducts = 4 * kSets, kWCodes = kWProducts + 1, kWTokens = kWProducts + 2, kWScales = kWProducts + 3, kWOut = kWProducts + 4;      // warps
+constexpr uint32_t kThreads = (kWOut + 4) * 32, kTmem = 512, kOut = 8 * 2048 + 8 * 128;       // shared memory of the way out: sixteen tokens of a warp, and their maxima, twice
 
 struct ProductArgs {
     const uint16_t *scales[2];   // [N][groups] fp16
@@ -45,47 +54,90 @@ struct ProductArgs {
     const float *factor;         // [M] or null
     void *y;                     // [M][N] or, gradient, [M][K]
     Kept keep;                   // forward
-    uint32_t N, K, M, T, group, groups, units, per_weight, split;
-    uint32_t nw, ns;             // stages of packed weights and of operands
-    uint32_t at_x, at_bar;       // shared-memory offsets
+    float *partial;              // [pairs][2][2][T][128]: sums of tiles that a pair's run begins (0) or ends (1) in the middle of
+    uint32_t *count;             // [tiles][2], zero: parts of a tile that have arrived
+    uint32_t N, K, M, T, group, groups;
+    uint32_t tok_tiles, tiles, per_tile, per_weight;         // of the grid of tiles; pieces of a tile's axis, of one weight's
+    uint32_t nw, ns, nd;         // stages of packed weights and of operands, accumulators
+    uint32_t at_x, at_out, at_bar;       // shared-memory offsets
+    uint32_t inverse;            // group_of
     int dtype, act;
     long long limit;             // clock ticks a wait may take
 };
 
-// Two words of shared memory at `mark`: the CTA has given up; the kernels before this one have ended (their time does not count).
+__device__ __forceinline__ uint32_t in_cta(uint32_t addr, uint32_t rank)
+{
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+// at a barrier of either CTA.  What is handed over lies in tensor memory, whose order tcgen05's fences keep: without a scope of the cluster, which
+// costs a fence of memory each time (920 clocks a block of 16 tokens, against 330).
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
+// a copy to this CTA whose bytes are counted by a barrier of either CTA of the pair
+__device__ __forceinline__ void tma_2d_pair(uint32_t dst, const CUtensorMap *map, uint32_t x, uint32_t y, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void mma_pair(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile("{\n\t.reg .pred e, p;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+                 "@e tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+// arrives at this barrier of both CTAs when the products so far are done
+__device__ __forceinline__ void commit_pair(uint32_t bar)
+{
+    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+                 "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(bar), "h"((uint16_t)3) : "memory");
+}
+
+// A wait that may sleep for a millisecond: warps that ask again and again take the issue slots of those that work.
+__device__ __forceinline__ bool bar_try_long(uint32_t bar, uint32_t parity)
+{
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok) : "r"(bar), "r"(parity), "r"(1000000u) : "memory");
+    return ok != 0;
+}
+
+// Two words of shared memory at `mark`: the CTA has given up; the kernels before this one have ended (their time does not count).  A warp
+// whose wait has run out is `lost`: it runs on, but requests no copies and tells no barriers (an arrival beyond a barrier's count while a copy is
+// under way would break it), so that the others' waits run out too.
 struct Patience {
     uint32_t mark;
     long long limit;
+    bool lost = false;
+    __device__ __forceinline__ Patience(uint32_t m, long long l) : mark(m), limit(l) {}
     __device__ __forceinline__ bool stopped() const
     {
         uint32_t v;
         asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(v) : "r"(mark) : "memory");
         return v != 0;
     }
-    __device__ __forceinline__ void operator()(uint32_t bar, uint32_t parity) const
+    __device__ __forceinline__ void operator()(uint32_t bar, uint32_t parity)
     {
-        if (!bar_try(bar, parity)) slow(bar, parity, mark, limit);
+        if (!bar_try(bar, parity)) lost = slow(bar, parity, mark, limit) || lost;
     }
-    // the same, and whether the CTA has not given up: a copy is requested then only
-    __device__ __forceinline__ bool go(uint32_t bar, uint32_t parity) const
-    {
-        (*this)(bar, parity);
-        return !stopped();
-    }
-    static __device__ __noinline__ void slow(uint32_t bar, uint32_t parity, uint32_t mark, long long limit)
+    static __device__ __noinline__ bool slow(uint32_t bar, uint32_t parity, uint32_t mark, long long limit)
     {
         long long t0 = clock64();
-        while (!bar_try(bar, parity)) {
+        bool gave_up = false;
+        while (!gave_up && !(limit ? bar_try_long(bar, parity) : bar_try(bar, parity))) {
             const long long now = clock64();
             uint32_t stop, alone;
             asm volatile("ld.volatile.shared.v2.u32 {%0, %1}, [%2];" : "=r"(stop), "=r"(alone) : "r"(mark) : "memory");
             if (!alone && limit) t0 = now;
             // once a launch has given up, the others of a grid of many rounds wait an eighth as long
-            if (!stop && now - t0 <= limit && !(now - t0 > limit / 8 && *reinterpret_cast<volatile uint32_t *>(&g_gated_status))) continue;
+            gave_up = stop || now - t0 > limit || (now - t0 > limit / 8 && *reinterpret_cast<volatile uint32_t *>(&g_gated_status));
+        }
+        gave_up = __any_sync(0xffffffffu, gave_up);
+        if (gave_up) {
             asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(mark), "r"(1u) : "memory");
             *reinterpret_cast<volatile uint32_t *>(&g_gated_status) = 1u;
-            return;
         }
+        return gave_up;
     }
 };
 
@@ -98,9 +150,9 @@ struct Piece {
     static constexpr uint32_t kStage = kRows * kBytes;
 };
 
-// barriers, eight bytes each
-enum { bWFull = 0, bWEmpty = 8, bFull = 16, bEmpty = 24, bDone = 32, bSFull = 40, bSEmpty = 44, bTmem = 48, bDrain = 49, bMark = 50, bUsedW = 51, bUsedX = 52 };
-constexpr uint32_t kScaleRing = 4, kScaleEntry = 8u * kRows * 2u;      // forward: 8 groups x 128 rows an entry; gradient: up to 4 groups x 128
+// barriers, eight bytes each.  Of a pair's first CTA both use Full (its products' warp waits for both CTAs' operands) and OutEmpty.
+enum { bWFull = 0, bWEmpty = 8, bFull = 16, bEmpty = 24, bOutFull = 32, bOutEmpty = 34, bTmem = 36, bDrain = 37, bMark = 38, bUsedW = 39, bTicket = 40, bEnd = 41 };
+constexpr uint32_t kScales = 8u * kRows * 2u;      // of a stage of codes: forward, up to 8 groups x 128 rows; gradient, up to 4 groups x 128
 
 __device__ __forceinline__ void ldmatrix_trans(uint32_t addr, uint32_t (&r)[4])
 {
@@ -151,446 +203,558 @@ gated_product_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap gm
     const uint32_t base = saddr(smem), bars = base + a.at_bar;
     auto bar = [&](uint32_t i) { return bars + 8u * i; };
     auto word = [&](uint32_t i) { return reinterpret_cast<volatile uint32_t *>(smem + a.at_bar + 8u * i); };
-    const Patience wait{bar(bMark), a.limit};
-    const uint32_t scale_ring = bars + 512u;
+    Patience wait(bar(bMark), a.limit);
+    const uint32_t scales_at = bars + 8u * bEnd + 8u;
     const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31u;
-    const uint32_t rank = blockIdx.x % a.split, tile = blockIdx.x / a.split, tok0 = blockIdx.y * a.T;
-    const uint32_t row0 = tile * (GRAD ? 128u : 64u);                // first column, or feature
-    const uint32_t u0 = (uint32_t)((uint64_t)a.units * rank / a.split), u1 = (uint32_t)((uint64_t)a.units * (rank + 1) / a.split);
-    // forward: the last piece's blocks past the last column are left out; gradient: rows past the last one are zeros
-    const uint32_t kb0 = u0 * P::kBlocks, nkb = (GRAD ? u1 * P::kBlocks : min(u1 * P::kBlocks, (a.K + 63u) / 64u)) - kb0;
-    const uint32_t xstage = a.T * 128u, a_base = a.T;
-    const uint32_t grp0 = kb0 * 64u / a.group, ngroups = GRAD ? 0u : (min((kb0 + nkb) * 64u, a.K) - 1u) / a.group - grp0 + 1u;
+    const uint32_t rank = blockIdx.x & 1u, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const uint32_t xstage = a.T * 64u, a_base = a.nd * a.T;          // half of a block's tokens; first column of A
+    constexpr uint32_t kWide = GRAD ? 128u : 64u;                    // columns, or features, of a CTA's tile
+
+    // A pair's run of pieces, and its parts of tiles in order
+    auto run_start = [&](uint32_t p) { return (uint64_t)a.tiles * a.per_tile * p / pairs; };
+    const uint64_t run0 = run_start(pair), run1 = run_start(pair + 1);
+    struct Part { uint32_t tile, p0, p1, blocks; };                  // pieces [p0, p1) of a tile, in blocks of 64
+    auto part_at = [&](uint64_t at) {
+        Part s;
+        s.tile = (uint32_t)(at / a.per_tile);
+        s.p0 = (uint32_t)(at - (uint64_t)s.tile * a.per_tile);
+        s.p1 = (uint32_t)min((uint64_t)a.per_tile, s.p0 + (run1 - at));
+        // forward: the last piece's blocks past the last column are left out; gradient: rows past the last one are zeros
+        s.blocks = (GRAD ? s.p1 * P::kBlocks : min(s.p1 * P::kBlocks, (a.K + 63u) / 64u)) - s.p0 * P::kBlocks;
+        return s;
+    };
+    // tokens fastest: the pairs that run at the same time share codes, which come from HBM, rather than activations, which the L2 holds
+    auto first_row = [&](uint32_t tile) { return (tile / a.tok_tiles * 2u + rank) * kWide; };
+    // k / group for groups of 32 columns and their multiples: with d = group / 16 and the inverse 2^32 / d rounded up, exact while (k / 16) d < 2^32
+    auto group_of = [&](uint32_t k) { return __umulhi(k >> 4, a.inverse); };
+    auto first_token = [&](uint32_t tile) { return tile % a.tok_tiles * a.T; };
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < 8; i++) {
-            bar_init(bar(bWFull + i), 1); bar_init(bar(bWEmpty + i), 4 * P::kBlocks);
-            bar_init(bar(bFull + i), 5); bar_init(bar(bEmpty + i), 1);          // four producer warps and the activation copy
+            bar_init(bar(bWFull + i), 2); bar_init(bar(bWEmpty + i), 4 * kSets);           // the copy and the scales; every producer warp
+            bar_init(bar(bFull + i), 9); bar_init(bar(bEmpty + i), 1);                     // four producer warps of either CTA and the copies' bytes
         }
-        for (uint32_t i = 0; i < kScaleRing; i++) { bar_init(bar(bSFull + i), 1); bar_init(bar(bSEmpty + i), 4 * (GRAD ? P::kBlocks : kSets)); }
-        bar_init(bar(bDone), 1);
+        for (uint32_t i = 0; i < 2; i++) { bar_init(bar(bOutFull + i), 1); bar_init(bar(bOutEmpty + i), 8); }
         bar_init(bar(bDrain), 1);
         word(bMark)[0] = word(bMark)[1] = 0u;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncwarp();
-    if (warp == 4 * kSets) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(bar(bTmem)), "n"(kTmem) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if (warp == kWProducts) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(bar(bTmem)), "n"(kTmem) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
     fence_before();
     __syncthreads();
+    cg::this_cluster().sync();                 // both CTAs' barriers are there before either arrives at the other's
     fence_after();
     constexpr uint32_t tmem = 0;               // all 512 columns are this CTA's
 
     if (warp < 4 * kSets) {
-        // ---- producers: codes, a block of 64 along the products' axis at a time, to the A operand in tensor memory
+        // ---- producers: codes, a block of 64 along the products' axis at a time, to the A operand in tensor memory.  The sets take the
+        // blocks in turn, through all parts; every warp comes by every piece and gives it back.
         const uint32_t set = warp >> 2, q = warp & 3u, r = q * 32u + lane;
-        const uint32_t lane_base = tmem + ((q * 32u) << 16) + a_base;
-        Ring wr, ar, sr;
-        uint32_t unit = 0, entry = 0, gi = 0, pos = 0;
-        bool here = false;
-        if (!GRAD) { const uint32_t c = (kb0 + set) * 64u; gi = c / a.group; pos = c - gi * a.group; gi -= grp0; }
-        // forward: scales of this row in the order of the groups, out of the ring
-        auto scale_of = [&](uint32_t g) {
-            while ((g >> 3) > entry) {
-                __syncwarp();
-                if (lane == 0) bar_arrive(bar(bSEmpty + sr.at));
-                sr.next(kScaleRing);
-                entry++;
-                here = false;
-            }
-            if (!here) { wait(bar(bSFull + sr.at), sr.lap); here = true; }
-            uint16_t v;
-            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(scale_ring + sr.at * kScaleEntry + (g & 7u) * (kRows * 2u) + r * 2u));
-            return v;
-        };
+        const uint32_t lane_base = tmem + ((q * 32u) << 16) + a_base, full0 = in_cta(bar(bFull), 0u);
+        Ring wr, ar;
         for (uint32_t j = 0; j < set; j++) ar.next(a.ns);
-        for (uint32_t i = set; i < nkb; i += kSets) {
-            const uint32_t qb = i % P::kBlocks, st = ar.at;
-            for (; unit < i / P::kBlocks; unit++) { wr.next(a.nw); if (GRAD) sr.next(kScaleRing); }
-            const uint32_t ws = wr.at;
-            wait(bar(bWFull + ws), wr.lap);
-            if constexpr (!GRAD) {
-                constexpr int kWords = BITS == 4 ? 8 : BITS == 2 ? 4 : 16;
-                const uint32_t row_at = base + ws * P::kStage + r * P::kBytes, sw = BITS == 2 ? (r >> 1) & 3u : r & 7u;
-                uint32_t w[kWords], h[32];
+        uint32_t turn = set;                   // blocks until this set's next one
+        for (uint64_t at = run0; at < run1;) {
+            const Part s = part_at(at);
+            at += s.p1 - s.p0;
+            const uint32_t row0 = first_row(s.tile);
+            for (uint32_t p = s.p0; p < s.p1; p++, wr.next(a.nw)) {
+                const uint32_t have = GRAD ? P::kBlocks : min(P::kBlocks, (a.K + 63u) / 64u - p * P::kBlocks), ws = wr.at;
+                wait(bar(bWFull + ws), wr.lap);
+                for (; turn < have; turn += kSets) {
+                    const uint32_t st = ar.at;
+                    if constexpr (!GRAD) {
+                        constexpr int kWords = BITS == 4 ? 8 : BITS == 2 ? 4 : 16;
+                        const uint32_t row_at = base + ws * P::kStage + r * P::kBytes, sw = BITS == 2 ? (r >> 1) & 3u : r & 7u;
+                        uint32_t w[kWords], h[32];
 #pragma unroll
-                for (uint32_t c = 0; c < kWords / 4; c++)
-                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[4 * c]), "=r"(w[4 * c + 1]), "=r"(w[4 * c + 2]), "=r"(w[4 * c + 3])
-                                 : "r"(row_at + (((qb * (kWords / 4) + c) ^ sw) << 4)));
-                const uint16_t s0 = scale_of(gi);
-                const bool other = pos + 32u >= a.group && (kb0 + i) * 64u + 32u < a.K;
-                const uint16_t s1 = other ? scale_of(gi + 1u) : s0;
-                for (pos += 64u * kSets; pos >= a.group; pos -= a.group) gi++;
+                        for (uint32_t c = 0; c < kWords / 4; c++)
+                            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[4 * c]), "=r"(w[4 * c + 1]), "=r"(w[4 * c + 2]), "=r"(w[4 * c + 3])
+                                         : "r"(row_at + (((turn * (kWords / 4) + c) ^ sw) << 4)));
+                        // the groups of the block's halves, counted from the piece's first
+                        const uint32_t c0 = p * P::kAlong, g0 = group_of(c0), k = c0 + turn * 64u;
+                        uint16_t sc[2];
 #pragma unroll
-                for (int c = 0; c < kWords; c++) codes_scaled<BITS, false>(w[c], h + c * (32 / kWords), c < kWords / 2 ? s0 : s1);
-                wait(bar(bEmpty + st), ar.lap ^ 1u);
-                fence_after();
-                __syncwarp();
-                tmem_st32(lane_base + st * 32u, h);
-            } else {
-                constexpr int kChunks = BITS == 8 ? 2 : 1;            // 16-byte pieces of a weight row that a quadrant's 32 columns take
-                const uint32_t rows_at = base + ws * P::kStage, chunk = BITS == 4 ? q : BITS == 8 ? 2u * q : q >> 1;
-                // scales of neighbouring weight rows at this lane's columns' group
-                const uint32_t col = place<true, BITS>(q, lane >> 2), gl = (row0 + col) / a.group - row0 / a.group;
-                wait(bar(bSFull + sr.at), sr.lap);
-                uint32_t sp[8];
+                        for (uint32_t j = 0; j < 2; j++)
+                            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(sc[j]) : "r"(scales_at + ws * kScales + (group_of(min(k + j * 32u, a.K - 1u)) - g0) * (kRows * 2u) + r * 2u));
 #pragma unroll
-                for (uint32_t b = 0; b < 8; b++)
-                    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(sp[b]) : "r"(scale_ring + sr.at * kScaleEntry + gl * (kRows * 2u) + qb * 128u + b * 16u + (lane & 3u) * 4u));
-                uint32_t m[kChunks][2][4];
+                        for (int c = 0; c < kWords; c++) codes_scaled<BITS, false>(w[c], h + c * (32 / kWords), c < kWords / 2 ? sc[0] : sc[1]);
+                        wait(bar(bEmpty + st), ar.lap ^ 1u);
+                        fence_after();
+                        __syncwarp();
+                        tmem_st32(lane_base + st * 32u, h);
+                    } else {
+                        constexpr int kChunks = BITS == 8 ? 2 : 1;            // 16-byte pieces of a weight row that a quadrant's 32 columns take
+                        const uint32_t rows_at = base + ws * P::kStage, chunk = BITS == 4 ? q : BITS == 8 ? 2u * q : q >> 1;
+                        // scales of neighbouring weight rows at this lane's columns' group
+                        const uint32_t gl = group_of(row0 + place<true, BITS>(q, lane >> 2)) - group_of(row0);
+                        uint32_t sp[8];
 #pragma unroll
-                for (uint32_t c = 0; c < kChunks; c++)
+                        for (uint32_t b = 0; b < 8; b++)
+                            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(sp[b]) : "r"(scales_at + ws * kScales + gl * (kRows * 2u) + turn * 128u + b * 16u + (lane & 3u) * 4u));
+                        uint32_t m[kChunks][2][4];
 #pragma unroll
-                    for (uint32_t hh = 0; hh < 2; hh++) {
-                        const uint32_t n = qb * 64u + hh * 32u + lane, sw = BITS == 8 ? n & 7u : BITS == 4 ? (n >> 1) & 3u : (n >> 2) & 1u;
-                        ldmatrix_trans(rows_at + n * P::kBytes + (((chunk + c) ^ sw) << 4), m[c][hh]);
+                        for (uint32_t c = 0; c < kChunks; c++)
+#pragma unroll
+                            for (uint32_t hh = 0; hh < 2; hh++) {
+                                const uint32_t n = turn * 64u + hh * 32u + lane, sw = BITS == 8 ? n & 7u : BITS == 4 ? (n >> 1) & 3u : (n >> 2) & 1u;
+                                ldmatrix_trans(rows_at + n * P::kBytes + (((chunk + c) ^ sw) << 4), m[c][hh]);
+                            }
+                        // sixteen lanes of tensor memory at a time: code j of the registers to lanes 0 .. 7, code j + 1 to lanes 8 .. 15
+                        uint32_t h[2][16];
+#pragma unroll
+                        for (int half = 0; half < 2; half++)
+#pragma unroll
+                            for (int b = 0; b < 8; b++)
+#pragma unroll
+                                for (int j = 0; j < 2; j++) {
+                                    uint32_t v = m[BITS == 8 ? half : 0][b >> 2][b & 3];
+                                    if (BITS == 2) v >>= (q & 1u) * 8u;
+                                    h[half][2 * b + j] = hmul2(row_pair<BITS>(v, (BITS == 8 ? 0 : 2 * half) + j), sp[b]);
+                                }
+                        wait(bar(bEmpty + st), ar.lap ^ 1u);
+                        fence_after();
+                        __syncwarp();
+                        tmem_st_16x128b(lane_base + st * 32u, h[0]);
+                        tmem_st_16x128b(lane_base + (16u << 16) + st * 32u, h[1]);
                     }
-                // sixteen lanes of tensor memory at a time: code j of the registers to lanes 0 .. 7, code j + 1 to lanes 8 .. 15
-                uint32_t h[2][16];
-#pragma unroll
-                for (int half = 0; half < 2; half++)
-#pragma unroll
-                    for (int b = 0; b < 8; b++)
-#pragma unroll
-                        for (int j = 0; j < 2; j++) {
-                            uint32_t v = m[BITS == 8 ? half : 0][b >> 2][b & 3];
-                            if (BITS == 2) v >>= (q & 1u) * 8u;
-                            h[half][2 * b + j] = hmul2(row_pair<BITS>(v, (BITS == 8 ? 0 : 2 * half) + j), sp[b]);
-                        }
-                wait(bar(bEmpty + st), ar.lap ^ 1u);
-                fence_after();
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    fence_before();
+                    __syncwarp();
+                    // (a CTA that has given up tells nobody: an arrival beyond a barrier's count while a copy is under way would break it)
+                    if (lane == 0 && !wait.lost) arrive_cluster(full0 + 8u * st);
+                    ar.at += kSets;
+                    if (ar.at >= a.ns) { ar.at -= a.ns; ar.lap ^= 1u; }
+                }
+                turn -= have;
+                // every lane's codes are converted and stored: only now may the copy engine have the stage
                 __syncwarp();
-                tmem_st_16x128b(lane_base + st * 32u, h[0]);
-                tmem_st_16x128b(lane_base + (16u << 16) + st * 32u, h[1]);
+                if (lane == 0 && !wait.lost) bar_arrive(bar(bWEmpty + ws));
             }
-            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-            fence_before();
-            __syncwarp();
-            // every lane's codes are converted and stored: only now may the copy engine have the stage.  A CTA that has given up
-            // tells nobody (an arrival beyond a barrier's count while a copy is under way would break it)
-            if (lane == 0 && !wait.stopped()) {
-                bar_arrive(bar(bFull + st));
-                bar_arrive(bar(bWEmpty + ws));
-                if (GRAD) bar_arrive(bar(bSEmpty + sr.at));
+        }
+    } else if (warp == kWProducts) {
+        // ---- products of both CTAs' rows, by the first one
+        if (rank == 0) {
+            const uint32_t idesc = (1u << 4) | ((a.T >> 3) << 17) | ((2u * kRows >> 4) << 24);
+            const uint64_t desc0 = sw128_desc(base + a.at_x);
+            Ring ar, dr;
+            for (uint64_t at = run0; at < run1; dr.next(a.nd)) {
+                const Part s = part_at(at);
+                at += s.p1 - s.p0;
+                const uint32_t d = tmem + dr.at * a.T;
+                wait(bar(bOutEmpty + dr.at), dr.lap ^ 1u);
+                fence_after();
+                for (uint32_t i = 0; i < s.blocks; i++) {
+                    wait(bar(bFull + ar.at), ar.lap);
+                    fence_after();
+                    const uint32_t from = tmem + a_base + ar.at * 32u;
+                    const uint64_t desc = desc0 + ((ar.at * xstage) >> 4);
+                    // (past the last column of a forward product the codes are the copy's zeros, times a scale, and the activations zeros)
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; j++) mma_pair(d, from + j * 8u, desc + j * 2u, idesc, i + j != 0);
+                    commit_pair(bar(bEmpty + ar.at));
+                    ar.next(a.ns);
+                }
+                commit_pair(bar(bOutFull + dr.at));
             }
-#pragma unroll
-            for (int j = 0; j < kSets; j++) ar.next(a.ns);
         }
-    } else if (warp == 4 * kSets) {
-        // ---- products
-        const uint32_t idesc = (1u << 4) | ((a.T >> 3) << 17) | ((kRows >> 4) << 24);
-        const uint64_t desc0 = sw128_desc(base + a.at_x);
-        uint32_t acc = 0;
-        Ring ar;
-        for (uint32_t i = 0; i < nkb; i++) {
-            wait(bar(bFull + ar.at), ar.lap);
-            fence_after();
-            const uint32_t at = tmem + a_base + ar.at * 32u;
-            const uint64_t desc = desc0 + ((ar.at * xstage) >> 4);
-            // (past the last column of a forward product the codes are zeros of the copy, times a scale, and the activations zeros)
-#pragma unroll
-            for (uint32_t j = 0; j < 4; j++) { mma_ts(tmem, at + j * 8u, desc + j * 2u, idesc, acc); acc = 1; }
-            mma_commit(bar(bEmpty + ar.at));
-            ar.next(a.ns);
-        }
-        mma_commit(bar(bDone));
-    } else if (warp == 4 * kSets + 1) {
+    } else if (warp == kWCodes) {
         // ---- weight copies: a resident weight depends on nothing that came before in the stream
         const bool leader = elect();
         Ring wr;
         uint32_t used = 0;
-        for (uint32_t u = u0; u < u1; u++) {
-            const bool go = wait.go(bar(bWEmpty + wr.at), wr.lap ^ 1u);
-            if (leader && go) {
-                used++;
-                const uint32_t to = base + wr.at * P::kStage, full = bar(bWFull + wr.at);
-                bar_expect(full, P::kStage);
-                if constexpr (GRAD) {
-                    const uint32_t which = u >= a.per_weight;
-                    tma_2d(to, which ? &umap : &gmap, tile * P::kBytes, (u - (which ? a.per_weight : 0u)) * P::kAlong, full);
-                } else {
-                    tma_2d(to, &gmap, u * P::kBytes, row0, full);
-                    tma_2d(to + P::kStage / 2u, &umap, u * P::kBytes, row0, full);
+        for (uint64_t at = run0; at < run1;) {
+            const Part s = part_at(at);
+            at += s.p1 - s.p0;
+            for (uint32_t p = s.p0; p < s.p1; p++, wr.next(a.nw)) {
+                wait(bar(bWEmpty + wr.at), wr.lap ^ 1u);
+                if (leader && !wait.lost) {
+                    used++;
+                    const uint32_t to = base + wr.at * P::kStage, full = bar(bWFull + wr.at);
+                    bar_expect(full, P::kStage);
+                    if constexpr (GRAD) {
+                        const uint32_t which = p >= a.per_weight, x = first_row(s.tile) / kWide * P::kBytes, y = (p - (which ? a.per_weight : 0u)) * P::kAlong;
+                        if (which) tma_2d(to, &umap, x, y, full);
+                        else tma_2d(to, &gmap, x, y, full);
+                    } else {
+                        tma_2d(to, &gmap, p * P::kBytes, first_row(s.tile), full);
+                        tma_2d(to + P::kStage / 2u, &umap, p * P::kBytes, first_row(s.tile), full);
+                    }
                 }
+                __syncwarp();
             }
-            __syncwarp();
-            wr.next(a.nw);
         }
         if (leader) *word(bUsedW) = used;
-    } else if (warp == 4 * kSets + 2) {
-        // ---- activation copies
+    } else if (warp == kWTokens) {
+        // ---- activation copies: this CTA's half of a block's tokens; the first CTA's barrier counts both halves' bytes
         const bool leader = elect();
         asm volatile("griddepcontrol.wait;" ::: "memory");
         if (leader) word(bMark)[1] = 1u;
+        const uint32_t full0 = in_cta(bar(bFull), 0u);
         Ring xr;
-        uint32_t used = 0;
-        for (uint32_t i = 0; i < nkb; i++) {
-            const bool go = wait.go(bar(bEmpty + xr.at), xr.lap ^ 1u);
-            if (leader && go) {
-                used++;
-                bar_expect(bar(bFull + xr.at), xstage);
-                uint32_t along = (kb0 + i) * 64u, rows = tok0;
-                if (GRAD && along >= a.per_weight * P::kAlong) { along -= a.per_weight * P::kAlong; rows += a.M; }
-                tma_2d(base + a.at_x + xr.at * xstage, &xmap, along, rows, bar(bFull + xr.at));
+        for (uint64_t at = run0; at < run1;) {
+            const Part s = part_at(at);
+            at += s.p1 - s.p0;
+            const uint32_t token = first_token(s.tile) + rank * (a.T / 2u);
+            for (uint32_t i = 0; i < s.blocks; i++, xr.next(a.ns)) {
+                wait(bar(bEmpty + xr.at), xr.lap ^ 1u);
+                if (leader && !wait.lost) {
+                    if (rank == 0) bar_expect(bar(bFull + xr.at), 2u * xstage);
+                    uint32_t along = (s.p0 * P::kBlocks + i) * 64u, y = token;
+                    if (GRAD && along >= a.per_weight * P::kAlong) { along -= a.per_weight * P::kAlong; y += a.M; }
+                    tma_2d_pair(base + a.at_x + xr.at * xstage, &xmap, along, y, full0 + 8u * xr.at);
+                }
+                __syncwarp();
             }
-            __syncwarp();
-            xr.next(a.ns);
         }
-        if (leader) *word(bUsedX) = used;
-    } else if constexpr (!GRAD) {
-        // ---- scales: eight groups of 128 rows at a time, transposed on the way ([group][row])
-        Ring sr;
-        for (uint32_t g0 = 0; g0 < ngroups; g0 += 8u) {
-            uint16_t v[4][8];
-#pragma unroll
-            for (uint32_t j = 0; j < 4; j++) {
-                const uint16_t *srow = a.scales[j >> 1] + (size_t)min(row0 + lane + 32u * (j & 1u), a.N - 1u) * a.groups;
-#pragma unroll
-                for (uint32_t g = 0; g < 8; g++) v[j][g] = __ldg(srow + min(grp0 + g0 + g, a.groups - 1u));
+    } else if (warp == kWScales) {
+        // ---- scales of a piece, [group][row], fetched some pieces ahead (one at a time, their latency is what bounds the launch).  Gradient: zero
+        // past the last weight row, so that what lies behind it (there the activations are zeros) cannot be an infinity.
+        constexpr uint32_t kGroups = GRAD ? 4u : 8u;
+        constexpr int kAhead = GRAD ? 4 : 2;
+        struct Fetched { uint16_t v[4][kGroups]; uint32_t ng; };
+        struct { uint64_t at; uint32_t p, p1, row0; } c = {run0, 0u, 0u, 0u};       // what is to be fetched next
+        auto fetch = [&](Fetched &f) {
+            f.ng = 0u;
+            if (c.p == c.p1) {
+                if (c.at >= run1) return;
+                const Part s = part_at(c.at);
+                c.at += s.p1 - s.p0;
+                c.p = s.p0; c.p1 = s.p1;
+                c.row0 = first_row(s.tile);
             }
-            wait(bar(bSEmpty + sr.at), sr.lap ^ 1u);
+            const uint32_t p = c.p++;
+            if constexpr (GRAD) {
+                const uint32_t which = p >= a.per_weight, n0 = (p - (which ? a.per_weight : 0u)) * P::kAlong, g_first = group_of(min(c.row0, a.K - 1u));
+                const uint16_t *from = (which ? a.scales[1] : a.scales[0]) + g_first;
+                const uint32_t ng = group_of(min(c.row0 + 127u, a.K - 1u)) - g_first + 1u;
 #pragma unroll
-            for (uint32_t j = 0; j < 4; j++)
+                for (uint32_t j = 0; j < 4; j++) {
+                    const uint32_t n = n0 + j * 32u + lane;
 #pragma unroll
-                for (uint32_t g = 0; g < 8; g++)
-                    asm volatile("st.shared.u16 [%0], %1;" ::"r"(scale_ring + sr.at * kScaleEntry + g * (kRows * 2u) + j * 64u + lane * 2u), "h"(v[j][g]) : "memory");
-            __syncwarp();
-            if (lane == 0) bar_arrive(bar(bSFull + sr.at));
-            sr.next(kScaleRing);
+                    for (uint32_t g = 0; g < kGroups; g++) f.v[j][g] = g < ng && n < a.N ? __ldg(from + (size_t)n * a.groups + g) : (uint16_t)0;
+                }
+                f.ng = kGroups;
+            } else {
+                const uint32_t g0 = group_of(p * P::kAlong);
+                f.ng = group_of(min((p + 1u) * P::kAlong, a.K) - 1u) - g0 + 1u;
+#pragma unroll
+                for (uint32_t j = 0; j < 4; j++) {
+                    const uint16_t *from = a.scales[j >> 1] + (size_t)min(c.row0 + lane + 32u * (j & 1u), a.N - 1u) * a.groups + g0;
+#pragma unroll
+                    for (uint32_t g = 0; g < kGroups; g++) if (g < f.ng) f.v[j][g] = __ldg(from + g);
+                }
+            }
+        };
+        Fetched f[kAhead];
+#pragma unroll
+        for (int d = 0; d < kAhead; d++) fetch(f[d]);
+        Ring wr;
+        for (bool more = true; more;) {
+#pragma unroll
+            for (int d = 0; d < kAhead; d++) {
+                if (!f[d].ng) { more = false; break; }
+                wait(bar(bWEmpty + wr.at), wr.lap ^ 1u);
+#pragma unroll
+                for (uint32_t j = 0; j < 4; j++)
+#pragma unroll
+                    for (uint32_t g = 0; g < kGroups; g++)
+                        if (g < f[d].ng) asm volatile("st.shared.u16 [%0], %1;" ::"r"(scales_at + wr.at * kScales + g * (kRows * 2u) + j * 64u + lane * 2u), "h"(f[d].v[j][g]) : "memory");
+                __syncwarp();
+                if (lane == 0 && !wait.lost) bar_arrive(bar(bWFull + wr.at));
+                wr.next(a.nw);
+                fetch(f[d]);
+            }
         }
     } else {
-        // ---- scales of a piece's 128 weight rows at the tile's columns, up to four groups ([group][row]); zero past the last row, so
-        // that what lies behind it (there the activations are zeros) cannot be an infinity
-        const uint32_t g_first = row0 / a.group, ng = (min(row0 + 127u, a.K - 1u)) / a.group - g_first + 1u;
-        Ring sr;
-        for (uint32_t u = u0; u < u1; u++) {
-            const uint32_t which = u >= a.per_weight, n0 = (u - (which ? a.per_weight : 0u)) * P::kAlong;
-            uint16_t v[4][4];
+        // ---- the way out.  A lane keeps its row: of 32 tokens at a time, a warp of the gate's rows hands the later sixteen to the warp that has the same
+        // features' up rows, and gets the earlier sixteen's, so that both make h of sixteen tokens, all in flight together.
+        const uint32_t q = warp & 3u, tid = threadIdx.x - kWOut * 32u, row = place<GRAD, BITS>(q, lane), empty0 = in_cta(bar(bOutEmpty), 0u);
+        const bool gate = q < 2u;                                // (forward)
+        const uint32_t exchange = base + a.at_out, maxima = exchange + 8u * 2048u;
+        asm volatile("griddepcontrol.wait;" ::: "memory");       // outputs, scratch and counters are the kernels' before this one until here
+        // sixteen tokens' values of this lane's column, `stride` apart, the first `count` of them
+        auto put = [&](void *to, size_t at, uint32_t stride, uint32_t count, const float (&v)[16]) {
+            uint16_t *p = reinterpret_cast<uint16_t *>(to) + at, o[16];
+            if (a.dtype == EOQ_B200_F16) {
 #pragma unroll
-            for (uint32_t j = 0; j < 4; j++) {
-                const uint32_t n = n0 + j * 32u + lane;
+                for (uint32_t j = 0; j < 16; j++) o[j] = __half_as_ushort(__float2half_rn(v[j]));
+            } else {
 #pragma unroll
-                for (uint32_t g = 0; g < 4; g++) v[j][g] = g < ng && n < a.N ? __ldg(a.scales[which] + (size_t)n * a.groups + g_first + g) : (uint16_t)0;
+                for (uint32_t j = 0; j < 16; j++) o[j] = __bfloat16_as_ushort(__float2bfloat16_rn(v[j]));
             }
-            wait(bar(bSEmpty + sr.at), sr.lap ^ 1u);
+            if (count >= 16u) {
 #pragma unroll
-            for (uint32_t j = 0; j < 4; j++)
+                for (uint32_t j = 0; j < 16; j++, p += stride) *p = o[j];
+            } else {
 #pragma unroll
-                for (uint32_t g = 0; g < 4; g++)
-                    asm volatile("st.shared.u16 [%0], %1;" ::"r"(scale_ring + sr.at * kScaleEntry + g * (kRows * 2u) + j * 64u + lane * 2u), "h"(v[j][g]) : "memory");
+                for (uint32_t j = 0; j < 16; j++, p += stride) if (j < count) *p = o[j];
+            }
+        };
+        uint32_t turn = 0;                                       // buffers of the exchange alternate
+        // a tile, its rows' sums of sixteen tokens from `take`; `behind` is called when the last have been taken
+        auto finish = [&](uint32_t tile, auto &&take, auto &&behind) {
+            const uint32_t row0 = first_row(tile), tok0 = first_token(tile), tokens = min(a.T, a.M - tok0);
+            if constexpr (GRAD) {
+                const uint32_t k = row0 + row;
+                for (uint32_t t0 = 0; t0 < a.T; t0 += 16u) {
+                    float v[16];
+                    take(t0, v);
+                    if (t0 + 16u >= a.T) behind();
+                    if (t0 >= tokens || k >= a.K) continue;
+                    if (a.factor) {
+#pragma unroll
+                        for (uint32_t j = 0; j < 16; j++) v[j] *= __ldg(a.factor + min(tok0 + t0 + j, a.M - 1u));
+                    }
+                    put(a.y, (size_t)(tok0 + t0) * a.K + k, a.K, tokens - t0, v);
+                }
+            } else {
+                const uint32_t n = row0 + (q & 1u) * 32u + lane;
+                const bool there = n < a.N;
+                const float bg = there && a.bias[0] ? __ldg(a.bias[0] + n) : 0.0f, bu = there && a.bias[1] ? __ldg(a.bias[1] + n) : 0.0f;
+                for (uint32_t t0 = 0; t0 < a.T; t0 += 32u, turn ^= 1u) {
+                    float g[16], u[16];
+                    const bool two = t0 + 16u < a.T;             // else the later sixteen do not exist
+                    const uint32_t mine = exchange + (turn * 4u + q) * 2048u + lane * 4u, other = exchange + (turn * 4u + (q ^ 2u)) * 2048u + lane * 4u;
+                    take(gate ? t0 + 16u : t0, g);               // what is handed over, first
+                    if (!gate || two) {
+#pragma unroll
+                        for (uint32_t j = 0; j < 16; j++) asm volatile("st.shared.f32 [%0], %1;" ::"r"(mine + j * 128u), "f"(g[j]) : "memory");
+                    }
+                    take(gate ? t0 : t0 + 16u, g);
+                    if (t0 + 32u >= a.T) behind();
+                    asm volatile("bar.sync %0, 64;" ::"r"(1u + (q & 1u)) : "memory");
+#pragma unroll
+                    for (uint32_t j = 0; j < 16; j++) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(u[j]) : "r"(other + j * 128u));
+                    const uint32_t t = gate ? t0 : t0 + 16u;
+                    const bool work = gate || two;
+                    if (!gate) {
+#pragma unroll
+                        for (uint32_t j = 0; j < 16; j++) { const float v = g[j]; g[j] = u[j]; u[j] = v; }
+                    }
+                    if (a.factor) {
+#pragma unroll
+                        for (uint32_t j = 0; j < 16; j++) {
+                            const float f = __ldg(a.factor + min(tok0 + t + j, a.M - 1u));
+                            g[j] *= f;
+                            u[j] *= f;
+                        }
+                    }
+#pragma unroll
+                    for (uint32_t j = 0; j < 16; j++) { g[j] += bg; u[j] += bu; }
+                    if (work && there && t < tokens) {
+                        const size_t at = (size_t)(tok0 + t) * a.N + n;
+                        float h[16];
+                        if (a.act == kActSilu) {
+#pragma unroll
+                            for (uint32_t j = 0; j < 16; j++) h[j] = activation(g[j], kActSilu) * u[j];
+                        } else {
+#pragma unroll
+                            for (uint32_t j = 0; j < 16; j++) h[j] = activation(g[j], a.act) * u[j];
+                        }
+                        put(a.y, at, a.N, tokens - t, h);
+                        if (a.keep.form == kKeepFull) {
+                            put(a.keep.v[0], at, a.N, tokens - t, g);
+                            put(a.keep.v[1], at, a.N, tokens - t, u);
+                        }
+                    }
+                    if (a.keep.form == kKeep8bit) {
+                        // the tile's 64 features of a token are one block of the 8-bit form: this warp's 32, and its neighbour's
+                        const uint32_t to = maxima + (turn * 4u + q) * 128u, from = maxima + (turn * 4u + (q ^ 1u)) * 128u;
+                        uint32_t most[2][16];
+#pragma unroll
+                        for (uint32_t j = 0; j < 16; j++) {
+                            most[0][j] = __reduce_max_sync(0xffffffffu, there ? __float_as_uint(g[j]) & 0x7fffffffu : 0u);
+                            most[1][j] = __reduce_max_sync(0xffffffffu, there ? __float_as_uint(u[j]) & 0x7fffffffu : 0u);
+                            if (lane == 0) asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to + j * 8u), "r"(most[0][j]), "r"(most[1][j]) : "memory");
+                        }
+                        asm volatile("bar.sync %0, 64;" ::"r"(3u + (q >> 1)) : "memory");
+#pragma unroll
+                        for (uint32_t j = 0; j < 16; j++) {
+                            uint32_t eg, eu;
+                            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(eg), "=r"(eu) : "r"(from + j * 8u));
+                            if (!work || t + j >= tokens) continue;
+                            const Storer sg(max(most[0][j], eg)), su(max(most[1][j], eu));
+                            const size_t m = tok0 + t + j, at = m * a.N + n, block = m * ((a.N + kStoreBlock - 1) / kStoreBlock) + row0 / 64u;
+                            if (there) {
+                                reinterpret_cast<int8_t *>(a.keep.v[0])[at] = sg.code(g[j]);
+                                reinterpret_cast<int8_t *>(a.keep.v[1])[at] = su.code(u[j]);
+                            }
+                            if ((q & 1u) == 0 && lane == 0 && there) { a.keep.scale[0][block] = sg.scale; a.keep.scale[1][block] = su.scale; }
+                        }
+                    }
+                }
+            }
+        };
+        auto partial_of = [&](uint32_t p, uint32_t begins) { return a.partial + ((size_t)(p * 2u + begins) * 2u + rank) * a.T * kRows + q * 32u + lane; };
+        Ring dr;
+        for (uint64_t at = run0; at < run1; dr.next(a.nd)) {
+            const Part s = part_at(at);
+            at += s.p1 - s.p0;
+            wait(bar(bOutFull + dr.at), dr.lap);
             __syncwarp();
-            if (lane == 0) bar_arrive(bar(bSFull + sr.at));
-            sr.next(kScaleRing);
+            fence_after();
+            const uint32_t from = tmem + ((q * 32u) << 16) + dr.at * a.T;
+            auto take = [&](uint32_t t, float (&v)[16]) {
+                uint32_t r[16] = {};
+                if (t < a.T) { tmem_ld16(from + t, r); tmem_ld_wait(r); }
+#pragma unroll
+                for (int j = 0; j < 16; j++) v[j] = wait.lost ? __uint_as_float(0x7fffffffu) : __uint_as_float(r[j]);
+            };
+            auto release = [&]() {                               // the next tile may have the accumulator
+                fence_before();
+                __syncwarp();
+                if (lane == 0 && !wait.lost) arrive_cluster(empty0 + 8u * dr.at);
+            };
+            if (s.p1 - s.p0 == a.per_tile) {
+                finish(s.tile, take, release);
+                continue;
+            }
+            // the tile's other parts are other pairs': the last to arrive adds them up
+            float *mine = partial_of(pair, s.p0 == 0u);
+            for (uint32_t t0 = 0; t0 < a.T; t0 += 16u) {
+                float v[16];
+                take(t0, v);
+                if (t0 + 16u >= a.T) release();
+#pragma unroll
+                for (uint32_t j = 0; j < 16; j++) __stcg(mine + (size_t)(t0 + j) * kRows, v[j]);
+            }
+            const uint64_t first = (uint64_t)s.tile * a.per_tile, total = (uint64_t)a.tiles * a.per_tile;
+            const uint32_t p_first = (uint32_t)(((first + 1) * pairs - 1) / total), p_last = (uint32_t)(((first + a.per_tile) * pairs - 1) / total);
+            __threadfence();
+            asm volatile("bar.sync 5, 128;" ::: "memory");
+            if (tid == 0) *word(bTicket) = atomicAdd(a.count + s.tile * 2u + rank, 1u);
+            asm volatile("bar.sync 5, 128;" ::: "memory");
+            if (*word(bTicket) != p_last - p_first) continue;
+            __threadfence();
+            finish(s.tile, [&](uint32_t t, float (&v)[16]) {
+#pragma unroll
+                for (int j = 0; j < 16; j++) v[j] = 0.0f;
+                if (t >= a.T) return;
+                for (uint32_t p = p_first; p <= p_last; p++) {       // a part's all requested before the first is added
+                    const float *part = partial_of(p, run_start(p) <= first) + (size_t)t * kRows;
+                    float o[16];
+#pragma unroll
+                    for (int j = 0; j < 16; j++) o[j] = __ldcg(part + j * kRows);
+#pragma unroll
+                    for (int j = 0; j < 16; j++) v[j] += o[j];
+                }
+            }, []() {});
         }
     }
     __syncwarp();
-    if (warp < 4 * kSets) {
-        // sums to shared memory, [token][row]: sixteen tokens at a time.  (All products are behind: the stages are free.)
-        wait(bar(bDone), 0u);
-        __syncwarp();
-        fence_after();
-        const uint32_t q = warp & 3u, to = place<GRAD, BITS>(q, lane);
-        for (uint32_t c = (warp >> 2) * 16u; c < a.T; c += kSets * 16u) {
-            uint32_t v[16];
-            tmem_ld16(tmem + ((q * 32u) << 16) + c, v);
-            tmem_ld_wait(v);
-#pragma unroll
-            for (int j = 0; j < 16; j++) reinterpret_cast<float *>(smem)[(size_t)(c + j) * kRows + to] = __uint_as_float(v[j]);
-        }
-        fence_before();
-    }
-    asm volatile("griddepcontrol.wait;" ::: "memory");
     __syncthreads();
-    if (wait.stopped()) {                          // the same for all threads: whoever sets the mark does so before the barrier above
-        // nothing may be under way any more when tensor and shared memory are given back
-        if (warp == 4 * kSets) { mma_commit(bar(bDrain)); drain(bar(bDrain), 1u, 1u); }
-        if (warp == 4 * kSets + 1) drain(bar(bWFull), *word(bUsedW), a.nw);
-        if (warp == 4 * kSets + 2) drain(bar(bFull), *word(bUsedX), a.ns);
-        __syncthreads();
-        for (uint32_t e = threadIdx.x; e < a.T * kRows; e += kThreads) reinterpret_cast<uint32_t *>(smem)[e] = 0x7fffffffu;
-        __syncthreads();
-    }
-    if (warp == 4 * kSets) {
-        fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kTmem) : "memory");
-    }
     cg::cluster_group cluster = cg::this_cluster();
-    if (a.split > 1) cluster.sync();
-    const float *mine = reinterpret_cast<const float *>(smem);
-    // four values of a token, all the cluster's CTAs' added up; requested before the first is added
-    auto sum4 = [&](uint32_t at) {
-        if (a.split == 1) return *reinterpret_cast<const float4 *>(mine + at);
-        float4 o[8], v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-        for (uint32_t k = 0; k < 8; k++) o[k] = k < a.split ? *reinterpret_cast<const float4 *>(cluster.map_shared_rank(mine, k) + at) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-        for (uint32_t k = 0; k < 8; k++) { v.x += o[k].x; v.y += o[k].y; v.z += o[k].z; v.w += o[k].w; }
-        return v;
-    };
-    auto store4 = [&](void *to, size_t at, uint32_t left, bool vec, const float (&o)[4]) {
-        if (a.dtype == EOQ_B200_F32) {
-            float *y = reinterpret_cast<float *>(to) + at;
-            if (vec) *reinterpret_cast<float4 *>(y) = make_float4(o[0], o[1], o[2], o[3]);
-            else for (uint32_t j = 0; j < 4; j++) if (j < left) y[j] = o[j];
-            return;
-        }
-        uint32_t p[2];
-#pragma unroll
-        for (int j = 0; j < 2; j++) {
-            if (a.dtype == EOQ_B200_F16) { const __half2 h = __floats2half2_rn(o[2 * j], o[2 * j + 1]); p[j] = *reinterpret_cast<const uint32_t *>(&h); }
-            else p[j] = pack_bf16(o[2 * j], o[2 * j + 1]);
-        }
-        uint16_t *y = reinterpret_cast<uint16_t *>(to) + at;
-        if (vec) *reinterpret_cast<uint2 *>(y) = make_uint2(p[0], p[1]);
-        else for (uint32_t j = 0; j < 4; j++) if (j < left) y[j] = (uint16_t)(p[j >> 1] >> (16 * (j & 1)));
-    };
-    constexpr uint32_t kQuads = GRAD ? 32u : 16u;              // of a token's results in this tile
-    const uint32_t width = GRAD ? a.K : a.N;
-    const bool vec = (width & 3u) == 0;
-    // (whole warps go on together: the 8-bit form's lanes exchange values)
-    for (uint32_t e = rank * kThreads + threadIdx.x; (e & ~31u) < a.T * kQuads; e += kThreads * a.split) {
-        const uint32_t t = e / kQuads, c = (e % kQuads) * 4u, m = tok0 + t, n = row0 + c;
-        const bool here = t < a.T && m < a.M && n < width;
-        if constexpr (GRAD) {
-            if (!here) continue;
-            const float4 v = sum4(t * kRows + c);
-            const float f = a.factor ? __ldg(a.factor + m) : 1.0f;
-            const float o[4] = {v.x * f, v.y * f, v.z * f, v.w * f};
-            store4(a.y, (size_t)m * width + n, width - n, vec, o);
-        } else {
-            float g[4] = {}, u[4] = {}, h[4];
-            if (here) {
-                const float4 vg = sum4(t * kRows + c), vu = sum4(t * kRows + 64u + c);
-                const float f = a.factor ? __ldg(a.factor + m) : 1.0f;
-                g[0] = vg.x * f; g[1] = vg.y * f; g[2] = vg.z * f; g[3] = vg.w * f;
-                u[0] = vu.x * f; u[1] = vu.y * f; u[2] = vu.z * f; u[3] = vu.w * f;
-#pragma unroll
-                for (uint32_t j = 0; j < 4; j++) {
-                    if (n + j >= a.N) { g[j] = u[j] = 0.0f; continue; }       // (would count in an 8-bit block's largest)
-                    if (a.bias[0]) g[j] += __ldg(a.bias[0] + n + j);
-                    if (a.bias[1]) u[j] += __ldg(a.bias[1] + n + j);
-                }
-                const size_t at = (size_t)m * a.N + n;
-#pragma unroll
-                for (int j = 0; j < 4; j++) h[j] = activation(g[j], a.act) * u[j];
-                store4(a.y, at, a.N - n, vec, h);
-                if (a.keep.form == kKeepFull) {
-                    store4(a.keep.v[0], at, a.N - n, vec, g);
-                    store4(a.keep.v[1], at, a.N - n, vec, u);
-                }
-            }
-            if (a.keep.form == kKeep8bit) {
-                // the tile's 64 features of a token are one block of the 8-bit form, four a lane
-                uint32_t mg = 0u, mu = 0u;
-#pragma unroll
-                for (int j = 0; j < 4; j++) { mg = max(mg, __float_as_uint(g[j]) & 0x7fffffffu); mu = max(mu, __float_as_uint(u[j]) & 0x7fffffffu); }
-#pragma unroll
-                for (int d = 8; d > 0; d >>= 1) { mg = max(mg, __shfl_xor_sync(0xffffffffu, mg, d)); mu = max(mu, __shfl_xor_sync(0xffffffffu, mu, d)); }
-                const Storer sg(mg), su(mu);
-                if (here) {
-                    const size_t at = (size_t)m * a.N + n, block = (size_t)m * ((a.N + kStoreBlock - 1) / kStoreBlock) + tile;
-                    if (c == 0) { a.keep.scale[0][block] = sg.scale; a.keep.scale[1][block] = su.scale; }
-                    uint32_t pg = 0u, pu = 0u;
-#pragma unroll
-                    for (int j = 0; j < 4; j++) { pg |= (uint32_t)(uint8_t)sg.code(g[j]) << (8 * j); pu |= (uint32_t)(uint8_t)su.code(u[j]) << (8 * j); }
-                    uint8_t *kg = reinterpret_cast<uint8_t *>(a.keep.v[0]) + at, *ku = reinterpret_cast<uint8_t *>(a.keep.v[1]) + at;
-                    if (vec) { *reinterpret_cast<uint32_t *>(kg) = pg; *reinterpret_cast<uint32_t *>(ku) = pu; }
-                    else for (uint32_t j = 0; j < 4; j++) if (n + j < a.N) { kg[j] = (uint8_t)(pg >> (8 * j)); ku[j] = (uint8_t)(pu >> (8 * j)); }
-                }
-            }
-        }
+    if (wait.stopped()) {
+        // nothing may be under way any more when tensor and shared memory are given back.  (Activations: their barrier also counts
+        // arrivals that may not come, so what is left of them gets the time of a lost copy.)
+        if (warp == kWProducts && rank == 0) { commit_pair(bar(bDrain)); drain(bar(bDrain), 1u, 1u); }
+        if (warp == kWCodes) drain(bar(bWFull), *word(bUsedW), a.nw);
+        if (warp == kWTokens) { const long long t0 = clock64(); while (clock64() - t0 < 20000000ll) {} }
     }
-    if (a.split > 1) cluster.sync();               // nobody leaves while its sums are being read
+    __syncthreads();
+    cluster.sync();                            // the other CTA's arrivals and products are behind
+    if (warp == kWProducts) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kTmem) : "memory");
+    }
 }
 
 std::atomic<long long> g_limit{4000000000ll};      // about two seconds
 
-struct Layout { uint32_t nw, ns, at_x, at_bar; size_t smem; };
+struct Layout { uint32_t nw, ns, nd, at_x, at_out, at_bar; size_t smem; };
 
-// A producer set has to come by every operand stage on every lap (its parity waits look one lap back): stages in multiples of the
-// sets, weight stages in multiples of the copies that a set steps over.
-Layout lay_out(uint32_t T, uint32_t stage_w, uint32_t blocks)
+// Operand stages in multiples of the producer sets, which take them in turn.
+Layout lay_out(uint32_t T, uint32_t stage_w)
 {
-    const uint32_t fixed = 512 + 1024 + kScaleRing * kScaleEntry, room = 226u * 1024u - fixed, xstage = T * 128u, step = std::max(1u, kSets / blocks);
+    const uint32_t fixed = 1024 + 8 * bEnd + 8, room = 226u * 1024u - fixed - kOut, xstage = T * 64u;
     Layout l = {};
-    l.ns = T <= 128u ? 8u : 4u;
-    if (room < l.ns * xstage + 4u * stage_w) l.ns = 4u;
-    l.nw = std::min(8u, (room - l.ns * xstage) / stage_w) / step * step;
+    l.nd = 2u * T + 4u * 32u <= kTmem ? 2u : 1u;
+    l.ns = l.nd * T + 8u * 32u <= kTmem ? 8u : 4u;
+    l.nw = std::min(8u, (room - l.ns * xstage) / (stage_w + kScales));
     l.at_x = l.nw * stage_w;
-    l.at_bar = std::max(l.at_x + l.ns * xstage, T * kRows * 4u);
-    l.smem = l.at_bar + fixed;
+    l.at_out = l.at_x + l.ns * xstage;
+    l.at_bar = l.at_out + kOut;
+    l.smem = l.at_bar + 8 * bEnd + 8 + (size_t)l.nw * kScales + 1024;
     return l;
 }
 
-struct Cut { uint32_t T, tok_tiles, split; };
-
-// Token tile and split with the least rounds of resident CTAs x what a CTA takes: blocks of 64, each the longer of its products
-// (two cycles a token) and its producers' work, and some four thousand cycles to start, fill and store (half as many more to meet in a
-// cluster).
-template <class Room>
-Cut cut(uint32_t tiles, uint32_t M, uint32_t units, uint32_t blocks, Room &&room)
+// Tokens of a tile: as few tiles as pay.  A block of 64 costs its products (two clocks a token) or its producers' work (some 330), whichever is
+// longer; with one accumulator a tile's way out (some 24 clocks a token) comes on top.
+uint32_t tile_tokens(uint32_t M, uint32_t blocks)
 {
-    Cut best = {};
+    uint32_t best = 0;
     double least = 1e30;
-    const uint32_t fewest = (M + 255u) / 256u;
-    for (uint32_t n = fewest; n < fewest + 4; n++) {
+    for (uint32_t n = (M + 255u) / 256u; n < (M + 255u) / 256u + 4u; n++) {
         const uint32_t T = ((M + n - 1) / n + 15u) / 16u * 16u;
-        if (n > fewest && (T >= best.T || (M + T - 1) / T < n)) continue;
-        const double block = std::max(400.0, 2.0 * T + 150.0);
-        for (uint32_t split = 1; split <= 8 && split <= units; split++) {
-            const uint32_t at_once = room(T, split);
-            if (!at_once) continue;
-            const double cost = (double)(((uint64_t)tiles * n * split + at_once - 1) / at_once) *
-                                ((double)((units + split - 1) / split) * blocks * block + 4000.0 * (split > 1 ? 1.5 : 1.0));
-            if (cost < least * (n > best.tok_tiles && best.T ? 0.95 : 0.999)) { least = cost; best = Cut{T, n, split}; }
-        }
+        const double cost = (double)((M + T - 1) / T) * (blocks * std::max(500.0, 2.0 * T) + (T > 192u ? 100.0 * T : 0.0));
+        if (cost < 0.999 * least) { least = cost; best = T; }
     }
     return best;
 }
 
+struct Plan { uint32_t T, tok_tiles, tiles, per_tile, per_weight, pairs; };
+
 template <bool GRAD, int BITS>
-int run(ProductArgs a, const PackedPair &w, int nw, const void *x, uint32_t pitch, cudaStream_t st)
+Plan plan_for(uint32_t N, uint32_t K, uint32_t M, int nw)
+{
+    using P = Piece<GRAD, BITS>;
+    Plan p = {};
+    p.per_weight = GRAD ? (N + P::kAlong - 1) / P::kAlong : 0u;
+    p.per_tile = GRAD ? p.per_weight * nw : (K + P::kAlong - 1) / P::kAlong;
+    p.T = tile_tokens(M, p.per_tile * P::kBlocks);
+    p.tok_tiles = (M + p.T - 1) / p.T;
+    p.tiles = ((GRAD ? K + 255u : N + 127u) / (GRAD ? 256u : 128u)) * p.tok_tiles;
+    // All the pairs there are, where tiles are that many; else as many to a tile as pay: a part more costs its sums' way through scratch.
+    const uint32_t room = (uint32_t)std::max(1, device_sm_count() / 2);
+    p.pairs = std::min(room, p.tiles);
+    if (p.tiles < room) {
+        double least = 1e30;
+        const double block = std::max(330.0, 2.0 * p.T);
+        for (uint32_t n = p.tiles; n <= room && n <= (uint64_t)p.tiles * p.per_tile; n++) {
+            const double parts = (double)n / p.tiles, pieces = std::ceil((double)p.tiles * p.per_tile / n);
+            const double cost = pieces * P::kBlocks * block + (n > p.tiles ? 4000.0 + std::ceil(p.T / 32.0) * 800.0 * (1.0 + std::ceil(parts)) : 0.0);
+            if (cost < 0.98 * least) { least = cost; p.pairs = n; }
+        }
+    }
+    return p;
+}
+
+template <bool GRAD>
+Plan plan_of(uint32_t N, uint32_t K, uint32_t bits, uint32_t M, int nw)
+{
+    return bits == 4 ? plan_for<GRAD, 4>(N, K, M, nw) : bits == 2 ? plan_for<GRAD, 2>(N, K, M, nw) : plan_for<GRAD, 8>(N, K, M, nw);
+}
+
+size_t count_bytes(const Plan &p) { return ((size_t)p.tiles * 8 + 255) & ~(size_t)255; }
+size_t scratch_bytes(const Plan &p) { return count_bytes(p) + (size_t)p.pairs * 4 * p.T * kRows * 4; }
+
+template <bool GRAD, int BITS>
+int run(ProductArgs a, const PackedPair &w, int nw, const void *x, uint32_t pitch, void *scratch, cudaStream_t st)
 {
     using P = Piece<GRAD, BITS>;
     auto kern = gated_product_kernel<GRAD, BITS>;
-    const uint32_t tiles = GRAD ? (a.K + 127u) / 128u : (a.N + 63u) / 64u;
-    a.per_weight = GRAD ? (a.N + P::kAlong - 1) / P::kAlong : 0u;
-    a.units = GRAD ? a.per_weight * nw : (a.K + P::kAlong - 1) / P::kAlong;
-    // the cuts of the last shapes (a model has a handful)
-    struct Known { uint32_t tiles, M, units; int dev; Cut c; };
-    static std::mutex mu;
-    static Known known[32];
-    static uint32_t used = 0;
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return (int)cudaErrorInvalidDevice;
-    Cut c = {};
-    {
-        std::lock_guard<std::mutex> lock(mu);
-        for (uint32_t i = 0; i < std::min(used, 32u); i++)
-            if (known[i].tiles == tiles && known[i].M == a.M && known[i].units == a.units && known[i].dev == dev) c = known[i].c;
-    }
-    if (!c.T) {
-        c = cut(tiles, a.M, a.units, P::kBlocks, [&](uint32_t T, uint32_t split) {
-            return resident_ctas(reinterpret_cast<const void *>(kern), kThreads, lay_out(T, P::kStage, P::kBlocks).smem, split);
-        });
-        if (!c.T) return (int)cudaErrorNotSupported;
-        std::lock_guard<std::mutex> lock(mu);
-        known[used % 32] = Known{tiles, a.M, a.units, dev, c};
-        used = used + 1 >= 64 ? 32 : used + 1;
-    }
-    const Layout l = lay_out(c.T, P::kStage, P::kBlocks);
-    a.T = c.T; a.split = c.split; a.nw = l.nw; a.ns = l.ns; a.at_x = l.at_x; a.at_bar = l.at_bar;
+    const Plan p = plan_for<GRAD, BITS>(w.N, w.K, a.M, nw);
+    const Layout l = lay_out(p.T, P::kStage);
+    const uint32_t at_once = resident_ctas(reinterpret_cast<const void *>(kern), kThreads, l.smem, 2) / 2u;
+    if (!at_once) return (int)cudaErrorNotSupported;
+    a.T = p.T; a.tok_tiles = p.tok_tiles; a.tiles = p.tiles; a.per_tile = p.per_tile; a.per_weight = p.per_weight;
+    a.nw = l.nw; a.ns = l.ns; a.nd = l.nd; a.at_x = l.at_x; a.at_out = l.at_out; a.at_bar = l.at_bar;
+    a.count = static_cast<uint32_t *>(scratch);
+    a.partial = reinterpret_cast<float *>(static_cast<uint8_t *>(scratch) + count_bytes(p));
     CUtensorMap maps[2], xmap;
     constexpr CUtensorMapSwizzle sw = P::kBytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : P::kBytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B;
     for (int i = 0; i < 2; i++)
         if (!map_2d(maps[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, w.codes[i], w.row_bytes, w.N, w.row_bytes, P::kBytes, GRAD ? kRows : kRows / 2, sw)) return (int)cudaErrorNotSupported;
-    if (!map_2d(xmap, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, x, GRAD ? w.N : w.K, (uint64_t)a.M * (GRAD ? nw : 1), (uint64_t)pitch * 2, 64, c.T, CU_TENSOR_MAP_SWIZZLE_128B))
+    if (!map_2d(xmap, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, x, GRAD ? w.N : w.K, (uint64_t)a.M * (GRAD ? nw : 1), (uint64_t)pitch * 2, 64, p.T / 2u, CU_TENSOR_MAP_SWIZZLE_128B))
         return (int)cudaErrorNotSupported;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(tiles * c.split, c.tok_tiles);
+    cfg.gridDim = dim3(2u * std::min(p.pairs, at_once));
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = l.smem;
     cfg.stream = st;
@@ -598,7 +762,7 @@ int run(ProductArgs a, const PackedPair &w, int nw, const void *x, uint32_t pitc
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = programmatic_launches();
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = c.split; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+    attr[1].val.clusterDim.x = 2; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a, maps[0], maps[1], xmap);
@@ -611,6 +775,7 @@ ProductArgs common(const PackedPair &w, const float *factor, uint32_t M, void *y
     ProductArgs a = {};
     a.scales[0] = w.scales[0]; a.scales[1] = w.scales[1];
     a.factor = factor; a.y = y; a.N = w.N; a.K = w.K; a.M = M; a.group = w.group; a.groups = w.K / w.group; a.dtype = dtype;
+    a.inverse = (uint32_t)(((1ull << 32) + w.group / 16u - 1) / (w.group / 16u));
     a.limit = g_limit.load(std::memory_order_relaxed);
     return a;
 }
@@ -621,28 +786,39 @@ bool product_takes(const PackedPair &w, int nw)
 {
     for (int i = 0; i < nw; i++)
         if (!qmm_takes(w.K, w.bits, w.group, w.codes[i], w.codes[i])) return false;
-    return true;
+    return w.K < 1u << 20;                     // (group_of: K / 16 times group / 16 is below 2^32)
 }
 
-int launch_gated_product(const GatedCall &c, const uint16_t *x, const float *factor, void *stream)
+Scratch gated_product_scratch(const PackedPair &w, uint32_t M)
+{
+    const Plan p = plan_of<false>(w.N, w.K, w.bits, M, 1);
+    return Scratch{scratch_bytes(p), p.tiles * 2u};
+}
+Scratch input_grad_product_scratch(const PackedPair &w, int nw, uint32_t M)
+{
+    const Plan p = plan_of<true>(w.N, w.K, w.bits, M, nw);
+    return Scratch{scratch_bytes(p), p.tiles * 2u};
+}
+
+int launch_gated_product(const GatedCall &c, const uint16_t *x, const float *factor, void *scratch, void *stream)
 {
     ProductArgs a = common(c.w, factor, c.M, c.h, c.dtype);
     a.bias[0] = c.bias[0]; a.bias[1] = c.bias[1];
     a.keep = c.keep;
     a.act = c.act;
     cudaStream_t st = (cudaStream_t)stream;
-    if (c.w.bits == 4) return run<false, 4>(a, c.w, 2, x, c.w.K, st);
-    if (c.w.bits == 2) return run<false, 2>(a, c.w, 2, x, c.w.K, st);
-    return run<false, 8>(a, c.w, 2, x, c.w.K, st);
+    if (c.w.bits == 4) return run<false, 4>(a, c.w, 2, x, c.w.K, scratch, st);
+    if (c.w.bits == 2) return run<false, 2>(a, c.w, 2, x, c.w.K, scratch, st);
+    return run<false, 8>(a, c.w, 2, x, c.w.K, scratch, st);
 }
 
-int launch_input_grad_product(const PackedPair &w, int nw, const uint16_t *dy, uint32_t pitch, const float *factor, uint32_t M, void *dx, int dtype, void *stream)
+int launch_input_grad_product(const PackedPair &w, int nw, const uint16_t *dy, uint32_t pitch, const float *factor, uint32_t M, void *dx, int dtype, void *scratch, void *stream)
 {
     const ProductArgs a = common(w, factor, M, dx, dtype);
     cudaStream_t st = (cudaStream_t)stream;
-    if (w.bits == 4) return run<true, 4>(a, w, nw, dy, pitch, st);
-    if (w.bits == 2) return run<true, 2>(a, w, nw, dy, pitch, st);
-    return run<true, 8>(a, w, nw, dy, pitch, st);
+    if (w.bits == 4) return run<true, 4>(a, w, nw, dy, pitch, scratch, st);
+    if (w.bits == 2) return run<true, 2>(a, w, nw, dy, pitch, scratch, st);
+    return run<true, 8>(a, w, nw, dy, pitch, scratch, st);
 }
 
 void set_gated_wait_us(int v) { g_limit.store(std::min(std::max(v, 0), 60000000) * 2000ll); }
