@@ -44,7 +44,7 @@ __device__ uint32_t g_gated_status = 0;
 namespace {
 
 constexpr uint32_t kRows = 128;            // of a weight tile
-constexpr int kSets = 4;                   // producer sets of four warps, one per quadrant of tensor memory
+constexpr int kSets = 6;                   // producer sets of four warps, one per quadrant of tensor memory
 constexpr int kWProducts = 4 * kSets, kWCodes = kWProducts + 1, kWTokens = kWProducts + 2, kWScales = kWProducts + 3, kWOut = kWProducts + 4;      // warps
 constexpr uint32_t kThreads = (kWOut + 4) * 32, kTmem = 512, kOut = 8 * 2048 + 8 * 128;       // shared memory of the way out: sixteen tokens of a warp, and their maxima, twice
 
@@ -72,8 +72,15 @@ __device__ __forceinline__ uint32_t in_cta(uint32_t addr, uint32_t rank)
     return r;
 }
 // at a barrier of either CTA.  What is handed over lies in tensor memory, whose order tcgen05's fences keep: without a scope of the cluster, which
-// costs a fence of memory each time (920 clocks a block of 16 tokens, against 330).
-__device__ __forceinline__ void arrive_cluster(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
+// costs a fence of memory each time (920 clocks a block of 16 tokens, against 650).  A predicate, not a branch: the warp stays together.
+__device__ __forceinline__ void arrive_cluster_if(uint32_t bar, bool yes)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %1, 0;\n\t@p mbarrier.arrive.shared::cluster.b64 _, [%0];\n\t}" ::"r"(bar), "r"((uint32_t)yes) : "memory");
+}
+__device__ __forceinline__ void bar_arrive_if(uint32_t bar, bool yes)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %1, 0;\n\t@p mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}" ::"r"(bar), "r"((uint32_t)yes) : "memory");
+}
 // a copy to this CTA whose bytes are counted by a barrier of either CTA of the pair
 __device__ __forceinline__ void tma_2d_pair(uint32_t dst, const CUtensorMap *map, uint32_t x, uint32_t y, uint32_t bar)
 {
@@ -158,8 +165,14 @@ __device__ __forceinline__ void ldmatrix_trans(uint32_t addr, uint32_t (&r)[4])
 {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
+// sixteen values exist from here on
+__device__ __forceinline__ void use16(const uint32_t *r)
+{
+    asm volatile("" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
+                 "r"(r[14]), "r"(r[15]) : "memory");
+}
 // sixteen lanes x 32 columns: register 2 b to lane (thread / 4), column 4 b + thread % 4, register 2 b + 1 to lane 8 + thread / 4
-__device__ __forceinline__ void tmem_st_16x128b(uint32_t addr, const uint32_t (&r)[16])
+__device__ __forceinline__ void tmem_st_16x128b(uint32_t addr, const uint32_t *r)
 {
     asm volatile("tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
                  ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
@@ -264,14 +277,16 @@ gated_product_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap gm
             at += s.p1 - s.p0;
             const uint32_t row0 = first_row(s.tile);
             for (uint32_t p = s.p0; p < s.p1; p++, wr.next(a.nw)) {
+                static_assert(P::kBlocks <= kSets, "a set has one block of a piece, or none");
                 const uint32_t have = GRAD ? P::kBlocks : min(P::kBlocks, (a.K + 63u) / 64u - p * P::kBlocks), ws = wr.at;
+                const bool work = turn < have;
                 wait(bar(bWFull + ws), wr.lap);
-                for (; turn < have; turn += kSets) {
-                    const uint32_t st = ar.at;
+                uint32_t h[32];
+                if (work) {
                     if constexpr (!GRAD) {
                         constexpr int kWords = BITS == 4 ? 8 : BITS == 2 ? 4 : 16;
                         const uint32_t row_at = base + ws * P::kStage + r * P::kBytes, sw = BITS == 2 ? (r >> 1) & 3u : r & 7u;
-                        uint32_t w[kWords], h[32];
+                        uint32_t w[kWords];
 #pragma unroll
                         for (uint32_t c = 0; c < kWords / 4; c++)
                             asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[4 * c]), "=r"(w[4 * c + 1]), "=r"(w[4 * c + 2]), "=r"(w[4 * c + 3])
@@ -284,10 +299,6 @@ gated_product_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap gm
                             asm volatile("ld.shared.u16 %0, [%1];" : "=h"(sc[j]) : "r"(scales_at + ws * kScales + (group_of(min(k + j * 32u, a.K - 1u)) - g0) * (kRows * 2u) + r * 2u));
 #pragma unroll
                         for (int c = 0; c < kWords; c++) codes_scaled<BITS, false>(w[c], h + c * (32 / kWords), c < kWords / 2 ? sc[0] : sc[1]);
-                        wait(bar(bEmpty + st), ar.lap ^ 1u);
-                        fence_after();
-                        __syncwarp();
-                        tmem_st32(lane_base + st * 32u, h);
                     } else {
                         constexpr int kChunks = BITS == 8 ? 2 : 1;            // 16-byte pieces of a weight row that a quadrant's 32 columns take
                         const uint32_t rows_at = base + ws * P::kStage, chunk = BITS == 4 ? q : BITS == 8 ? 2u * q : q >> 1;
@@ -306,7 +317,6 @@ gated_product_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap gm
                                 ldmatrix_trans(rows_at + n * P::kBytes + (((chunk + c) ^ sw) << 4), m[c][hh]);
                             }
                         // sixteen lanes of tensor memory at a time: code j of the registers to lanes 0 .. 7, code j + 1 to lanes 8 .. 15
-                        uint32_t h[2][16];
 #pragma unroll
                         for (int half = 0; half < 2; half++)
 #pragma unroll
@@ -315,26 +325,35 @@ gated_product_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap gm
                                 for (int j = 0; j < 2; j++) {
                                     uint32_t v = m[BITS == 8 ? half : 0][b >> 2][b & 3];
                                     if (BITS == 2) v >>= (q & 1u) * 8u;
-                                    h[half][2 * b + j] = hmul2(row_pair<BITS>(v, (BITS == 8 ? 0 : 2 * half) + j), sp[b]);
+                                    h[half * 16 + 2 * b + j] = hmul2(row_pair<BITS>(v, (BITS == 8 ? 0 : 2 * half) + j), sp[b]);
                                 }
-                        wait(bar(bEmpty + st), ar.lap ^ 1u);
-                        fence_after();
-                        __syncwarp();
-                        tmem_st_16x128b(lane_base + st * 32u, h[0]);
-                        tmem_st_16x128b(lane_base + (16u << 16) + st * 32u, h[1]);
+                    }
+                    // every code has left shared memory when all of these are there, and only then may the copy engine have the stage
+                    use16(h);
+                    use16(h + 16);
+                }
+                __syncwarp();
+                bar_arrive_if(bar(bWEmpty + ws), lane == 0 && !wait.lost);
+                if (work) {
+                    const uint32_t to = lane_base + ar.at * 32u;
+                    wait(bar(bEmpty + ar.at), ar.lap ^ 1u);
+                    fence_after();
+                    __syncwarp();
+                    if constexpr (!GRAD) {
+                        tmem_st32(to, h);
+                    } else {
+                        tmem_st_16x128b(to, h);
+                        tmem_st_16x128b(to + (16u << 16), h + 16);
                     }
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                     fence_before();
                     __syncwarp();
-                    // (a CTA that has given up tells nobody: an arrival beyond a barrier's count while a copy is under way would break it)
-                    if (lane == 0 && !wait.lost) arrive_cluster(full0 + 8u * st);
+                    arrive_cluster_if(full0 + 8u * ar.at, lane == 0 && !wait.lost);
                     ar.at += kSets;
                     if (ar.at >= a.ns) { ar.at -= a.ns; ar.lap ^= 1u; }
+                    turn += kSets;
                 }
                 turn -= have;
-                // every lane's codes are converted and stored: only now may the copy engine have the stage
-                __syncwarp();
-                if (lane == 0 && !wait.lost) bar_arrive(bar(bWEmpty + ws));
             }
         }
     } else if (warp == kWProducts) {
@@ -416,7 +435,7 @@ gated_product_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap gm
         // ---- scales of a piece, [group][row], fetched some pieces ahead (one at a time, their latency is what bounds the launch).  Gradient: zero
         // past the last weight row, so that what lies behind it (there the activations are zeros) cannot be an infinity.
         constexpr uint32_t kGroups = GRAD ? 4u : 8u;
-        constexpr int kAhead = GRAD ? 4 : 2;
+        constexpr int kAhead = GRAD ? 2 : 1;
         struct Fetched { uint16_t v[4][kGroups]; uint32_t ng; };
         struct { uint64_t at; uint32_t p, p1, row0; } c = {run0, 0u, 0u, 0u};       // what is to be fetched next
         auto fetch = [&](Fetched &f) {
@@ -466,7 +485,7 @@ gated_product_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap gm
                     for (uint32_t g = 0; g < kGroups; g++)
                         if (g < f[d].ng) asm volatile("st.shared.u16 [%0], %1;" ::"r"(scales_at + wr.at * kScales + g * (kRows * 2u) + j * 64u + lane * 2u), "h"(f[d].v[j][g]) : "memory");
                 __syncwarp();
-                if (lane == 0 && !wait.lost) bar_arrive(bar(bWFull + wr.at));
+                bar_arrive_if(bar(bWFull + wr.at), lane == 0 && !wait.lost);
                 wr.next(a.nw);
                 fetch(f[d]);
             }
@@ -566,20 +585,20 @@ gated_product_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap gm
                     if (a.keep.form == kKeep8bit) {
                         // the tile's 64 features of a token are one block of the 8-bit form: this warp's 32, and its neighbour's
                         const uint32_t to = maxima + (turn * 4u + q) * 128u, from = maxima + (turn * 4u + (q ^ 1u)) * 128u;
-                        uint32_t most[2][16];
 #pragma unroll
                         for (uint32_t j = 0; j < 16; j++) {
-                            most[0][j] = __reduce_max_sync(0xffffffffu, there ? __float_as_uint(g[j]) & 0x7fffffffu : 0u);
-                            most[1][j] = __reduce_max_sync(0xffffffffu, there ? __float_as_uint(u[j]) & 0x7fffffffu : 0u);
-                            if (lane == 0) asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to + j * 8u), "r"(most[0][j]), "r"(most[1][j]) : "memory");
+                            const uint32_t mg = __reduce_max_sync(0xffffffffu, there ? __float_as_uint(g[j]) & 0x7fffffffu : 0u);
+                            const uint32_t mu = __reduce_max_sync(0xffffffffu, there ? __float_as_uint(u[j]) & 0x7fffffffu : 0u);
+                            if (lane == 0) asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to + j * 8u), "r"(mg), "r"(mu) : "memory");
                         }
                         asm volatile("bar.sync %0, 64;" ::"r"(3u + (q >> 1)) : "memory");
 #pragma unroll
                         for (uint32_t j = 0; j < 16; j++) {
-                            uint32_t eg, eu;
-                            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(eg), "=r"(eu) : "r"(from + j * 8u));
+                            uint32_t mg, mu, eg, eu;
+                            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(mg), "=r"(mu) : "r"(to + j * 8u) : "memory");
+                            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(eg), "=r"(eu) : "r"(from + j * 8u) : "memory");
                             if (!work || t + j >= tokens) continue;
-                            const Storer sg(max(most[0][j], eg)), su(max(most[1][j], eu));
+                            const Storer sg(max(mg, eg)), su(max(mu, eu));
                             const size_t m = tok0 + t + j, at = m * a.N + n, block = m * ((a.N + kStoreBlock - 1) / kStoreBlock) + row0 / 64u;
                             if (there) {
                                 reinterpret_cast<int8_t *>(a.keep.v[0])[at] = sg.code(g[j]);
@@ -609,7 +628,7 @@ gated_product_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap gm
             auto release = [&]() {                               // the next tile may have the accumulator
                 fence_before();
                 __syncwarp();
-                if (lane == 0 && !wait.lost) arrive_cluster(empty0 + 8u * dr.at);
+                arrive_cluster_if(empty0 + 8u * dr.at, lane == 0 && !wait.lost);
             };
             if (s.p1 - s.p0 == a.per_tile) {
                 finish(s.tile, take, release);
@@ -669,13 +688,14 @@ std::atomic<long long> g_limit{4000000000ll};      // about two seconds
 
 struct Layout { uint32_t nw, ns, nd, at_x, at_out, at_bar; size_t smem; };
 
-// Operand stages in multiples of the producer sets, which take them in turn.
+// Two accumulators where they leave as many stages of operands as there are producer sets: these wait for a stage's last use by its parity, which is
+// right while the use before that is behind, and the set's own last block is `kSets` back.
 Layout lay_out(uint32_t T, uint32_t stage_w)
 {
     const uint32_t fixed = 1024 + 8 * bEnd + 8, room = 226u * 1024u - fixed - kOut, xstage = T * 64u;
     Layout l = {};
-    l.nd = 2u * T + 4u * 32u <= kTmem ? 2u : 1u;
-    l.ns = l.nd * T + 8u * 32u <= kTmem ? 8u : 4u;
+    l.nd = 2u * T + kSets * 32u <= kTmem ? 2u : 1u;
+    l.ns = std::min(8u, (kTmem - l.nd * T) / 32u);
     l.nw = std::min(8u, (room - l.ns * xstage) / (stage_w + kScales));
     l.at_x = l.nw * stage_w;
     l.at_out = l.at_x + l.ns * xstage;
@@ -684,15 +704,15 @@ Layout lay_out(uint32_t T, uint32_t stage_w)
     return l;
 }
 
-// Tokens of a tile: as few tiles as pay.  A block of 64 costs its products (two clocks a token) or its producers' work (some 330), whichever is
-// longer; with one accumulator a tile's way out (some 24 clocks a token) comes on top.
+// Tokens of a tile: as few tiles as pay.  A block of 64 costs its products (two clocks a token) or its producers' work (some 400), whichever is
+// longer; with one accumulator a tile's way out (some 100 clocks a token) comes on top.
 uint32_t tile_tokens(uint32_t M, uint32_t blocks)
 {
     uint32_t best = 0;
     double least = 1e30;
     for (uint32_t n = (M + 255u) / 256u; n < (M + 255u) / 256u + 4u; n++) {
         const uint32_t T = ((M + n - 1) / n + 15u) / 16u * 16u;
-        const double cost = (double)((M + T - 1) / T) * (blocks * std::max(500.0, 2.0 * T) + (T > 192u ? 100.0 * T : 0.0));
+        const double cost = (double)((M + T - 1) / T) * (blocks * std::max(400.0, 2.0 * T) + (T > 160u ? 100.0 * T : 0.0));
         if (cost < 0.999 * least) { least = cost; best = T; }
     }
     return best;
@@ -715,7 +735,7 @@ Plan plan_for(uint32_t N, uint32_t K, uint32_t M, int nw)
     p.pairs = std::min(room, p.tiles);
     if (p.tiles < room) {
         double least = 1e30;
-        const double block = std::max(330.0, 2.0 * p.T);
+        const double block = std::max(400.0, 2.0 * p.T);
         for (uint32_t n = p.tiles; n <= room && n <= (uint64_t)p.tiles * p.per_tile; n++) {
             const double parts = (double)n / p.tiles, pieces = std::ceil((double)p.tiles * p.per_tile / n);
             const double cost = pieces * P::kBlocks * block + (n > p.tiles ? 4000.0 + std::ceil(p.T / 32.0) * 800.0 * (1.0 + std::ceil(parts)) : 0.0);
