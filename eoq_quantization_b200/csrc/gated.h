@@ -70,7 +70,7 @@ Scratch input_grad_product_scratch(const PackedPair &w, int nw, uint32_t M);
 int launch_gated_product(const GatedCall &c, const uint16_t *x, const float *factor, void *scratch, void *stream);
 int launch_input_grad_product(const PackedPair &w, int nw, const uint16_t *dy, uint32_t pitch, const float *factor, uint32_t M, void *dx, int dtype, void *scratch,
                               void *stream);
-// Up to eight rows of 16-bit activations, 16-byte aligned; kept in full or in fp32 (gated_rows.cu).
+// Up to 32 rows of 16-bit activations, 16-byte aligned; kept in full or in fp32 (gated_rows.cu).
 bool gated_rows_takes(const PackedPair &w, uint32_t batch);
 int launch_gated_rows(const GatedCall &c, void *stream);
 long long gated_wait_limit();

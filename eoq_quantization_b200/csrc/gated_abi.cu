@@ -56,7 +56,7 @@ bool exact_products(const PackedPair &w, int dtype, const void *codes, const voi
     return dtype == EOQ_B200_F32 && qmm_takes(w.K, w.bits, w.group, codes, x) && split_rows_takes(w.K, 1);
 }
 
-// Up to eight rows of 16-bit activations: one pass over the codes.
+// Up to 32 rows of 16-bit activations: one pass over the codes.
 bool few_rows(const PackedPair &w, int dtype, uint32_t batch) { return dtype != EOQ_B200_F32 && gated_rows_takes(w, batch); }
 
 // 16-bit activations on the tensor cores: fp16 rows as they are, where copies of them can be aligned; others as fp16 times a

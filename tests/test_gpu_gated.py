@@ -25,6 +25,9 @@ SHAPES = [
     (129, 320, 768, 4, 128, BF16), (257, 96, 320, 4, 64, F16), (300, 1000, 512, 4, 128, F16), (513, 65, 256, 4, 128, BF16),
     (40, 257, 384, 8, 128, F16), (70, 127, 320, 8, 32, BF16), (40, 257, 512, 2, 128, BF16), (280, 190, 256, 2, 64, F16),
     (5, 301, 512, 4, 128, F32), (40, 66, 256, 8, 64, F32),
+    # several slices of activations, several tiles a CTA, groups of several units
+    (32, 1201, 8192, 4, 128, F16), (19, 1190, 2816, 8, 64, BF16), (17, 130, 512, 2, 64, BF16), (30, 77, 256, 8, 32, F16), (12, 64, 768, 4, 256, F16),
+    (25, 40, 1024, 2, 128, F16), (10, 200, 1536, 4, 96, BF16), (31, 9500, 256, 4, 32, BF16), (4, 70, 768, 4, 256, BF16), (1, 2500, 4096, 4, 128, BF16),
     # rows that end inside a scale group, odd columns, other widths, odd groups
     (3, 50, 200, 4, 128, F16), (20, 33, 77, 4, 16, BF16), (2, 30, 90, 2, 24, F32), (11, 45, 96, 3, 48, F16), (6, 20, 40, 6, 40, BF16),
     (17, 40, 130, 8, 130, F16),
