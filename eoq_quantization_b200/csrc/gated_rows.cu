@@ -16,11 +16,33 @@
 #include "tensor_core.h"
 
 #include <algorithm>
+#include <type_traits>
 
 #include "activations.cuh"
 
 namespace eoq {
 namespace {
+
+// Scales of `ntiles` tiles from tile0 on to shared memory by whole rows, [gate, up][row][pitch]: a load of a few of each row would touch as many
+// lines as one of their codes.  Eight rows a warp and step, all requested before the first is stored.
+template <bool WORDS>
+__device__ __forceinline__ void fetch_scales(const uint16_t *gate, const uint16_t *up, uint32_t *to, uint32_t tile0, uint32_t ntiles, uint32_t N, uint32_t groups,
+                                             uint32_t pitch, uint32_t warp, uint32_t nwarps, uint32_t lane)
+{
+    using T = std::conditional_t<WORDS, uint32_t, uint16_t>;       // two groups at a time, or one
+    const uint32_t rows = ntiles * 16u, half = ntiles * 8u, count = WORDS ? groups / 2u : groups;
+    for (uint32_t j = lane; j < count; j += 32u)
+        for (uint32_t r0 = warp; r0 < rows; r0 += 8u * nwarps) {
+            T v[8];
+#pragma unroll
+            for (uint32_t i = 0; i < 8; i++) {
+                const uint32_t row = min(r0 + i * nwarps, rows - 1u), n = min(tile0 * 8u + (row >= half ? row - half : row), N - 1u);
+                v[i] = __ldg(reinterpret_cast<const T *>((row >= half ? up : gate) + (size_t)n * groups) + j);
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < 8; i++) if (r0 + i * nwarps < rows) reinterpret_cast<T *>(to + (r0 + i * nwarps) * pitch)[j] = v[i];
+        }
+}
 
 // The addresses of a chunk's loads come from here, behind the wait for it: the loads themselves may move among the products.
 __device__ __forceinline__ void pin(uint32_t &w, uint32_t &x, uint32_t &s) { asm volatile("" : "+r"(w), "+r"(x), "+r"(s)::"memory"); }
@@ -52,52 +74,15 @@ __device__ __forceinline__ uint4 piece_load(const uint16_t *x, uint32_t span, ui
         const uint32_t j = i >> 1, c = span * 128u + (U == 128 ? t * 32u + j * 16u : j * 64u + t * 16u) + (i & 1u) * 4u;
         const uint2 a = __ldg(reinterpret_cast<const uint2 *>(x + c)), b = __ldg(reinterpret_cast<const uint2 *>(x + c + 8u));
         return make_uint4(a.x, a.y, b.x, b.y);
+    } else {
+        return __ldg(reinterpret_cast<const uint4 *>(x + span * 128u + (U == 128 ? t * 32u + i * 8u : U == 64 ? (i >> 1) * 64u + t * 16u + (i & 1u) * 8u : i * 32u + t * 8u)));
     }
-    return __ldg(reinterpret_cast<const uint4 *>(x + span * 128u + (U == 128 ? t * 32u + i * 8u : U == 64 ? (i >> 1) * 64u + t * 16u + (i & 1u) * 8u : i * 32u + t * 8u)));
 }
 template <int BITS>
 __device__ __forceinline__ uint4 piece_order(const uint4 &v)
 {
     if constexpr (BITS == 8) return v;
-    return make_uint4(__byte_perm(v.x, v.z, 0x5410u), __byte_perm(v.x, v.z, 0x7632u), __byte_perm(v.y, v.w, 0x5410u), __byte_perm(v.y, v.w, 0x7632u));
-}
-
-// The addresses of a chunk's loads come from here, behind the wait for it: the loads themselves may move among the products.
-__device__ __forceinline__ void pin(uint32_t &w, uint32_t &x, uint32_t &s) { asm volatile("" : "+r"(w), "+r"(x), "+r"(s)::"memory"); }
-
-struct RowsArgs {
-    const uint16_t *scales[2];
-    const float *bias[2];
-    const void *x;
-    void *h;
-    void *kept[2];               // [batch][N] of x's type, fp32 (kept32), or null
-    uint32_t N, K, group, batch, per, more;      // tiles a CTA takes, and how many CTAs take one more
-    uint32_t most, pitch, slots; // tiles at a time, words that a row's scales take in shared memory, chunks of a warp's ring
-    int act, kept32;
-    long long limit;             // clock ticks a wait may take
-    uint32_t *status;            // set when one runs out
-};
-
-constexpr int most_threads(int bt) { return bt == 1 ? 1024 : 768; }        // 64 or 80 registers a thread
-constexpr int kParts = 3;        // tiles that a warp's run touches at most, for up to two tiles a warp
-
-// A unit (half of one, where that has 128 bytes) in bytes and columns: a lane takes a quarter of it.
-template <int BITS, int U> struct Part { static constexpr int kBytes = U * BITS / 8 < 64 ? U * BITS / 8 : 64, kCols = kBytes * 8 / BITS; };
-
-// x in the order of the codes: sixteen-byte pieces [span][i][row][t], piece i of lane (row, t) the columns of its registers 4 i .. 4 i + 3.
-template <int BITS, int U>
-__device__ __forceinline__ uint4 piece_of(const uint16_t *x, uint32_t span, uint32_t i, uint32_t t)
-{
-    if constexpr (BITS == 2) {       // columns 16 j + (r & 7) and + 8 of a lane's, j = i / 2
-        const uint32_t j = i >> 1, c = span * 128u + (U == 128 ? t * 32u + j * 16u : j * 64u + t * 16u) + (i & 1u) * 4u;
-        const uint2 a = __ldg(reinterpret_cast<const uint2 *>(x + c)), b = __ldg(reinterpret_cast<const uint2 *>(x + c + 8u));
-        return make_uint4(__byte_perm(a.x, b.x, 0x5410u), __byte_perm(a.x, b.x, 0x7632u), __byte_perm(a.y, b.y, 0x5410u), __byte_perm(a.y, b.y, 0x7632u));
-    } else {
-        const uint32_t c = span * 128u + (U == 128 ? t * 32u + i * 8u : U == 64 ? (i >> 1) * 64u + t * 16u + (i & 1u) * 8u : i * 32u + t * 8u);
-        const uint4 v = __ldg(reinterpret_cast<const uint4 *>(x + c));
-        if constexpr (BITS == 8) return v;
-        return make_uint4(__byte_perm(v.x, v.z, 0x5410u), __byte_perm(v.x, v.z, 0x7632u), __byte_perm(v.y, v.w, 0x5410u), __byte_perm(v.y, v.w, 0x7632u));
-    }
+    else return make_uint4(__byte_perm(v.x, v.z, 0x5410u), __byte_perm(v.x, v.z, 0x7632u), __byte_perm(v.y, v.w, 0x5410u), __byte_perm(v.y, v.w, 0x7632u));
 }
 
 // U: columns of a unit whose scale is applied on its own.
@@ -164,15 +149,7 @@ __global__ void __launch_bounds__(most_threads(BT), 1) gated_rows_kernel(const R
             *reinterpret_cast<volatile uint32_t *>(a.status) = 1u;
         }
     };
-    // Scales by whole rows to shared memory: a load of a few of each row would touch as many lines as one of their codes.
-    auto fetch_scales = [&]() {
-        for (uint32_t row = warp; row < ntiles * 16u; row += nwarps) {
-            const uint32_t which = row >= ntiles * 8u, n = min(tile0 * 8u + row - which * ntiles * 8u, a.N - 1u);
-            const uint16_t *from = (which ? a.scales[1] : a.scales[0]) + (size_t)n * sgroups;
-            if (EXACT && CH * kUnits > 1) for (uint32_t j = lane; j < sgroups / 2u; j += 32u) scales[row * a.pitch + j] = __ldg(reinterpret_cast<const uint32_t *>(from) + j);
-            else for (uint32_t j = lane; j < sgroups; j += 32u) reinterpret_cast<uint16_t *>(scales + row * a.pitch)[j] = __ldg(from + j);
-        }
-    };
+    auto fetch = [&]() { fetch_scales<EXACT && (CH * kUnits > 1)>(a.scales[0], a.scales[1], scales, tile0, ntiles, a.N, sgroups, a.pitch, warp, nwarps, lane); };
 
     // codes and scales do not depend on the kernel before this one in the stream, the activations may
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -182,7 +159,7 @@ __global__ void __launch_bounds__(most_threads(BT), 1) gated_rows_kernel(const R
     __syncwarp();
     begin();
     for (uint32_t i = 0; i < a.slots; i++) load(i);
-    fetch_scales();
+    fetch();
     asm volatile("griddepcontrol.wait;" ::: "memory");
     for (uint32_t e = threadIdx.x; e < chunks * kPieces; e += blockDim.x) {
         const uint32_t tt = e & 3u, b = (e >> 2) % BT, i = (e >> 2) / BT & 3u, s = e / (16u * BT);
@@ -358,7 +335,7 @@ __global__ void __launch_bounds__(most_threads(BT), 1) gated_rows_kernel(const R
         begin();
         // (the slots in the order in which the ring comes by them)
         for (uint32_t i = 0, slot = at_slot.at; i < a.slots; i++, slot = slot + 1 == a.slots ? 0 : slot + 1) load(slot);
-        fetch_scales();
+        fetch();
         __syncthreads();
     }
 }
@@ -478,12 +455,7 @@ gated_many_rows_kernel(const ManyArgs a, const __grid_constant__ CUtensorMap gma
                 requested += a.split;
             };
             for (uint32_t i = 0, slot = wr.at; i < kSlots; i++, slot ^= 1u) request(slot);
-            for (uint32_t row = warp; row < ntiles * 16u; row += nwarps) {
-                const uint32_t which = row >= ntiles * 8u, n = min(tile0 * 8u + row - which * ntiles * 8u, a.N - 1u);
-                const uint16_t *from = (which ? a.scales[1] : a.scales[0]) + (size_t)n * sgroups;
-                if (EXACT && CH * kUnits > 1) for (uint32_t j = lane; j < sgroups / 2u; j += 32u) scales[row * a.pitch + j] = __ldg(reinterpret_cast<const uint32_t *>(from) + j);
-                else for (uint32_t j = lane; j < sgroups; j += 32u) reinterpret_cast<uint16_t *>(scales + row * a.pitch)[j] = __ldg(from + j);
-            }
+            fetch_scales<EXACT && (CH * kUnits > 1)>(a.scales[0], a.scales[1], scales, tile0, ntiles, a.N, sgroups, a.pitch, warp, nwarps, lane);
             asm volatile("bar.sync 1, %0;" ::"r"(nwarps * 32u) : "memory");
             asm volatile("griddepcontrol.wait;" ::: "memory");         // (the time of the kernels before this one is not a slice's)
             const uint32_t s0 = saddr(scales) + (my_tile * 8u + myrow) * a.pitch * 4u, up = ntiles * 32u * a.pitch;
