@@ -113,7 +113,7 @@ class TilesView(C.Structure):
 
 class Gated(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("gate", "up", "gate_scales", "up_scales", "gate_bias", "up_bias")] + \
-               [(n, C.c_uint32) for n in ("rows", "cols", "bits", "group")] + [("activation", C.c_int)]
+               [(n, C.c_uint32) for n in ("rows", "cols", "bits", "group")] + [("activation", C.c_int), ("bias_dtype", C.c_int)]
 
 
 class Kept(C.Structure):

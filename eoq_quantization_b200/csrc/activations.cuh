@@ -3,11 +3,20 @@
 #pragma once
 
 #include <cstdint>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include "gated.h"
 
 namespace eoq {
+
+__device__ __forceinline__ float bias_at(const void *p, uint32_t n, int dtype)
+{
+    if (!p) return 0.0f;
+    if (dtype == EOQ_B200_F32) return __ldg(reinterpret_cast<const float *>(p) + n);
+    const uint16_t b = __ldg(reinterpret_cast<const uint16_t *>(p) + n);
+    return dtype == EOQ_B200_F16 ? __half2float(__ushort_as_half(b)) : __uint_as_float((uint32_t)b << 16);
+}
 
 // value and derivative: silu g s(g), s(g) (1 + g (1 - s(g))); gelu g P(g), P(g) + g p(g) of the normal distribution; gelu_tanh with
 // P(g) = (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))) / 2

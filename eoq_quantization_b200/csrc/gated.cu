@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(256) gated_general_kernel(const GatedCall c)
             for (int j = 0; j < 2; j++) {
                 const uint32_t m = m0 + ty + 16 * i, n = n0 + tx + 16 * j;
                 if (m >= c.M || n >= w.N) continue;
-                const float g = acc[0][i][j] + (c.bias[0] ? __ldg(c.bias[0] + n) : 0.0f), u = acc[1][i][j] + (c.bias[1] ? __ldg(c.bias[1] + n) : 0.0f);
+                const float g = acc[0][i][j] + bias_at(c.bias[0], n, c.bias_dtype), u = acc[1][i][j] + bias_at(c.bias[1], n, c.bias_dtype);
                 const size_t at = (size_t)m * w.N + n;
                 store_from_float(c.h, at, activation(g, c.act) * u, c.dtype);
                 if (c.keep.form == kKeepFull || c.keep.form == kKeepF32) {

@@ -30,11 +30,11 @@ struct Kept {
 
 struct GatedCall {
     PackedPair w;
-    const float *bias[2];
+    const void *bias[2];         // of bias_dtype, or null
     const void *x;               // [M][K]
     void *h;                     // [M][N]
     uint32_t M;
-    int dtype, act;
+    int dtype, act, bias_dtype;
     Kept keep;
 };
 

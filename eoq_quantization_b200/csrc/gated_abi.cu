@@ -97,12 +97,12 @@ extern "C" eoq_error_t eoq_b200_gated_packed(const eoq_b200_gated_t *w, const vo
     const int form = kept ? kept->form : kKeepNone;
     if (form != kKeepNone && (!kept->gate || !kept->up || (form == kKeep8bit && (!kept->gate_scales || !kept->up_scales)))) return EOQ_ERR_NULL_PTR;
     if (batch == 0 || w->rows == 0) return EOQ_OK;
-    if (dtype < 0 || dtype > 2 || form < 0 || form > kKeep8bit || w->activation < 0 || w->activation > kActGeluTanh) return EOQ_ERR_UNSUPPORTED;
+    if (dtype < 0 || dtype > 2 || w->bias_dtype < 0 || w->bias_dtype > 2 || form < 0 || form > kKeep8bit || w->activation < 0 || w->activation > kActGeluTanh) return EOQ_ERR_UNSUPPORTED;
     if (!fine(w->rows, w->cols, w->bits, w->group)) return EOQ_ERR_INVALID_HEADER;
     if (eoq_b200_gated_scratch(w, kept, dtype, batch) && !d_scratch) return EOQ_ERR_NULL_PTR;
     if (!have_device()) return EOQ_ERR_CUDA;
     const char *where = "eoq_b200_gated_packed";
-    GatedCall c = {pair_of(w), {w->gate_bias, w->up_bias}, x, h, batch, dtype, w->activation, kept_of(kept)};
+    GatedCall c = {pair_of(w), {w->gate_bias, w->up_bias}, x, h, batch, dtype, w->activation, w->bias_dtype, kept_of(kept)};
     Carve scratch{static_cast<uint8_t *>(d_scratch)};
     const size_t n = values(batch, w->rows);
     int e = 0;
@@ -132,7 +132,8 @@ extern "C" eoq_error_t eoq_b200_gated_packed(const eoq_b200_gated_t *w, const vo
         if (e == 0) e = launch_gated_product(c, half, factor, parts, stream);
         return launched(e, where);
     }
-    if (exact_products(c.w, dtype, w->gate, d_scratch) && exact_products(c.w, dtype, w->up, d_scratch)) {
+    const bool bf_bias = w->bias_dtype == EOQ_B200_BF16 && (w->gate_bias || w->up_bias);       // (that kernel has fp32 and fp16 biases)
+    if (!bf_bias && exact_products(c.w, dtype, w->gate, d_scratch) && exact_products(c.w, dtype, w->up, d_scratch)) {
         void *planes = scratch.take<void>(values(batch, w->cols + 1) * 4);
         float *factors = reinterpret_cast<float *>(static_cast<uint8_t *>(planes) + values(batch, w->cols) * 4);
         float *out[2] = {static_cast<float *>(c.keep.v[0]), static_cast<float *>(c.keep.v[1])};
@@ -141,7 +142,7 @@ extern "C" eoq_error_t eoq_b200_gated_packed(const eoq_b200_gated_t *w, const vo
         for (int i = 0; i < 2 && e == 0; i++) {
             QmmCall q = {};
             q.packed = c.w.codes[i]; q.scales = c.w.scales[i]; q.bias = c.bias[i]; q.tok_scale = factors; q.x = planes; q.y = out[i];
-            q.N = w->rows; q.K = w->cols; q.M = batch; q.bits = w->bits; q.group = w->group; q.split_x = 1; q.y_dtype = EOQ_B200_F32;
+            q.N = w->rows; q.K = w->cols; q.M = batch; q.bits = w->bits; q.group = w->group; q.split_x = 1; q.bias_half = w->bias_dtype == EOQ_B200_F16; q.y_dtype = EOQ_B200_F32;
             e = launch_qmm(q, stream);
         }
         if (e != (int)cudaErrorNotSupported) {

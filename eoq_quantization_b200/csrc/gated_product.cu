@@ -50,7 +50,7 @@ constexpr uint32_t kThreads = (kWOut + 4) * 32, kTmem = 512, kOut = 8 * 2048 + 8
 
 struct ProductArgs {
     const uint16_t *scales[2];   // [N][groups] fp16
-    const float *bias[2];        // forward: [N] or null
+    const void *bias[2];         // forward: [N] of bias_dtype, or null
     const float *factor;         // [M] or null
     void *y;                     // [M][N] or, gradient, [M][K]
     Kept keep;                   // forward
@@ -61,7 +61,7 @@ struct ProductArgs {
     uint32_t nw, ns, nd;         // stages of packed weights and of operands, accumulators
     uint32_t at_x, at_out, at_bar;       // shared-memory offsets
     uint32_t inverse;            // group_of
-    int dtype, act;
+    int dtype, act, bias_dtype;
     long long limit;             // clock ticks a wait may take
 };
 
@@ -152,14 +152,14 @@ struct Patience {
 template <bool GRAD, int BITS>
 struct Piece {
     static constexpr uint32_t kBytes = GRAD ? 16u * BITS : BITS == 2 ? 64u : 128u;      // of one row
-    static constexpr uint32_t kAlong = GRAD ? 128u : kBytes * 8u / BITS;                 // along the products' axis
+    static constexpr uint32_t kAlong = GRAD ? 256u : kBytes * 8u / BITS;                 // along the products' axis
     static constexpr uint32_t kBlocks = kAlong / 64u;
-    static constexpr uint32_t kStage = kRows * kBytes;
+    static constexpr uint32_t kStage = (GRAD ? kAlong : kRows) * kBytes;
 };
 
 // barriers, eight bytes each.  Of a pair's first CTA both use Full (its products' warp waits for both CTAs' operands) and OutEmpty.
 enum { bWFull = 0, bWEmpty = 8, bFull = 16, bEmpty = 24, bOutFull = 32, bOutEmpty = 34, bTmem = 36, bDrain = 37, bMark = 38, bUsedW = 39, bTicket = 40, bEnd = 41 };
-constexpr uint32_t kScales = 8u * kRows * 2u;      // of a stage of codes: forward, up to 8 groups x 128 rows; gradient, up to 4 groups x 128
+constexpr uint32_t kScales = 8u * kRows * 2u;      // of a stage of codes: forward, up to 8 groups x 128 rows; gradient, up to 4 groups x 256
 
 __device__ __forceinline__ void ldmatrix_trans(uint32_t addr, uint32_t (&r)[4])
 {
@@ -307,7 +307,7 @@ gated_product_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap gm
                         uint32_t sp[8];
 #pragma unroll
                         for (uint32_t b = 0; b < 8; b++)
-                            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(sp[b]) : "r"(scales_at + ws * kScales + gl * (kRows * 2u) + turn * 128u + b * 16u + (lane & 3u) * 4u));
+                            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(sp[b]) : "r"(scales_at + ws * kScales + gl * (P::kAlong * 2u) + turn * 128u + b * 16u + (lane & 3u) * 4u));
                         uint32_t m[kChunks][2][4];
 #pragma unroll
                         for (uint32_t c = 0; c < kChunks; c++)
@@ -432,11 +432,10 @@ gated_product_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap gm
             }
         }
     } else if (warp == kWScales) {
-        // ---- scales of a piece, [group][row], fetched some pieces ahead (one at a time, their latency is what bounds the launch).  Gradient: zero
-        // past the last weight row, so that what lies behind it (there the activations are zeros) cannot be an infinity.
+        // ---- scales of a piece, [group][row], a piece ahead of the stage they wait for.  Gradient: zero past the last weight row, so that what lies behind it (there the activations are zeros) cannot be an infinity.
         constexpr uint32_t kGroups = GRAD ? 4u : 8u;
-        constexpr int kAhead = GRAD ? 2 : 1;
-        struct Fetched { uint16_t v[4][kGroups]; uint32_t ng; };
+        constexpr uint32_t kEach = (GRAD ? P::kAlong : kRows) / 32u;              // rows a lane
+        struct Fetched { uint16_t v[kEach][kGroups]; uint32_t ng; };
         struct { uint64_t at; uint32_t p, p1, row0; } c = {run0, 0u, 0u, 0u};       // what is to be fetched next
         auto fetch = [&](Fetched &f) {
             f.ng = 0u;
@@ -453,7 +452,7 @@ gated_product_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap gm
                 const uint16_t *from = (which ? a.scales[1] : a.scales[0]) + g_first;
                 const uint32_t ng = group_of(min(c.row0 + 127u, a.K - 1u)) - g_first + 1u;
 #pragma unroll
-                for (uint32_t j = 0; j < 4; j++) {
+                for (uint32_t j = 0; j < kEach; j++) {
                     const uint32_t n = n0 + j * 32u + lane;
 #pragma unroll
                     for (uint32_t g = 0; g < kGroups; g++) f.v[j][g] = g < ng && n < a.N ? __ldg(from + (size_t)n * a.groups + g) : (uint16_t)0;
@@ -463,32 +462,25 @@ gated_product_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap gm
                 const uint32_t g0 = group_of(p * P::kAlong);
                 f.ng = group_of(min((p + 1u) * P::kAlong, a.K) - 1u) - g0 + 1u;
 #pragma unroll
-                for (uint32_t j = 0; j < 4; j++) {
+                for (uint32_t j = 0; j < kEach; j++) {
                     const uint16_t *from = a.scales[j >> 1] + (size_t)min(c.row0 + lane + 32u * (j & 1u), a.N - 1u) * a.groups + g0;
 #pragma unroll
                     for (uint32_t g = 0; g < kGroups; g++) if (g < f.ng) f.v[j][g] = __ldg(from + g);
                 }
             }
         };
-        Fetched f[kAhead];
+        Fetched f;
+        fetch(f);
+        for (Ring wr; f.ng; wr.next(a.nw)) {
+            wait(bar(bWEmpty + wr.at), wr.lap ^ 1u);
 #pragma unroll
-        for (int d = 0; d < kAhead; d++) fetch(f[d]);
-        Ring wr;
-        for (bool more = true; more;) {
+            for (uint32_t j = 0; j < kEach; j++)
 #pragma unroll
-            for (int d = 0; d < kAhead; d++) {
-                if (!f[d].ng) { more = false; break; }
-                wait(bar(bWEmpty + wr.at), wr.lap ^ 1u);
-#pragma unroll
-                for (uint32_t j = 0; j < 4; j++)
-#pragma unroll
-                    for (uint32_t g = 0; g < kGroups; g++)
-                        if (g < f[d].ng) asm volatile("st.shared.u16 [%0], %1;" ::"r"(scales_at + wr.at * kScales + g * (kRows * 2u) + j * 64u + lane * 2u), "h"(f[d].v[j][g]) : "memory");
-                __syncwarp();
-                bar_arrive_if(bar(bWFull + wr.at), lane == 0 && !wait.lost);
-                wr.next(a.nw);
-                fetch(f[d]);
-            }
+                for (uint32_t g = 0; g < kGroups; g++)
+                    if (g < f.ng) asm volatile("st.shared.u16 [%0], %1;" ::"r"(scales_at + wr.at * kScales + g * (kEach * 64u) + j * 64u + lane * 2u), "h"(f.v[j][g]) : "memory");
+            __syncwarp();
+            bar_arrive_if(bar(bWFull + wr.at), lane == 0 && !wait.lost);
+            fetch(f);
         }
     } else {
         // ---- the way out.  A lane keeps its row: of 32 tokens at a time, a warp of the gate's rows hands the later sixteen to the warp that has the same
@@ -535,7 +527,7 @@ gated_product_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap gm
             } else {
                 const uint32_t n = row0 + (q & 1u) * 32u + lane;
                 const bool there = n < a.N;
-                const float bg = there && a.bias[0] ? __ldg(a.bias[0] + n) : 0.0f, bu = there && a.bias[1] ? __ldg(a.bias[1] + n) : 0.0f;
+                const float bg = there ? bias_at(a.bias[0], n, a.bias_dtype) : 0.0f, bu = there ? bias_at(a.bias[1], n, a.bias_dtype) : 0.0f;
                 for (uint32_t t0 = 0; t0 < a.T; t0 += 32u, turn ^= 1u) {
                     float g[16], u[16];
                     const bool two = t0 + 16u < a.T;             // else the later sixteen do not exist
@@ -770,7 +762,7 @@ int run(ProductArgs a, const PackedPair &w, int nw, const void *x, uint32_t pitc
     CUtensorMap maps[2], xmap;
     constexpr CUtensorMapSwizzle sw = P::kBytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : P::kBytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B;
     for (int i = 0; i < 2; i++)
-        if (!map_2d(maps[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, w.codes[i], w.row_bytes, w.N, w.row_bytes, P::kBytes, GRAD ? kRows : kRows / 2, sw)) return (int)cudaErrorNotSupported;
+        if (!map_2d(maps[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, w.codes[i], w.row_bytes, w.N, w.row_bytes, P::kBytes, GRAD ? P::kAlong : kRows / 2, sw)) return (int)cudaErrorNotSupported;
     if (!map_2d(xmap, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, x, GRAD ? w.N : w.K, (uint64_t)a.M * (GRAD ? nw : 1), (uint64_t)pitch * 2, 64, p.T / 2u, CU_TENSOR_MAP_SWIZZLE_128B))
         return (int)cudaErrorNotSupported;
     cudaLaunchConfig_t cfg = {};
@@ -826,6 +818,7 @@ int launch_gated_product(const GatedCall &c, const uint16_t *x, const float *fac
     a.bias[0] = c.bias[0]; a.bias[1] = c.bias[1];
     a.keep = c.keep;
     a.act = c.act;
+    a.bias_dtype = c.bias_dtype;
     cudaStream_t st = (cudaStream_t)stream;
     if (c.w.bits == 4) return run<false, 4>(a, c.w, 2, x, c.w.K, scratch, st);
     if (c.w.bits == 2) return run<false, 2>(a, c.w, 2, x, c.w.K, scratch, st);

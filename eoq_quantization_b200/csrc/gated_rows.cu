@@ -49,13 +49,13 @@ __device__ __forceinline__ void pin(uint32_t &w, uint32_t &x, uint32_t &s) { asm
 
 struct RowsArgs {
     const uint16_t *scales[2];
-    const float *bias[2];
+    const void *bias[2];
     const void *x;
     void *h;
     void *kept[2];               // [batch][N] of x's type, fp32 (kept32), or null
     uint32_t N, K, group, batch, per, more;      // tiles a CTA takes, and how many CTAs take one more
     uint32_t most, pitch, slots; // tiles at a time, words that a row's scales take in shared memory, chunks of a warp's ring
-    int act, kept32;
+    int act, kept32, bias_dtype;
     long long limit;             // clock ticks a wait may take
     uint32_t *status;            // set when one runs out
 };
@@ -310,8 +310,8 @@ __global__ void __launch_bounds__(most_threads(BT), 1) gated_rows_kernel(const R
                 }
                 from = to;
             }
-            if (a.bias[0]) gs += __ldg(a.bias[0] + feature);
-            if (a.bias[1]) us += __ldg(a.bias[1] + feature);
+            gs += bias_at(a.bias[0], feature, a.bias_dtype);
+            us += bias_at(a.bias[1], feature, a.bias_dtype);
             if (stopped) gs = us = __uint_as_float(0x7fffffffu);
             const size_t at = (size_t)b * a.N + feature;
             auto put = [&](void *to, float value) {
@@ -351,13 +351,13 @@ constexpr uint32_t kManyWarps = 20, kStagers = 4;
 
 struct ManyArgs {
     const uint16_t *scales[2];
-    const float *bias[2];
+    const void *bias[2];
     const void *x;
     void *h;
     void *kept[2];
     uint32_t N, K, group, batch, per, more;      // tiles a CTA takes, and how many CTAs take one more
     uint32_t most, split, slice, pitch;          // tiles at a time, warps of a tile, chunks of a slice, words of a row's scales
-    int act, kept32;
+    int act, kept32, bias_dtype;
     long long limit;
     uint32_t *status;
 };
@@ -583,8 +583,8 @@ gated_many_rows_kernel(const ManyArgs a, const __grid_constant__ CUtensorMap gma
                     gs += from[f * (8 * NT) + b];
                     us += from[(8 + f) * (8 * NT) + b];
                 }
-                if (a.bias[0]) gs += __ldg(a.bias[0] + feature);
-                if (a.bias[1]) us += __ldg(a.bias[1] + feature);
+                gs += bias_at(a.bias[0], feature, a.bias_dtype);
+                us += bias_at(a.bias[1], feature, a.bias_dtype);
                 if (stopped) gs = us = __uint_as_float(0x7fffffffu);
                 const size_t at = (size_t)b * a.N + feature;
                 auto put = [&](void *to, float value) {
@@ -705,7 +705,7 @@ static int launch_many_rows(const GatedCall &c, void *stream)
     const ManyRoom room = many_room(c.w, c.M);
     ManyArgs a = {};
     for (int i = 0; i < 2; i++) { a.scales[i] = c.w.scales[i]; a.bias[i] = c.bias[i]; a.kept[i] = c.keep.v[i]; }
-    a.x = c.x; a.h = c.h; a.N = c.w.N; a.K = c.w.K; a.group = c.w.group; a.batch = c.M; a.act = c.act; a.kept32 = c.keep.form == kKeepF32;
+    a.x = c.x; a.h = c.h; a.N = c.w.N; a.K = c.w.K; a.group = c.w.group; a.batch = c.M; a.act = c.act; a.kept32 = c.keep.form == kKeepF32; a.bias_dtype = c.bias_dtype;
     a.limit = gated_wait_limit();
     a.status = gated_status_word();
     if (!a.status) return (int)cudaErrorInvalidDevice;
@@ -742,7 +742,7 @@ int launch_gated_rows(const GatedCall &c, void *stream)
     if (c.M > 8) return launch_many_rows(c, stream);
     RowsArgs a = {};
     for (int i = 0; i < 2; i++) { a.scales[i] = c.w.scales[i]; a.bias[i] = c.bias[i]; a.kept[i] = c.keep.v[i]; }
-    a.x = c.x; a.h = c.h; a.N = c.w.N; a.K = c.w.K; a.group = c.w.group; a.batch = c.M; a.act = c.act; a.kept32 = c.keep.form == kKeepF32;
+    a.x = c.x; a.h = c.h; a.N = c.w.N; a.K = c.w.K; a.group = c.w.group; a.batch = c.M; a.act = c.act; a.kept32 = c.keep.form == kKeepF32; a.bias_dtype = c.bias_dtype;
     a.limit = gated_wait_limit();
     a.status = gated_status_word();
     if (!a.status) return (int)cudaErrorInvalidDevice;

@@ -164,10 +164,10 @@ struct Parameter {
 // `bias` (None or a vector of N values beside x) as the kernels take it, fp32; false if it is anything else.
 struct Bias {
     const float *p = nullptr;
-    bool open(PyObject *o, const Tensor &x, int64_t N)
+    bool open(PyObject *o, const Tensor &x, int64_t N, at::ScalarType type = at::kFloat)
     {
         if (o == Py_None) return true;
-        if (!tensor_of(o) || kind_of(*tensor_of(o)) != kPlain || !value.open(o, x, at::kFloat) || value.t->numel() != N) return false;
+        if (!tensor_of(o) || kind_of(*tensor_of(o)) != kPlain || !value.open(o, x, type) || value.t->numel() != N) return false;
         p = static_cast<const float *>(value.t->data_ptr());
         return true;
     }
@@ -454,13 +454,17 @@ PyObject *gated_packed(PyObject *, PyObject *const *a, Py_ssize_t n)
     Activations act;
     Packed gate, up;
     Bias bias[2];
-    if (!act.open(a[8], K) || !gate.open(a[0], a[1], *act.x, N, K, bits, group) || !up.open(a[2], a[3], *act.x, N, K, bits, group) ||
-        !bias[0].open(a[9], *act.x, N) || !bias[1].open(a[10], *act.x, N))
+    // biases as they are where both have the activations' 16-bit type, else in fp32
+    auto of_x = [&](PyObject *o) { return o == Py_None || (tensor_of(o) && tensor_of(o)->scalar_type() == act.x->scalar_type()); };
+    const bool opened = act.open(a[8], K);
+    const at::ScalarType bias_type = opened && act.code != EOQ_B200_F32 && of_x(a[9]) && of_x(a[10]) ? act.x->scalar_type() : at::kFloat;
+    if (!opened || !gate.open(a[0], a[1], *act.x, N, K, bits, group) || !up.open(a[2], a[3], *act.x, N, K, bits, group) ||
+        !bias[0].open(a[9], *act.x, N, bias_type) || !bias[1].open(a[10], *act.x, N, bias_type))
         Py_RETURN_NONE;
     const Tensor &x = *act.x;
     const Ordered ordered(gate.converted || up.converted);
     const eoq_b200_gated_t w = {gate.codes, up.codes, gate.scales, up.scales, bias[0].p, bias[1].p, (uint32_t)N, (uint32_t)K, (uint32_t)bits, (uint32_t)group,
-                                (int)PyLong_AsLong(a[11])};
+                                (int)PyLong_AsLong(a[11]), dtype_code(bias_type)};
     if (PyErr_Occurred()) return nullptr;
     KeptTensors kept(form, x, act.rows, N);
     Tensor h = result(x, N, x.scalar_type()), scratch;
@@ -504,7 +508,7 @@ PyObject *gated_grad(PyObject *, PyObject *const *a, Py_ssize_t n)
     }
     const Ordered ordered(gate.converted || up.converted);
     const eoq_b200_gated_t w = {gate.codes, up.codes, gate.scales, up.scales, nullptr, nullptr, (uint32_t)N, (uint32_t)K, (uint32_t)bits, (uint32_t)group,
-                                (int)PyLong_AsLong(a[8])};
+                                (int)PyLong_AsLong(a[8]), EOQ_B200_F32};
     const bool want[3] = {PyObject_IsTrue(a[14]) == 1, PyObject_IsTrue(a[15]) == 1, PyObject_IsTrue(a[16]) == 1};
     if (PyErr_Occurred()) return nullptr;
     Tensor scratch = bytes_beside(dh, eoq_b200_gated_grad_scratch(&w, &kept, act.code, (uint32_t)act.rows)), out[3];

@@ -47,6 +47,10 @@ def _check_activations(x: torch.Tensor, cols: int, what: str) -> None:
         raise TypeError(f"{what}: unsupported activation dtype {x.dtype}")
 
 
+class _Unsupported(RuntimeError):
+    pass
+
+
 class _Gated(torch.autograd.Function):
     """h, and from what the forward pass kept of gate and up the gradients of x and the biases."""
 
@@ -54,7 +58,7 @@ class _Gated(torch.autograd.Function):
     def forward(ctx, x, gate_bias, up_bias, gate, gate_scales, up, up_scales, shape, activation, form):
         out = _lib.native().gated_packed(gate, gate_scales, up, up_scales, *shape, x, gate_bias, up_bias, activation, form)
         if out is None:
-            raise RuntimeError("gated_packed: the call is not supported")
+            raise _Unsupported("gated_packed: the call is not supported")
         ctx.shape, ctx.activation, ctx.form, ctx.x_shape = shape, activation, form, x.shape
         ctx.bias_dtypes = [None if b is None else b.dtype for b in (gate_bias, up_bias)]
         ctx.save_for_backward(gate, gate_scales, up, up_scales, *out[1:])
@@ -110,6 +114,12 @@ def gated_packed(gate: torch.Tensor, gate_scales: torch.Tensor, up: torch.Tensor
         h = _lib.native().gated_packed(gate, gate_scales, up, up_scales, rows, cols, bits, group, x, gate_bias, up_bias, code, 0)
         if h is not None:
             return h
+        # training: the checks below are for what this does not take
+        if call_kind(x, gate_bias, up_bias) == GRADIENT and not torch.is_autocast_enabled("cuda") and not gate_scales.requires_grad and not up_scales.requires_grad:
+            try:
+                return _Gated.apply(x, gate_bias, up_bias, gate, gate_scales, up, up_scales, (rows, cols, bits, group), code, KEEP[saved])
+            except _Unsupported:
+                pass
     what = "gated_packed"
     if code is None:
         raise ValueError(f"{what}: unknown activation {activation!r}; one of {', '.join(ACTIVATIONS)}")

@@ -530,13 +530,13 @@ eoq_error_t eoq_b200_gemv_polar_codes(const uint8_t *d_codes, const uint16_t *d_
  *   h = act(x Wg^T + bg) * (x Wu^T + bu),
  * with its backward pass.  Both weights as QuantizedLinear packs them (core/quantized_linear.py:49-66; 2 and 4 bits packed low
  * bits first, any other width one signed code per byte), rows x cols each, scales in fp16 over the flattened matrix; biases
- * NULL or fp32 [rows].  Device pointers. */
+ * NULL or [rows] of bias_dtype (EOQ_B200_F16 / BF16 / F32).  Device pointers. */
 typedef struct eoq_b200_gated {
     const uint8_t *gate, *up;
     const uint16_t *gate_scales, *up_scales;
-    const float *gate_bias, *up_bias;
+    const void *gate_bias, *up_bias;
     uint32_t rows, cols, bits, group;
-    int activation;
+    int activation, bias_dtype;
 } eoq_b200_gated_t;
 
 #define EOQ_B200_SILU      0

@@ -13,7 +13,7 @@ P = 0x1000                                     # an address that nothing reads: 
 
 
 def _gated(**kw):
-    w = L.Gated(P, P, P, P, None, None, 64, 128, 4, 128, 0)
+    w = L.Gated(P, P, P, P, None, None, 64, 128, 4, 128, 0, L.F32)
     for k, v in kw.items():
         setattr(w, k, v)
     return w
@@ -22,7 +22,7 @@ def _gated(**kw):
 @pytest.mark.parametrize("weight,dtype,batch,kept,code", [
     (dict(gate=None), 0, 1, None, NULL_PTR), (dict(up=None), 0, 1, None, NULL_PTR), (dict(gate_scales=None), 0, 1, None, NULL_PTR),
     (dict(up_scales=None), 0, 1, None, NULL_PTR), (dict(), 3, 1, None, UNSUPPORTED), (dict(), -1, 1, None, UNSUPPORTED),
-    (dict(activation=3), 0, 1, None, UNSUPPORTED), (dict(activation=-1), 0, 1, None, UNSUPPORTED), (dict(bits=1), 0, 1, None, INVALID),
+    (dict(activation=3), 0, 1, None, UNSUPPORTED), (dict(bias_dtype=3), 0, 1, None, UNSUPPORTED), (dict(activation=-1), 0, 1, None, UNSUPPORTED), (dict(bits=1), 0, 1, None, INVALID),
     (dict(bits=9), 0, 1, None, INVALID), (dict(group=0), 0, 1, None, INVALID), (dict(cols=0), 0, 1, None, INVALID),
     (dict(), 0, 1, L.Kept(3, P, P, P, P), UNSUPPORTED), (dict(), 0, 1, L.Kept(1, None, P, None, None), NULL_PTR),
     (dict(), 0, 1, L.Kept(2, P, P, P, None), NULL_PTR), (dict(), 0, 0, None, 0), (dict(rows=0), 0, 1, None, 0)])
