@@ -55,22 +55,21 @@ __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((u
 // (Markstein's step), so that quotients halfway between two codes, which 16-bit values often have, come out as such and go to
 // the even one.
 struct Storer {
-    float scale, most, inv;
+    float scale, most, inv, up;
     __device__ __forceinline__ explicit Storer(uint32_t bits)
     {
-        most = __uint_as_float(bits);
-        const bool fine = bits < 0x7f800000u, zero = most < 1e-30f;
-        scale = !fine ? __uint_as_float(0x7fffffffu) : zero ? 0.0f : __fdiv_rn(most, 127.0f);
+        const float v = __uint_as_float(bits);
+        const bool fine = bits < 0x7f800000u, zero = v < 1e-30f;
+        scale = !fine ? __uint_as_float(0x7fffffffu) : zero ? 0.0f : __fdiv_rn(v, 127.0f);
+        // in 128ths where 127 v or the products would leave the range; a factor of zero makes every code zero
+        up = !fine || zero ? 0.0f : v > 1e36f ? 0.9921875f : 127.0f;
+        most = !fine || zero ? 0.0f : v > 1e36f ? v * 0.0078125f : v;
         inv = !fine || zero ? 0.0f : __fdiv_rn(1.0f, most);
-        if (!fine || zero) most = 0.0f;
     }
-    __device__ __forceinline__ int8_t code(float v) const
+    __device__ __forceinline__ int code(float v) const
     {
-        if (inv == 0.0f) return 0;
-        // (1e-30 and more; above 2^120 in 128ths, so that neither 127 v nor the products leave the range)
-        const float f = most > 1e36f ? 0.0078125f : 1.0f, w = 127.0f * (v * f), q = w * inv, p = most * f;
-        const float t = f == 1.0f ? q : q * 128.0f;
-        return (int8_t)__float2int_rn(fmaf(fmaf(-t, p, w), f == 1.0f ? inv : inv * 128.0f, t));
+        const float w = up == 0.0f ? 0.0f : v * up, t = w * inv;
+        return __float2int_rn(fmaf(fmaf(-t, most, w), inv, t));
     }
 };
 

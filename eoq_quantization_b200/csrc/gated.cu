@@ -539,7 +539,7 @@ __global__ void __launch_bounds__(256) store_8bit_kernel(const void *__restrict_
             *reinterpret_cast<uint2 *>(codes + m * N + first + lane8 * 8u) = make_uint2(p[0], p[1]);
         } else {
 #pragma unroll
-            for (uint32_t j = 0; j < 8; j++) if (first + j * 8u + lane8 < N) codes[m * N + first + j * 8u + lane8] = to.code(v[j]);
+            for (uint32_t j = 0; j < 8; j++) if (first + j * 8u + lane8 < N) codes[m * N + first + j * 8u + lane8] = (int8_t)to.code(v[j]);
         }
     }
 }

@@ -87,17 +87,33 @@ __device__ __forceinline__ void tma_2d_pair(uint32_t dst, const CUtensorMap *map
     asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
                  ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar) : "memory");
 }
-__device__ __forceinline__ void mma_pair(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate)
+// The four products (K = 16 each) of a block, and `done` of both CTAs told when they are: one election for all five, for it is this warp's issue
+// that bounds a block of few tokens (one each: 350 clocks a block).
+__device__ __forceinline__ void mma_block(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate, uint32_t done)
 {
-    asm volatile("{\n\t.reg .pred e, p;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-                 "@e tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-                 ::"r"(d), "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+    asm volatile("{\n\t.reg .pred e, p;\n\t.reg .b32 a1, a2, a3;\n\t.reg .b64 b1, b2, b3;\n\t"
+                 "setp.ne.u32 p, %4, 0;\n\tadd.u32 a1, %1, 8;\n\tadd.u32 a2, %1, 16;\n\tadd.u32 a3, %1, 24;\n\t"
+                 "add.u64 b1, %2, 2;\n\tadd.u64 b2, %2, 4;\n\tadd.u64 b3, %2, 6;\n\telect.sync _|e, 0xffffffff;\n\t"
+                 "@e tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+                 "@e tcgen05.mma.cta_group::2.kind::f16 [%0], [a1], b1, %3, 1;\n\t"
+                 "@e tcgen05.mma.cta_group::2.kind::f16 [%0], [a2], b2, %3, 1;\n\t"
+                 "@e tcgen05.mma.cta_group::2.kind::f16 [%0], [a3], b3, %3, 1;\n\t"
+                 "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%5], %6;\n\t}"
+                 ::"r"(d), "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(done), "h"((uint16_t)3) : "memory");
 }
 // arrives at this barrier of both CTAs when the products so far are done
 __device__ __forceinline__ void commit_pair(uint32_t bar)
 {
     asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
                  "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(bar), "h"((uint16_t)3) : "memory");
+}
+
+// Whether a phase is over, without waiting (a try_wait, whose answer may take until it is, would keep the warp).
+__device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity)
+{
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
 }
 
 // A wait that may sleep for a millisecond: warps that ask again and again take the issue slots of those that work.
@@ -362,6 +378,7 @@ gated_product_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap gm
             const uint32_t idesc = (1u << 4) | ((a.T >> 3) << 17) | ((2u * kRows >> 4) << 24);
             const uint64_t desc0 = sw128_desc(base + a.at_x);
             Ring ar, dr;
+            bool ready = false;
             for (uint64_t at = run0; at < run1; dr.next(a.nd)) {
                 const Part s = part_at(at);
                 at += s.p1 - s.p0;
@@ -369,15 +386,14 @@ gated_product_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap gm
                 wait(bar(bOutEmpty + dr.at), dr.lap ^ 1u);
                 fence_after();
                 for (uint32_t i = 0; i < s.blocks; i++) {
-                    wait(bar(bFull + ar.at), ar.lap);
+                    if (!ready) wait(bar(bFull + ar.at), ar.lap);
                     fence_after();
-                    const uint32_t from = tmem + a_base + ar.at * 32u;
-                    const uint64_t desc = desc0 + ((ar.at * xstage) >> 4);
+                    Ring nr = ar;
+                    nr.next(a.ns);
+                    ready = bar_test(bar(bFull + nr.at), nr.lap);         // asked for while this block's products are being issued
                     // (past the last column of a forward product the codes are the copy's zeros, times a scale, and the activations zeros)
-#pragma unroll
-                    for (uint32_t j = 0; j < 4; j++) mma_pair(d, from + j * 8u, desc + j * 2u, idesc, i + j != 0);
-                    commit_pair(bar(bEmpty + ar.at));
-                    ar.next(a.ns);
+                    mma_block(d, tmem + a_base + ar.at * 32u, desc0 + ((ar.at * xstage) >> 4), idesc, i, bar(bEmpty + ar.at));
+                    ar = nr;
                 }
                 commit_pair(bar(bOutFull + dr.at));
             }
@@ -593,8 +609,8 @@ gated_product_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap gm
                             const Storer sg(max(mg, eg)), su(max(mu, eu));
                             const size_t m = tok0 + t + j, at = m * a.N + n, block = m * ((a.N + kStoreBlock - 1) / kStoreBlock) + row0 / 64u;
                             if (there) {
-                                reinterpret_cast<int8_t *>(a.keep.v[0])[at] = sg.code(g[j]);
-                                reinterpret_cast<int8_t *>(a.keep.v[1])[at] = su.code(u[j]);
+                                reinterpret_cast<int8_t *>(a.keep.v[0])[at] = (int8_t)sg.code(g[j]);
+                                reinterpret_cast<int8_t *>(a.keep.v[1])[at] = (int8_t)su.code(u[j]);
                             }
                             if ((q & 1u) == 0 && lane == 0 && there) { a.keep.scale[0][block] = sg.scale; a.keep.scale[1][block] = su.scale; }
                         }
@@ -647,13 +663,16 @@ gated_product_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap gm
 #pragma unroll
                 for (int j = 0; j < 16; j++) v[j] = 0.0f;
                 if (t >= a.T) return;
-                for (uint32_t p = p_first; p <= p_last; p++) {       // a part's all requested before the first is added
-                    const float *part = partial_of(p, run_start(p) <= first) + (size_t)t * kRows;
-                    float o[16];
+                for (uint32_t p = p_first; p <= p_last; p += 2u) {   // two parts' requested before the first is added
+                    const bool two = p < p_last;
+                    const float *one = partial_of(p, run_start(p) <= first) + (size_t)t * kRows, *other = two ? partial_of(p + 1u, run_start(p + 1u) <= first) + (size_t)t * kRows : one;
+                    float o[16], q[16];
 #pragma unroll
-                    for (int j = 0; j < 16; j++) o[j] = __ldcg(part + j * kRows);
+                    for (int j = 0; j < 16; j++) o[j] = __ldcg(one + j * kRows);
 #pragma unroll
-                    for (int j = 0; j < 16; j++) v[j] += o[j];
+                    for (int j = 0; j < 16; j++) q[j] = __ldcg(other + j * kRows);
+#pragma unroll
+                    for (int j = 0; j < 16; j++) v[j] = v[j] + o[j] + (two ? q[j] : 0.0f);
                 }
             }, []() {});
         }
@@ -696,45 +715,45 @@ Layout lay_out(uint32_t T, uint32_t stage_w)
     return l;
 }
 
-// Tokens of a tile: as few tiles as pay.  A block of 64 costs its products (two clocks a token) or its producers' work (some 400), whichever is
-// longer; with one accumulator a tile's way out (some 100 clocks a token) comes on top.
-uint32_t tile_tokens(uint32_t M, uint32_t blocks)
-{
-    uint32_t best = 0;
-    double least = 1e30;
-    for (uint32_t n = (M + 255u) / 256u; n < (M + 255u) / 256u + 4u; n++) {
-        const uint32_t T = ((M + n - 1) / n + 15u) / 16u * 16u;
-        const double cost = (double)((M + T - 1) / T) * (blocks * std::max(400.0, 2.0 * T) + (T > 160u ? 100.0 * T : 0.0));
-        if (cost < 0.999 * least) { least = cost; best = T; }
-    }
-    return best;
-}
-
 struct Plan { uint32_t T, tok_tiles, tiles, per_tile, per_weight, pairs; };
 
+// Tokens of a tile, and pairs of CTAs.  In clocks, as measured: a block of 64 takes its products (two a token) or what the products' warp and the
+// producers take at least (some 430), whichever is longer; with one accumulator a tile's way out (70 a token) comes on top, else only the last one's;
+// and a tile that several pairs share costs their sums' way through scratch, 150 a token and part.
 template <bool GRAD, int BITS>
 Plan plan_for(uint32_t N, uint32_t K, uint32_t M, int nw)
 {
     using P = Piece<GRAD, BITS>;
-    Plan p = {};
-    p.per_weight = GRAD ? (N + P::kAlong - 1) / P::kAlong : 0u;
-    p.per_tile = GRAD ? p.per_weight * nw : (K + P::kAlong - 1) / P::kAlong;
-    p.T = tile_tokens(M, p.per_tile * P::kBlocks);
-    p.tok_tiles = (M + p.T - 1) / p.T;
-    p.tiles = ((GRAD ? K + 255u : N + 127u) / (GRAD ? 256u : 128u)) * p.tok_tiles;
-    // All the pairs there are, where tiles are that many; else as many to a tile as pay: a part more costs its sums' way through scratch.
-    const uint32_t room = (uint32_t)std::max(1, device_sm_count() / 2);
-    p.pairs = std::min(room, p.tiles);
-    if (p.tiles < room) {
-        double least = 1e30;
-        const double block = std::max(400.0, 2.0 * p.T);
-        for (uint32_t n = p.tiles; n <= room && n <= (uint64_t)p.tiles * p.per_tile; n++) {
-            const double parts = (double)n / p.tiles, pieces = std::ceil((double)p.tiles * p.per_tile / n);
-            const double cost = pieces * P::kBlocks * block + (n > p.tiles ? 4000.0 + std::ceil(p.T / 32.0) * 800.0 * (1.0 + std::ceil(parts)) : 0.0);
-            if (cost < 0.98 * least) { least = cost; p.pairs = n; }
+    Plan best = {};
+    best.per_weight = GRAD ? (N + P::kAlong - 1) / P::kAlong : 0u;
+    best.per_tile = GRAD ? best.per_weight * nw : (K + P::kAlong - 1) / P::kAlong;
+    const uint32_t room = (uint32_t)std::max(1, device_sm_count() / 2), across = (GRAD ? K + 255u : N + 127u) / (GRAD ? 256u : 128u);
+    double least = 1e30;
+    uint32_t last = 0;
+    for (uint32_t n = (M + 255u) / 256u; n < (M + 255u) / 256u * 2u + 3u; n++) {
+        Plan p = best;
+        p.T = ((M + n - 1) / n + 15u) / 16u * 16u;
+        if (p.T == last) continue;
+        last = p.T;
+        p.tok_tiles = (M + p.T - 1) / p.T;
+        p.tiles = across * p.tok_tiles;
+        const double block = std::max(430.0, 2.0 * p.T), out = 70.0 * p.T, each = p.T > 160u ? out : 0.0;
+        auto consider = [&](uint32_t pairs, double cost) {
+            if (cost >= 0.98 * least) return;
+            least = cost;
+            best = p;
+            best.pairs = pairs;
+        };
+        if (p.tiles >= room) {
+            consider(room, (double)p.tiles / room * (p.per_tile * P::kBlocks * block + each) + out + (p.tiles % room ? 300.0 * p.T : 0.0));
+            continue;
+        }
+        for (uint32_t pairs = p.tiles; pairs <= room && pairs <= (uint64_t)p.tiles * p.per_tile; pairs++) {
+            const double pieces = std::ceil((double)p.tiles * p.per_tile / pairs), parts = std::ceil((double)pairs / p.tiles);
+            consider(pairs, pieces * P::kBlocks * block + out + (pairs > p.tiles ? 4000.0 + 150.0 * p.T * (1.0 + parts) : 0.0));
         }
     }
-    return p;
+    return best;
 }
 
 template <bool GRAD>
