@@ -57,7 +57,7 @@ struct ProductArgs {
     float *partial;              // [pairs][2][2][T][128]: sums of tiles that a pair's run begins (0) or ends (1) in the middle of
     uint32_t *count;             // [tiles][2], zero: parts of a tile that have arrived
     uint32_t N, K, M, T, group, groups;
-    uint32_t tok_tiles, tiles, per_tile, per_weight;         // of the grid of tiles; pieces of a tile's axis, of one weight's
+    uint32_t tok_tiles, tiles, per_tile, per_weight, unit;         // of the grid of tiles; pieces of a tile's axis, of one weight's
     uint32_t nw, ns, nd;         // stages of packed weights and of operands, accumulators
     uint32_t at_x, at_out, at_bar;       // shared-memory offsets
     uint32_t inverse;            // group_of
@@ -239,9 +239,11 @@ gated_product_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap gm
     const uint32_t xstage = a.T * 64u, a_base = a.nd * a.T;          // half of a block's tokens; first column of A
     constexpr uint32_t kWide = GRAD ? 128u : 64u;                    // columns, or features, of a CTA's tile
 
-    // A pair's run of pieces, and its parts of tiles in order
-    auto run_start = [&](uint32_t p) { return (uint64_t)a.tiles * a.per_tile * p / pairs; };
-    const uint64_t run0 = run_start(pair), run1 = run_start(pair + 1);
+    // A pair's run of pieces, and its parts of tiles.  Where its run ends inside a tile, that part comes first: then the next pair, which has the rest of
+    // that tile and takes it up last but one run later, finds the other sums there and adds its own to them on the way out.  (In the run's order the sums of
+    // shared tiles were added up when nothing else was left to do: 68 of 255 thousand clocks for a 11008 x 4096 gradient of 2048 rows.)
+    auto run_start = [&](uint32_t p) { return (uint64_t)a.tiles * (a.per_tile / a.unit) * p / pairs * a.unit; };
+    const uint64_t run0 = run_start(pair), run1 = run_start(pair + 1), cut = run1 - run1 % a.per_tile, head = cut > run0 && cut < run1 ? cut : run0;
     struct Part { uint32_t tile, p0, p1, blocks; };                  // pieces [p0, p1) of a tile, in blocks of 64
     auto part_at = [&](uint64_t at) {
         Part s;
@@ -251,6 +253,11 @@ gated_product_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap gm
         // forward: the last piece's blocks past the last column are left out; gradient: rows past the last one are zeros
         s.blocks = (GRAD ? s.p1 * P::kBlocks : min(s.p1 * P::kBlocks, (a.K + 63u) / 64u)) - s.p0 * P::kBlocks;
         return s;
+    };
+    auto go_on = [&](uint64_t &at, uint64_t &left, const Part &s) {
+        left -= s.p1 - s.p0;
+        at += s.p1 - s.p0;
+        if (at == run1) at = run0;
     };
     // tokens fastest: the pairs that run at the same time share codes, which come from HBM, rather than activations, which the L2 holds
     auto first_row = [&](uint32_t tile) { return (tile / a.tok_tiles * 2u + rank) * kWide; };
@@ -288,9 +295,9 @@ gated_product_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap gm
         Ring wr, ar;
         for (uint32_t j = 0; j < set; j++) ar.next(a.ns);
         uint32_t turn = set;                   // blocks until this set's next one
-        for (uint64_t at = run0; at < run1;) {
+        for (uint64_t at = head, left = run1 - run0; left;) {
             const Part s = part_at(at);
-            at += s.p1 - s.p0;
+            go_on(at, left, s);
             const uint32_t row0 = first_row(s.tile);
             for (uint32_t p = s.p0; p < s.p1; p++, wr.next(a.nw)) {
                 static_assert(P::kBlocks <= kSets, "a set has one block of a piece, or none");
@@ -379,9 +386,9 @@ gated_product_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap gm
             const uint64_t desc0 = sw128_desc(base + a.at_x);
             Ring ar, dr;
             bool ready = false;
-            for (uint64_t at = run0; at < run1; dr.next(a.nd)) {
+            for (uint64_t at = head, left = run1 - run0; left; dr.next(a.nd)) {
                 const Part s = part_at(at);
-                at += s.p1 - s.p0;
+                go_on(at, left, s);
                 const uint32_t d = tmem + dr.at * a.T;
                 wait(bar(bOutEmpty + dr.at), dr.lap ^ 1u);
                 fence_after();
@@ -403,9 +410,9 @@ gated_product_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap gm
         const bool leader = elect();
         Ring wr;
         uint32_t used = 0;
-        for (uint64_t at = run0; at < run1;) {
+        for (uint64_t at = head, left = run1 - run0; left;) {
             const Part s = part_at(at);
-            at += s.p1 - s.p0;
+            go_on(at, left, s);
             for (uint32_t p = s.p0; p < s.p1; p++, wr.next(a.nw)) {
                 wait(bar(bWEmpty + wr.at), wr.lap ^ 1u);
                 if (leader && !wait.lost) {
@@ -432,9 +439,9 @@ gated_product_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap gm
         if (leader) word(bMark)[1] = 1u;
         const uint32_t full0 = in_cta(bar(bFull), 0u);
         Ring xr;
-        for (uint64_t at = run0; at < run1;) {
+        for (uint64_t at = head, left = run1 - run0; left;) {
             const Part s = part_at(at);
-            at += s.p1 - s.p0;
+            go_on(at, left, s);
             const uint32_t token = first_token(s.tile) + rank * (a.T / 2u);
             for (uint32_t i = 0; i < s.blocks; i++, xr.next(a.ns)) {
                 wait(bar(bEmpty + xr.at), xr.lap ^ 1u);
@@ -452,13 +459,13 @@ gated_product_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap gm
         constexpr uint32_t kGroups = GRAD ? 4u : 8u;
         constexpr uint32_t kEach = (GRAD ? P::kAlong : kRows) / 32u;              // rows a lane
         struct Fetched { uint16_t v[kEach][kGroups]; uint32_t ng; };
-        struct { uint64_t at; uint32_t p, p1, row0; } c = {run0, 0u, 0u, 0u};       // what is to be fetched next
+        struct { uint64_t at, left; uint32_t p, p1, row0; } c = {head, run1 - run0, 0u, 0u, 0u};       // what is to be fetched next
         auto fetch = [&](Fetched &f) {
             f.ng = 0u;
             if (c.p == c.p1) {
-                if (c.at >= run1) return;
+                if (!c.left) return;
                 const Part s = part_at(c.at);
-                c.at += s.p1 - s.p0;
+                go_on(c.at, c.left, s);
                 c.p = s.p0; c.p1 = s.p1;
                 c.row0 = first_row(s.tile);
             }
@@ -620,9 +627,9 @@ gated_product_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap gm
         };
         auto partial_of = [&](uint32_t p, uint32_t begins) { return a.partial + ((size_t)(p * 2u + begins) * 2u + rank) * a.T * kRows + q * 32u + lane; };
         Ring dr;
-        for (uint64_t at = run0; at < run1; dr.next(a.nd)) {
+        for (uint64_t at = head, left = run1 - run0; left; dr.next(a.nd)) {
             const Part s = part_at(at);
-            at += s.p1 - s.p0;
+            go_on(at, left, s);
             wait(bar(bOutFull + dr.at), dr.lap);
             __syncwarp();
             fence_after();
@@ -642,39 +649,48 @@ gated_product_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap gm
                 finish(s.tile, take, release);
                 continue;
             }
-            // the tile's other parts are other pairs': the last to arrive adds them up
-            float *mine = partial_of(pair, s.p0 == 0u);
-            for (uint32_t t0 = 0; t0 < a.T; t0 += 16u) {
-                float v[16];
-                take(t0, v);
-                if (t0 + 16u >= a.T) release();
-#pragma unroll
-                for (uint32_t j = 0; j < 16; j++) __stcg(mine + (size_t)(t0 + j) * kRows, v[j]);
-            }
+            // the tile's other parts are other pairs': the last to arrive adds them up, in the order of the pairs, its own (the same bits)
+            // from the accumulator where the others' are there already
             const uint64_t first = (uint64_t)s.tile * a.per_tile, total = (uint64_t)a.tiles * a.per_tile;
             const uint32_t p_first = (uint32_t)(((first + 1) * pairs - 1) / total), p_last = (uint32_t)(((first + a.per_tile) * pairs - 1) / total);
-            __threadfence();
-            asm volatile("bar.sync 5, 128;" ::: "memory");
-            if (tid == 0) *word(bTicket) = atomicAdd(a.count + s.tile * 2u + rank, 1u);
-            asm volatile("bar.sync 5, 128;" ::: "memory");
-            if (*word(bTicket) != p_last - p_first) continue;
+            uint32_t *count = a.count + s.tile * 2u + rank;
+            auto ask = [&](uint32_t add) {                       // parts that have arrived before this one
+                asm volatile("bar.sync 5, 128;" ::: "memory");
+                if (tid == 0) *word(bTicket) = add ? atomicAdd(count, 1u) : *reinterpret_cast<volatile uint32_t *>(count);
+                asm volatile("bar.sync 5, 128;" ::: "memory");
+                return *word(bTicket) == p_last - p_first;
+            };
+            const bool here = ask(0u);
+            if (!here) {
+                float *mine = partial_of(pair, s.p0 == 0u);
+                for (uint32_t t0 = 0; t0 < a.T; t0 += 16u) {
+                    float v[16];
+                    take(t0, v);
+                    if (t0 + 16u >= a.T) release();
+#pragma unroll
+                    for (uint32_t j = 0; j < 16; j++) __stcg(mine + (size_t)(t0 + j) * kRows, v[j]);
+                }
+                __threadfence();
+                if (!ask(1u)) continue;
+            }
             __threadfence();
             finish(s.tile, [&](uint32_t t, float (&v)[16]) {
+                float o[16];
 #pragma unroll
                 for (int j = 0; j < 16; j++) v[j] = 0.0f;
                 if (t >= a.T) return;
-                for (uint32_t p = p_first; p <= p_last; p += 2u) {   // two parts' requested before the first is added
-                    const bool two = p < p_last;
-                    const float *one = partial_of(p, run_start(p) <= first) + (size_t)t * kRows, *other = two ? partial_of(p + 1u, run_start(p + 1u) <= first) + (size_t)t * kRows : one;
-                    float o[16], q[16];
+                for (uint32_t p = p_first; p <= p_last; p++) {
+                    if (here && p == pair) {
+                        take(t, o);
+                    } else {
+                        const float *part = partial_of(p, run_start(p) <= first) + (size_t)t * kRows;
 #pragma unroll
-                    for (int j = 0; j < 16; j++) o[j] = __ldcg(one + j * kRows);
+                        for (int j = 0; j < 16; j++) o[j] = __ldcg(part + j * kRows);
+                    }
 #pragma unroll
-                    for (int j = 0; j < 16; j++) q[j] = __ldcg(other + j * kRows);
-#pragma unroll
-                    for (int j = 0; j < 16; j++) v[j] = v[j] + o[j] + (two ? q[j] : 0.0f);
+                    for (int j = 0; j < 16; j++) v[j] += o[j];
                 }
-            }, []() {});
+            }, [&]() { if (here) release(); });
         }
     }
     __syncwarp();
@@ -715,11 +731,15 @@ Layout lay_out(uint32_t T, uint32_t stage_w)
     return l;
 }
 
-struct Plan { uint32_t T, tok_tiles, tiles, per_tile, per_weight, pairs; };
+struct Plan { uint32_t T, tok_tiles, tiles, per_tile, per_weight, pairs, unit; };       // runs are whole numbers of `unit` pieces: 1, or a tile's
 
 // Tokens of a tile, and pairs of CTAs.  In clocks, as measured: a block of 64 takes its products (two a token) or what the products' warp and the
-// producers take at least (some 430), whichever is longer; with one accumulator a tile's way out (70 a token) comes on top, else only the last one's;
-// and a tile that several pairs share costs their sums' way through scratch, 150 a token and part.
+// producers take at least (some 430; gate and up of 8 bits, 600), whichever is longer; with one accumulator a tile's way out (70 a token) comes on top, else only the last one's.
+// Sums of shared tiles go through scratch: where pairs outnumber tiles 60 a token and part (11008 x 4096 gradient, us, tiles of 48, 112, 208 and 256
+// tokens in one part: 38.9, 41.7, 48.4, 58.4; in two: 26.1, 33.1, 47.5, 56.8; in four: 23.6, 35.4, 54.8, 65.5), and as much again where a run holds parts of
+// two tiles (16 tiles by 74 pairs: 26.8, 43.6, 71.3, 85.8); else 100 a token at the end, which runs of whole tiles spare (4096 x 2816 8-bit gated block,
+// 1024 rows, 128 tiles: 74 pairs 73.8, 64 pairs of two tiles 54.0).  More tiles of tokens unpack the codes more often, beside all this: they are taken
+// where they seem to save 15 per cent.
 template <bool GRAD, int BITS>
 Plan plan_for(uint32_t N, uint32_t K, uint32_t M, int nw)
 {
@@ -728,29 +748,33 @@ Plan plan_for(uint32_t N, uint32_t K, uint32_t M, int nw)
     best.per_weight = GRAD ? (N + P::kAlong - 1) / P::kAlong : 0u;
     best.per_tile = GRAD ? best.per_weight * nw : (K + P::kAlong - 1) / P::kAlong;
     const uint32_t room = (uint32_t)std::max(1, device_sm_count() / 2), across = (GRAD ? K + 255u : N + 127u) / (GRAD ? 256u : 128u);
-    double least = 1e30;
+    double least = 1e30, fewer = 1e30;           // of the plans so far, and of those with fewer tokens' tiles than this one's
     uint32_t last = 0;
     for (uint32_t n = (M + 255u) / 256u; n < (M + 255u) / 256u * 2u + 3u; n++) {
         Plan p = best;
         p.T = ((M + n - 1) / n + 15u) / 16u * 16u;
         if (p.T == last) continue;
         last = p.T;
+        fewer = least;
         p.tok_tiles = (M + p.T - 1) / p.T;
         p.tiles = across * p.tok_tiles;
-        const double block = std::max(430.0, 2.0 * p.T), out = 70.0 * p.T, each = p.T > 160u ? out : 0.0;
-        auto consider = [&](uint32_t pairs, double cost) {
-            if (cost >= 0.98 * least) return;
+        const double block = std::max(!GRAD && BITS == 8 ? 600.0 : 430.0, 2.0 * p.T), out = 70.0 * p.T, each = p.T > 160u ? out : 0.0;
+        auto consider = [&](uint32_t pairs, uint32_t unit, double cost) {
+            if (cost >= least || cost >= 0.85 * fewer) return;
             least = cost;
             best = p;
             best.pairs = pairs;
+            best.unit = unit;
         };
         if (p.tiles >= room) {
-            consider(room, (double)p.tiles / room * (p.per_tile * P::kBlocks * block + each) + out + (p.tiles % room ? 300.0 * p.T : 0.0));
+            const uint32_t rounds = (p.tiles + room - 1) / room;
+            consider((p.tiles + rounds - 1) / rounds, p.per_tile, rounds * (p.per_tile * P::kBlocks * block + each) - each + out);
+            if (p.tiles % room) consider(room, 1u, (double)p.tiles / room * (p.per_tile * P::kBlocks * block + each) + out + 100.0 * p.T);
             continue;
         }
         for (uint32_t pairs = p.tiles; pairs <= room && pairs <= (uint64_t)p.tiles * p.per_tile; pairs++) {
             const double pieces = std::ceil((double)p.tiles * p.per_tile / pairs), parts = std::ceil((double)pairs / p.tiles);
-            consider(pairs, pieces * P::kBlocks * block + out + (pairs > p.tiles ? 4000.0 + 150.0 * p.T * (1.0 + parts) : 0.0));
+            consider(pairs, pairs > p.tiles ? 1u : p.per_tile, pieces * P::kBlocks * block + out + (pairs > p.tiles ? 60.0 * p.T * (1.0 + parts + (pairs % p.tiles != 0)) : 0.0));
         }
     }
     return best;
@@ -774,7 +798,7 @@ int run(ProductArgs a, const PackedPair &w, int nw, const void *x, uint32_t pitc
     const Layout l = lay_out(p.T, P::kStage);
     const uint32_t at_once = resident_ctas(reinterpret_cast<const void *>(kern), kThreads, l.smem, 2) / 2u;
     if (!at_once) return (int)cudaErrorNotSupported;
-    a.T = p.T; a.tok_tiles = p.tok_tiles; a.tiles = p.tiles; a.per_tile = p.per_tile; a.per_weight = p.per_weight;
+    a.T = p.T; a.tok_tiles = p.tok_tiles; a.tiles = p.tiles; a.per_tile = p.per_tile; a.per_weight = p.per_weight; a.unit = p.unit;
     a.nw = l.nw; a.ns = l.ns; a.nd = l.nd; a.at_x = l.at_x; a.at_out = l.at_out; a.at_bar = l.at_bar;
     a.count = static_cast<uint32_t *>(scratch);
     a.partial = reinterpret_cast<float *>(static_cast<uint8_t *>(scratch) + count_bytes(p));
