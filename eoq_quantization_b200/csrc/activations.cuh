@@ -60,16 +60,19 @@ struct Storer {
     {
         const float v = __uint_as_float(bits);
         const bool fine = bits < 0x7f800000u, zero = v < 1e-30f;
-        scale = !fine ? __uint_as_float(0x7fffffffu) : zero ? 0.0f : __fdiv_rn(v, 127.0f);
+        // v / 127 by the reciprocal and one such step: the rounded quotient for all 2^23 significands (compared with a division's)
+        const float r = 1.0f / 127.0f, q = v * r;
+        scale = !fine ? __uint_as_float(0x7fffffffu) : zero ? 0.0f : fmaf(fmaf(-q, 127.0f, v), r, q);
         // in 128ths where 127 v or the products would leave the range; a factor of zero makes every code zero
         up = !fine || zero ? 0.0f : v > 1e36f ? 0.9921875f : 127.0f;
         most = !fine || zero ? 0.0f : v > 1e36f ? v * 0.0078125f : v;
-        inv = !fine || zero ? 0.0f : __fdiv_rn(1.0f, most);
+        inv = !fine || zero ? 0.0f : __fdividef(1.0f, most);       // (two units off at most, which the step makes good)
     }
-    __device__ __forceinline__ int code(float v) const
+    // in the low byte: beside 1.5 x 2^23 a whole number is all that a sum's rounding leaves (a conversion takes four times an addition's slots)
+    __device__ __forceinline__ uint32_t code(float v) const
     {
         const float w = up == 0.0f ? 0.0f : v * up, t = w * inv;
-        return __float2int_rn(fmaf(fmaf(-t, most, w), inv, t));
+        return __float_as_uint(fmaf(fmaf(-t, most, w), inv, t) + 12582912.0f);
     }
 };
 

@@ -488,15 +488,31 @@ __global__ void __launch_bounds__(256) rows_to_half_kernel(const void *__restric
                                                            float *__restrict__ factor, const Zeros zeros)
 {
     __shared__ float part[8];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     set_zeros(zeros);
     for (uint32_t m = blockIdx.x; m < M; m += gridDim.x) {
         float most = 0.0f;
-        for (uint32_t k = threadIdx.x; k < K; k += 256u) most = fmaxf(most, finite_magnitude(load_as_float(x, (size_t)m * K + k, dtype)));
+        for (uint32_t k0 = threadIdx.x; k0 < K; k0 += 8u * 256u) {       // eight requested together; past the row's end its last value again
+            float v[8];
+#pragma unroll
+            for (uint32_t j = 0; j < 8; j++) v[j] = load_as_float(x, (size_t)m * K + min(k0 + j * 256u, K - 1u), dtype);
+#pragma unroll
+            for (uint32_t j = 0; j < 8; j++) most = fmaxf(most, finite_magnitude(v[j]));
+        }
         const int e = half_exponent(largest_of(most, part));
         const float up = power_of_two(e);
         if (threadIdx.x == 0) factor[m] = power_of_two(-e);
-        for (uint32_t k = threadIdx.x; k < pitch; k += 256u)
-            out[(size_t)m * pitch + k] = __float2half_rn(k < K ? load_as_float(x, (size_t)m * K + k, dtype) * up : 0.0f);
+        for (uint32_t k0 = threadIdx.x; k0 < pitch; k0 += 8u * 256u) {
+            float v[8];
+#pragma unroll
+            for (uint32_t j = 0; j < 8; j++) v[j] = load_as_float(x, (size_t)m * K + min(k0 + j * 256u, K - 1u), dtype);
+#pragma unroll
+            for (uint32_t j = 0; j < 8; j++) {
+                const uint32_t k = k0 + j * 256u;
+                if (k < pitch) out[(size_t)m * pitch + k] = __float2half_rn(k < K ? v[j] * up : 0.0f);
+            }
+        }
     }
 }
 
@@ -508,17 +524,31 @@ __global__ void __launch_bounds__(256) rows_to_half_kernel(const void *__restric
 // ---------------------------------------------------------------------------
 // VEC: rows are multiples of eight values and 16-byte aligned, a lane's eight lie together; else they are eight apart.
 template <int DTYPE, bool VEC>
-__global__ void __launch_bounds__(256) store_8bit_kernel(const void *__restrict__ x, size_t blocks, uint32_t N, int8_t *__restrict__ codes, float *__restrict__ scales)
+__global__ void __launch_bounds__(256) store_8bit_kernel(const void *__restrict__ x, size_t M, uint32_t N, int8_t *__restrict__ codes, float *__restrict__ scales)
 {
     const uint32_t per_row = (N + kStoreBlock - 1) / kStoreBlock, lane8 = threadIdx.x & 7u;
-    for (size_t b0 = ((size_t)blockIdx.x * 256u + (threadIdx.x & ~31u)) / 8u; b0 < blocks; b0 += (size_t)gridDim.x * 32u) {
-        const size_t b = b0 + ((threadIdx.x & 31u) >> 3);
-        const bool here = b < blocks;
-        const size_t m = !here ? 0 : blocks <= 0xffffffffu ? (uint32_t)b / per_row : b / per_row;
-        const uint32_t first = here ? (uint32_t)(b - m * per_row) * kStoreBlock : N;
+    // a warp's turns: four blocks of one row, `fours` such to a row; on by `warps` of them without dividing again
+    const uint32_t fours = (per_row + 3u) / 4u, warps = gridDim.x * 8u, on_m = warps / fours, on_f = warps - on_m * fours;
+    const uint32_t t = blockIdx.x * 8u + (threadIdx.x >> 5);
+    size_t m = t / fours;
+    uint32_t f = t % fours;
+    auto first_of = [&](uint32_t f) { return (f * 4u + ((threadIdx.x & 31u) >> 3)) * kStoreBlock; };
+    auto fetch = [&](size_t m, uint32_t f) {
+        Raw8<DTYPE> raw = {};
+        if (VEC && m < M && first_of(f) + lane8 * 8u < N) raw = load8<DTYPE>(x, m * N + first_of(f) + lane8 * 8u);
+        return raw;
+    };
+    Raw8<DTYPE> raw = fetch(m, f);
+    while (m < M) {
+        // the next turn's values are on their way while this one's are made into codes
+        size_t nm = m + on_m;
+        uint32_t nf = f + on_f;
+        if (nf >= fours) { nf -= fours; nm++; }
+        const Raw8<DTYPE> soon = fetch(nm, nf);
+        const uint32_t first = first_of(f);
         float v[8] = {};
         if constexpr (VEC) {
-            if (first + lane8 * 8u < N) values_of<DTYPE>(load8<DTYPE>(x, m * N + first + lane8 * 8u), v);
+            values_of<DTYPE>(raw, v);
         } else {
 #pragma unroll
             for (uint32_t j = 0; j < 8; j++) if (first + j * 8u + lane8 < N) v[j] = load_as_float(x, m * N + first + j * 8u + lane8, DTYPE);
@@ -529,18 +559,20 @@ __global__ void __launch_bounds__(256) store_8bit_kernel(const void *__restrict_
 #pragma unroll
         for (int d = 4; d > 0; d >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
         const Storer to(most);
-        if (!here) continue;
-        if (lane8 == 0) scales[b] = to.scale;
+        if (first < N && lane8 == 0) scales[m * per_row + first / kStoreBlock] = to.scale;
         if constexpr (VEC) {
-            if (first + lane8 * 8u >= N) continue;
-            uint32_t p[2] = {0u, 0u};
+            if (first + lane8 * 8u < N) {
+                uint32_t p[2];
 #pragma unroll
-            for (int j = 0; j < 8; j++) p[j >> 2] |= (uint32_t)(uint8_t)to.code(v[j]) << (8 * (j & 3));
-            *reinterpret_cast<uint2 *>(codes + m * N + first + lane8 * 8u) = make_uint2(p[0], p[1]);
+                for (int j = 0; j < 2; j++)
+                    p[j] = __byte_perm(__byte_perm(to.code(v[4 * j]), to.code(v[4 * j + 1]), 0x0040), __byte_perm(to.code(v[4 * j + 2]), to.code(v[4 * j + 3]), 0x0040), 0x5410);
+                *reinterpret_cast<uint2 *>(codes + m * N + first + lane8 * 8u) = make_uint2(p[0], p[1]);
+            }
         } else {
 #pragma unroll
             for (uint32_t j = 0; j < 8; j++) if (first + j * 8u + lane8 < N) codes[m * N + first + j * 8u + lane8] = (int8_t)to.code(v[j]);
         }
+        m = nm; f = nf; raw = soon;
     }
 }
 
@@ -665,36 +697,36 @@ int launch_column_sums(const float *const in32[2], const uint16_t *half, uint32_
 
 int launch_rows_to_half(const void *x, int dtype, uint32_t M, uint32_t K, uint32_t pitch, uint16_t *out, float *factor, Zeros zeros, void *stream)
 {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(std::min(M, 65535u));
+    cfg.blockDim = dim3(256);
+    cfg.stream = (cudaStream_t)stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = programmatic_launches();
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaError_t e;
     if (dtype != EOQ_B200_F32 && K % 8u == 0 && pitch == K && K <= 16384u && aligned(x, 16)) {
 #define EOQ_ROWS(D) (K <= 2048u ? rows_to_half_vector_kernel<D, 1> : K <= 4096u ? rows_to_half_vector_kernel<D, 2> : rows_to_half_vector_kernel<D, 8>)
         auto kern = dtype == EOQ_B200_F16 ? EOQ_ROWS(EOQ_B200_F16) : EOQ_ROWS(EOQ_B200_BF16);
 #undef EOQ_ROWS
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(std::min(M, 65535u));
-        cfg.blockDim = dim3(256);
-        cfg.stream = (cudaStream_t)stream;
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = programmatic_launches();
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
-        const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, x, M, K, (__half *)out, factor, zeros);
-        count_launch();
-        return (int)(e != cudaSuccess ? e : cudaGetLastError());
+        e = cudaLaunchKernelEx(&cfg, kern, x, M, K, (__half *)out, factor, zeros);
+    } else {
+        e = cudaLaunchKernelEx(&cfg, rows_to_half_kernel, x, dtype, M, K, pitch, (__half *)out, factor, zeros);
     }
-    rows_to_half_kernel<<<std::min(M, 65535u), 256, 0, (cudaStream_t)stream>>>(x, dtype, M, K, pitch, (__half *)out, factor, zeros);
     count_launch();
-    return (int)cudaGetLastError();
+    return (int)(e != cudaSuccess ? e : cudaGetLastError());
 }
 
 int launch_store_8bit(const void *x, int dtype, size_t M, uint32_t N, int8_t *codes, float *scales, void *stream)
 {
-    const size_t blocks = M * ((N + kStoreBlock - 1) / kStoreBlock);
+    const size_t turns = M * ((N + 4u * kStoreBlock - 1) / (4u * kStoreBlock));
     const bool vec = N % 8u == 0 && aligned(x, 16) && aligned(codes, 8);
     auto kern = dtype == EOQ_B200_F32 ? (vec ? store_8bit_kernel<EOQ_B200_F32, true> : store_8bit_kernel<EOQ_B200_F32, false>)
               : dtype == EOQ_B200_F16 ? (vec ? store_8bit_kernel<EOQ_B200_F16, true> : store_8bit_kernel<EOQ_B200_F16, false>)
                                       : (vec ? store_8bit_kernel<EOQ_B200_BF16, true> : store_8bit_kernel<EOQ_B200_BF16, false>);
-    kern<<<ctas_for(blocks, 32u), 256, 0, (cudaStream_t)stream>>>(x, blocks, N, codes, scales);
+    kern<<<ctas_for(turns, 8u), 256, 0, (cudaStream_t)stream>>>(x, M, N, codes, scales);
     count_launch();
     return (int)cudaGetLastError();
 }

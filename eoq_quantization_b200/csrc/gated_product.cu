@@ -660,7 +660,7 @@ gated_product_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap gm
                 asm volatile("bar.sync 5, 128;" ::: "memory");
                 return *word(bTicket) == p_last - p_first;
             };
-            const bool here = ask(0u);
+            const bool here = pairs <= a.tiles && ask(0u);       // (parts that all run at the same time end so, too)
             if (!here) {
                 float *mine = partial_of(pair, s.p0 == 0u);
                 for (uint32_t t0 = 0; t0 < a.T; t0 += 16u) {
