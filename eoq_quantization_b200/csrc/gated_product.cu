@@ -399,10 +399,10 @@ gated_product_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap gm
                     nr.next(a.ns);
                     ready = bar_test(bar(bFull + nr.at), nr.lap);         // asked for while this block's products are being issued
                     // (past the last column of a forward product the codes are the copy's zeros, times a scale, and the activations zeros)
-                    mma_block(d, tmem + a_base + ar.at * 32u, desc0 + ((ar.at * xstage) >> 4), idesc, i, bar(bEmpty + ar.at));
+                    if (!wait.lost) mma_block(d, tmem + a_base + ar.at * 32u, desc0 + ((ar.at * xstage) >> 4), idesc, i, bar(bEmpty + ar.at));
                     ar = nr;
                 }
-                commit_pair(bar(bOutFull + dr.at));
+                if (!wait.lost) commit_pair(bar(bOutFull + dr.at));       // else the way out's waits run out too, in both CTAs
             }
         }
     } else if (warp == kWCodes) {

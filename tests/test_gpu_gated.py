@@ -350,3 +350,56 @@ def test_quantized_linear_is_what_it_was():
     dy = _inputs(40, 320, BF16, 41)
     layer(x).backward(dy)
     assert torch.equal(x.grad, dy @ layer._dequantize_weight().to(BF16))
+
+
+@pytest.mark.parametrize("m,n,k,bits,group,dtype", [
+    # more tiles than pairs of SMs, whose runs end inside tiles; fewer tiles, several pairs each; runs of two whole tiles
+    (60, 10100, 4096, 4, 128, F16), (250, 5000, 8192, 4, 128, BF16), (1000, 2400, 4096, 2, 128, F16), (90, 4500, 2816, 8, 64, F16),
+    (40, 3000, 20000, 4, 160, BF16), (150, 11000, 512, 4, 64, F16), (230, 9000, 2048, 8, 128, BF16), (200, 9000, 1024, 2, 64, F16),
+])
+def test_tiles_that_pairs_share(m, n, k, bits, group, dtype):
+    (pg, sg, wg), (pu, su, wu) = _layers(n, k, bits, group, 7)
+    x = _inputs(m, k, dtype, 1)
+    want = Gated(x, wg, wu, "silu", None, None)
+    inside(gated.gated_packed(pg, sg, pu, su, n, k, bits, group, x), want.h, want.h_bound(), "h")
+    test_input_grad(m, n, k, bits, group, dtype)
+
+
+def test_waits_that_run_out_say_so_and_leave_the_next_call_alone():
+    """No patience at all, behind a kernel that waits for a peer that never sends: a call whose waits run out gives NaN and a status, once (one that started
+    late enough is right); the calls after it are right."""
+    import ctypes as C
+    from eoq_quantization_b200 import _lib as L
+    lib = L.lib()
+    n, k = 700, 1024
+    (pg, sg, _), (pu, su, _) = _layers(n, k, 4, 128, 3)
+    handle, g = (C.c_ubyte * 64)(), C.c_void_p()
+    L.check(lib.eoq_b200_gather_create(2, 0, 2, 2 * 96 * 2, C.byref(g), handle), "eoq_b200_gather_create")
+    L.check(lib.eoq_b200_gather_set_timeout_ms(g, 100), "eoq_b200_gather_set_timeout_ms")
+    ran_out = 0
+    try:
+        for m in (48, 300):
+            x, dy = _inputs(m, k, F16, 1), _inputs(m, n, F16, 2)
+            for call in (lambda: gated.gated_packed(pg, sg, pu, su, n, k, 4, 128, x), lambda: gated.packed_input_grad(pg, sg, n, k, 4, 128, dy)):
+                want = call()
+                assert want.isfinite().all() and lib.eoq_b200_linear_status() == 0
+                torch.cuda.synchronize()
+                assert lib.eoq_b200_tune(b"qmm_wait_us", 0) == 0
+                L.check(lib.eoq_b200_gather_wait(g, 0, 96, 1, L.F16, 3, torch.cuda.current_stream().cuda_stream), "eoq_b200_gather_wait")
+                late = call()
+                torch.cuda.synchronize()
+                assert lib.eoq_b200_tune(b"qmm_wait_us", 2000000) == 0
+                assert torch.equal(call(), want)
+                status = lib.eoq_b200_linear_status()
+                assert lib.eoq_b200_linear_status() == 0
+                assert late.isnan().any() if status else torch.equal(late, want)
+                ran_out += status
+                # a kernel in front that takes longer than a wait may: its time does not count
+                assert lib.eoq_b200_tune(b"qmm_wait_us", 20000) == 0
+                L.check(lib.eoq_b200_gather_wait(g, 0, 96, 1, L.F16, 3, torch.cuda.current_stream().cuda_stream), "eoq_b200_gather_wait")
+                assert torch.equal(call(), want) and lib.eoq_b200_linear_status() == 0
+                assert lib.eoq_b200_tune(b"qmm_wait_us", 2000000) == 0
+        assert ran_out
+    finally:
+        lib.eoq_b200_tune(b"qmm_wait_us", 2000000)
+        lib.eoq_b200_gather_destroy(g)
