@@ -505,8 +505,9 @@ size_t eoq_b200_weight_linear_scratch(const eoq_b200_weight_t *w, uint32_t batch
 eoq_error_t eoq_b200_weight_linear(eoq_b200_weight_t *w, const void *x, int x_dtype, uint32_t batch, void *d_scratch, void *y,
                                    int y_dtype, const float *bias, void *stream);
 
-/* 0, or nonzero if a bounded wait of one of the two kernels above eoq_b200_weight_linear has run out on the current device
- * since the last call (synchronises; what a weight's own products meet is in its eoq_b200_weight_status).  The results of
+/* 0, or nonzero if a bounded wait of one of the two kernels above eoq_b200_weight_linear, or of the gated block's or the packed
+ * gradient's below, has run out on the current device since the last call (synchronises; what a weight's own products meet is in
+ * its eoq_b200_weight_status).  The results of
  * such a launch are NaN; the launches after it are not affected. */
 uint32_t eoq_b200_linear_status(void);
 
@@ -558,13 +559,16 @@ typedef struct eoq_b200_kept {
 /* x [batch, cols] to h [batch, rows], both of type dtype (EOQ_B200_F16 / BF16 / F32), sums in fp32; kept may be NULL.  d_scratch:
  * eoq_b200_gated_scratch() bytes, 16-byte aligned (may be NULL where that is 0).  Any shape; 16-byte aligned pointers, whole
  * groups per row, groups that are multiples of 32 and packed rows that are multiples of 16 bytes take the tensor-core forms.
- * There (more than eight rows) 16-bit activations go in as fp16, bf16 ones times a power of two per row, which is exact for all
- * but what is 2^-24 below the row's largest, and code x scale is rounded to fp16 once.  Asynchronous. */
+ * Up to 24 rows of 16-bit activations (32, where a weight has no more than 50 Mi values), codes and activations are exact there and
+ * scales apply to the sums.  Beyond, activations go in as
+ * fp16, bf16 ones times a power of two per row, which is exact for all but what is 2^-24 below the row's largest, and code x scale is
+ * rounded to fp16 once.  Asynchronous. */
 size_t eoq_b200_gated_scratch(const eoq_b200_gated_t *w, const eoq_b200_kept_t *kept, int dtype, uint32_t batch);
 eoq_error_t eoq_b200_gated_packed(const eoq_b200_gated_t *w, const void *x, int dtype, uint32_t batch, void *d_scratch, void *h,
                                   const eoq_b200_kept_t *kept, void *stream);
 
 /* The backward pass: dh [batch, rows] to dx [batch, cols] (NULL: not wanted) and to the biases' gradients (NULL, or fp32 [rows]).
+ * For 16-bit types dg = dh u act'(g) and du = dh act(g) are rounded to fp16, times a power of two per row, before the products and sums.
  * The sums over rows have a fixed order: two calls give the same bits. */
 size_t eoq_b200_gated_grad_scratch(const eoq_b200_gated_t *w, const eoq_b200_kept_t *kept, int dtype, uint32_t batch);
 eoq_error_t eoq_b200_gated_grad(const eoq_b200_gated_t *w, const eoq_b200_kept_t *kept, const void *dh, int dtype, uint32_t batch,
