@@ -398,8 +398,9 @@ struct SumArgs {
     const __half *half;
     const float *factor;
     float *part;                 // [chunks][2][N]
-    float *out[2];
+    void *out[2];
     uint32_t M, N, pitch, chunks;
+    int dtype;                   // of out
 };
 
 __global__ void __launch_bounds__(256) column_parts_kernel(const SumArgs a)
@@ -441,7 +442,7 @@ __global__ void __launch_bounds__(256) column_sums_kernel(const SumArgs a)
     if (n >= a.N || !a.out[which]) return;
     float v = 0.0f;
     for (uint32_t c = 0; c < a.chunks; c++) v += a.part[((size_t)c * 2 + which) * a.N + n];
-    a.out[which][n] = v;
+    store_from_float(a.out[which], n, v, a.dtype);
 }
 
 // bf16 or fp16 rows of multiples of eight values, aligned: read once, kept in registers.
@@ -682,11 +683,11 @@ int launch_gate_grad(const Kept &k, const void *dh, int dtype, int act, uint32_t
 static uint32_t sum_chunks(uint32_t M) { return (M + kSumRows - 1) / kSumRows; }
 size_t column_sums_scratch(uint32_t M, uint32_t N) { return (size_t)sum_chunks(M) * 2 * N * 4; }
 
-int launch_column_sums(const float *const in32[2], const uint16_t *half, uint32_t pitch, const float *factor, uint32_t M, uint32_t N, float *scratch, float *out[2],
-                       void *stream)
+int launch_column_sums(const float *const in32[2], const uint16_t *half, uint32_t pitch, const float *factor, uint32_t M, uint32_t N, float *scratch, void *const out[2],
+                       int dtype, void *stream)
 {
     cudaStream_t st = (cudaStream_t)stream;
-    SumArgs a = {{in32 ? in32[0] : nullptr, in32 ? in32[1] : nullptr}, (const __half *)half, factor, scratch, {out[0], out[1]}, M, N, pitch, sum_chunks(M)};
+    SumArgs a = {{in32 ? in32[0] : nullptr, in32 ? in32[1] : nullptr}, (const __half *)half, factor, scratch, {out[0], out[1]}, M, N, pitch, sum_chunks(M), dtype};
     column_parts_kernel<<<dim3((N + 63u) / 64u, std::min(a.chunks, 65535u), 2), 256, 0, st>>>(a);
     count_launch();
     cudaError_t e = cudaGetLastError();

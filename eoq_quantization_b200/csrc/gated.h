@@ -51,9 +51,9 @@ struct Zeros { uint32_t *p; uint32_t n; };
 int launch_gate_grad(const Kept &k, const void *dh, int dtype, int act, uint32_t M, uint32_t N, float *out32[2], uint16_t *half, uint32_t pitch, float *factor,
                      Zeros zeros, void *stream);
 int launch_zeros(Zeros zeros, void *stream);
-// Sums over the rows: of fp32 [M][N] x 2, or of the form above.  scratch: column_sums_scratch() bytes.
+// Sums over the rows, to values of dtype: of fp32 [M][N] x 2, or of the form above.  scratch: column_sums_scratch() bytes.
 int launch_column_sums(const float *const in32[2], const uint16_t *half, uint32_t pitch, const float *factor, uint32_t M, uint32_t N, float *scratch,
-                       float *out[2], void *stream);
+                       void *const out[2], int dtype, void *stream);
 size_t column_sums_scratch(uint32_t M, uint32_t N);
 // Rows to fp16, pitch values apart (a multiple of 8; the pad is zero), times a power of two that brings the largest to 2^14 .. 2^15.
 int launch_rows_to_half(const void *x, int dtype, uint32_t M, uint32_t K, uint32_t pitch, uint16_t *out, float *factor, Zeros zeros, void *stream);

@@ -181,11 +181,11 @@ extern "C" size_t eoq_b200_gated_grad_scratch(const eoq_b200_gated_t *w, const e
 }
 
 extern "C" eoq_error_t eoq_b200_gated_grad(const eoq_b200_gated_t *w, const eoq_b200_kept_t *kept, const void *dh, int dtype, uint32_t batch,
-                                           void *d_scratch, void *dx, float *d_gate_bias, float *d_up_bias, void *stream)
+                                           void *d_scratch, void *dx, void *d_gate_bias, void *d_up_bias, void *stream)
 {
     if (!w || !w->gate || !w->up || !w->gate_scales || !w->up_scales || !kept || !kept->gate || !kept->up || !dh || !d_scratch) return EOQ_ERR_NULL_PTR;
     if (kept->form == kKeep8bit && (!kept->gate_scales || !kept->up_scales)) return EOQ_ERR_NULL_PTR;
-    if (dtype < 0 || dtype > 2 || (kept->form != kKeepFull && kept->form != kKeep8bit) || w->activation < 0 || w->activation > kActGeluTanh) return EOQ_ERR_UNSUPPORTED;
+    if (dtype < 0 || dtype > 2 || w->bias_dtype < 0 || w->bias_dtype > 2 || (kept->form != kKeepFull && kept->form != kKeep8bit) || w->activation < 0 || w->activation > kActGeluTanh) return EOQ_ERR_UNSUPPORTED;
     if (batch == 0 || w->rows == 0 || (!dx && !d_gate_bias && !d_up_bias)) return EOQ_OK;
     if (!fine(w->rows, w->cols, w->bits, w->group)) return EOQ_ERR_INVALID_HEADER;
     if (!have_device()) return EOQ_ERR_CUDA;
@@ -193,7 +193,7 @@ extern "C" eoq_error_t eoq_b200_gated_grad(const eoq_b200_gated_t *w, const eoq_
     const PackedPair pair = pair_of(w);
     Carve scratch{static_cast<uint8_t *>(d_scratch)};
     const char *where = "eoq_b200_gated_grad";
-    float *to[2] = {d_gate_bias, d_up_bias};
+    void *const to[2] = {d_gate_bias, d_up_bias};
     if (dtype != EOQ_B200_F32 && product_takes(pair, 2)) {
         const uint32_t pitch = pitch_of(w->rows);
         uint16_t *half = scratch.take<uint16_t>(2 * half_bytes(batch, w->rows));
@@ -202,14 +202,14 @@ extern "C" eoq_error_t eoq_b200_gated_grad(const eoq_b200_gated_t *w, const eoq_
         uint32_t *parts = scratch.take<uint32_t>(s.bytes);
         float *sums = scratch.take<float>(0);
         int e = launch_gate_grad(kept_of(kept), dh, dtype, w->activation, batch, w->rows, nullptr, half, pitch, factor, Zeros{parts, s.zeros}, stream);
-        if (e == 0 && (d_gate_bias || d_up_bias)) e = launch_column_sums(nullptr, half, pitch, factor, batch, w->rows, sums, to, stream);
+        if (e == 0 && (d_gate_bias || d_up_bias)) e = launch_column_sums(nullptr, half, pitch, factor, batch, w->rows, sums, to, w->bias_dtype, stream);
         if (e == 0 && dx) e = launch_input_grad_product(pair, 2, half, pitch, factor, batch, dx, dtype, parts, stream);
         return launched(e, where);
     }
     float *d = scratch.take<float>(2 * n * 4), *out[2] = {d, d + n};
     void *sums = scratch.take<void>(0);
     int e = launch_gate_grad(kept_of(kept), dh, dtype, w->activation, batch, w->rows, out, nullptr, 0, nullptr, Zeros{nullptr, 0}, stream);
-    if (e == 0 && (d_gate_bias || d_up_bias)) e = launch_column_sums(out, nullptr, 0, nullptr, batch, w->rows, static_cast<float *>(sums), to, stream);
+    if (e == 0 && (d_gate_bias || d_up_bias)) e = launch_column_sums(out, nullptr, 0, nullptr, batch, w->rows, static_cast<float *>(sums), to, w->bias_dtype, stream);
     if (e == 0 && dx) {
         const void *dy[2] = {out[0], out[1]};
         e = launch_input_grad_general(pair, 2, dy, EOQ_B200_F32, batch, sums, dx, dtype, stream);

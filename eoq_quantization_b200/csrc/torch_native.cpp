@@ -484,10 +484,10 @@ PyObject *gated_packed(PyObject *, PyObject *const *a, Py_ssize_t n)
 }
 
 // gated_grad(gate, gate_scales, up, up_scales, N, K, bits, group, activation, dh, kept gate, kept up, their scales or None x 2, want dx,
-// want the gate's bias, want the up's): (dx or None, fp32 or None, fp32 or None).
+// want the gate's bias, want the up's, the type of their gradients): (dx or None, a bias's or None, a bias's or None).
 PyObject *gated_grad(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
-    if (n != 17) { PyErr_SetString(PyExc_TypeError, "gated_grad takes 17 arguments"); return nullptr; }
+    if (n != 18) { PyErr_SetString(PyExc_TypeError, "gated_grad takes 18 arguments"); return nullptr; }
     GUARD_BEGIN
     const int64_t N = PyLong_AsLongLong(a[4]), K = PyLong_AsLongLong(a[5]), bits = PyLong_AsLongLong(a[6]), group = PyLong_AsLongLong(a[7]);
     Activations act;
@@ -508,15 +508,16 @@ PyObject *gated_grad(PyObject *, PyObject *const *a, Py_ssize_t n)
     }
     const Ordered ordered(gate.converted || up.converted);
     const eoq_b200_gated_t w = {gate.codes, up.codes, gate.scales, up.scales, nullptr, nullptr, (uint32_t)N, (uint32_t)K, (uint32_t)bits, (uint32_t)group,
-                                (int)PyLong_AsLong(a[8]), EOQ_B200_F32};
+                                (int)PyLong_AsLong(a[8]), (int)PyLong_AsLong(a[17])};
+    const at::ScalarType bias_type = w.bias_dtype == EOQ_B200_F16 ? at::kHalf : w.bias_dtype == EOQ_B200_BF16 ? at::kBFloat16 : at::kFloat;
     const bool want[3] = {PyObject_IsTrue(a[14]) == 1, PyObject_IsTrue(a[15]) == 1, PyObject_IsTrue(a[16]) == 1};
     if (PyErr_Occurred()) return nullptr;
     Tensor scratch = bytes_beside(dh, eoq_b200_gated_grad_scratch(&w, &kept, act.code, (uint32_t)act.rows)), out[3];
     if (want[0]) out[0] = result(dh, K, dh.scalar_type());
-    for (int i = 1; i < 3; i++) if (want[i]) out[i] = at::detail::empty_cuda({N}, at::kFloat, dh.device(), std::nullopt);
+    for (int i = 1; i < 3; i++) if (want[i]) out[i] = at::detail::empty_cuda({N}, bias_type, dh.device(), std::nullopt);
     const eoq_error_t rc = eoq_b200_gated_grad(&w, &kept, dh.data_ptr(), act.code, (uint32_t)act.rows, scratch.data_ptr(), want[0] ? out[0].data_ptr() : nullptr,
-                                               want[1] ? static_cast<float *>(out[1].data_ptr()) : nullptr,
-                                               want[2] ? static_cast<float *>(out[2].data_ptr()) : nullptr, stream_of(dh));
+                                               want[1] ? out[1].data_ptr() : nullptr,
+                                               want[2] ? out[2].data_ptr() : nullptr, stream_of(dh));
     if (rc != EOQ_OK) return failed(rc, "eoq_b200_gated_grad");
     PyObject *r = PyTuple_New(3);
     if (!r) return nullptr;

@@ -6,6 +6,7 @@ torch is used for device memory, streams and the autograd graph; every computati
 """
 from __future__ import annotations
 
+from contextlib import nullcontext
 from typing import Optional
 
 import torch
@@ -51,6 +52,11 @@ class _Unsupported(RuntimeError):
     pass
 
 
+def _without_autocast():
+    """A backward pass's types are its tensors'.  (Entering torch's context takes ten microseconds, so only where autocast is on.)"""
+    return torch.autocast("cuda", enabled=False) if torch.is_autocast_enabled("cuda") else nullcontext()
+
+
 class _Gated(torch.autograd.Function):
     """h, and from what the forward pass kept of gate and up the gradients of x and the biases."""
 
@@ -70,13 +76,15 @@ class _Gated(torch.autograd.Function):
         gate, gate_scales, up, up_scales, *kept = ctx.saved_tensors          # an error if the weights have been written since
         if ctx.form == KEEP["full"]:
             kept += [None, None]
-        with torch.autocast("cuda", enabled=False):
-            out = _lib.native().gated_grad(gate, gate_scales, up, up_scales, *ctx.shape, ctx.activation, dh.detach(), *kept, *ctx.needs_input_grad[:3])
+        types = {t for t in ctx.bias_dtypes if t is not None}          # of one type: written in it; else cast below
+        bias_type = _DTYPES.get(next(iter(types)), _lib.F32) if len(types) == 1 else _lib.F32
+        with _without_autocast():
+            out = _lib.native().gated_grad(gate, gate_scales, up, up_scales, *ctx.shape, ctx.activation, dh.detach(), *kept, *ctx.needs_input_grad[:3], bias_type)
         if out is None:
             raise RuntimeError("gated_packed: the backward pass is not supported")
         dx, *db = out
         dx = None if dx is None else dx.view(ctx.x_shape)
-        db = [None if b is None else b.to(t) for b, t in zip(db, ctx.bias_dtypes)]
+        db = [b if b is None or b.dtype == t else b.to(t) for b, t in zip(db, ctx.bias_dtypes)]
         return (dx, *db) + (None,) * 7
 
 
@@ -94,7 +102,7 @@ class _InputGradProduct(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         packed, scales = ctx.saved_tensors
-        with torch.autocast("cuda", enabled=False):
+        with _without_autocast():
             dx = packed_input_grad(packed, scales, *ctx.shape, dy.detach()) if ctx.needs_input_grad[0] else None
             db = dy.reshape(-1, dy.shape[-1]).sum(0).to(ctx.bias_dtype) if ctx.needs_input_grad[1] else None
         return dx, db, None, None, None

@@ -567,12 +567,13 @@ size_t eoq_b200_gated_scratch(const eoq_b200_gated_t *w, const eoq_b200_kept_t *
 eoq_error_t eoq_b200_gated_packed(const eoq_b200_gated_t *w, const void *x, int dtype, uint32_t batch, void *d_scratch, void *h,
                                   const eoq_b200_kept_t *kept, void *stream);
 
-/* The backward pass: dh [batch, rows] to dx [batch, cols] (NULL: not wanted) and to the biases' gradients (NULL, or fp32 [rows]).
+/* The backward pass: dh [batch, rows] to dx [batch, cols] (NULL: not wanted) and to the biases' gradients (NULL, or [rows] of
+ * bias_dtype, summed in fp32).
  * For 16-bit types dg = dh u act'(g) and du = dh act(g) are rounded to fp16, times a power of two per row, before the products and sums.
  * The sums over rows have a fixed order: two calls give the same bits. */
 size_t eoq_b200_gated_grad_scratch(const eoq_b200_gated_t *w, const eoq_b200_kept_t *kept, int dtype, uint32_t batch);
 eoq_error_t eoq_b200_gated_grad(const eoq_b200_gated_t *w, const eoq_b200_kept_t *kept, const void *dh, int dtype, uint32_t batch,
-                                void *d_scratch, void *dx, float *d_gate_bias, float *d_up_bias, void *stream);
+                                void *d_scratch, void *dx, void *d_gate_bias, void *d_up_bias, void *stream);
 
 /* dx = dy W, the gradient that a packed weight passes on: dy [batch, rows], dx [batch, cols], both of type dtype. */
 size_t eoq_b200_packed_input_grad_scratch(uint32_t rows, uint32_t cols, uint32_t bits, uint32_t group, int dtype, uint32_t batch);
