@@ -116,14 +116,6 @@ __device__ __forceinline__ void commit_pair(uint32_t bar)
                  "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(bar), "h"((uint16_t)3) : "memory");
 }
 
-// Whether a phase is over, without waiting (a try_wait, whose answer may take until it is, would keep the warp).
-__device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity)
-{
-    uint32_t ok;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-    return ok != 0;
-}
-
 // A wait that may sleep for a millisecond: warps that ask again and again take the issue slots of those that work.
 __device__ __forceinline__ bool bar_try_long(uint32_t bar, uint32_t parity)
 {
@@ -149,7 +141,7 @@ struct Patience {
     }
     __device__ __forceinline__ void operator()(uint32_t bar, uint32_t parity)
     {
-        if (!bar_try(bar, parity)) lost = slow(bar, parity, mark, limit) || lost;
+        if (!for_the_warp(bar_try(bar, parity))) lost = slow(bar, parity, mark, limit) || lost;
     }
     static __device__ __noinline__ bool slow(uint32_t bar, uint32_t parity, uint32_t mark, long long limit)
     {
@@ -405,7 +397,7 @@ gated_product_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap gm
                     fence_after();
                     Ring nr = ar;
                     nr.next(a.ns);
-                    ready = bar_test(bar(bFull + nr.at), nr.lap);         // asked for while this block's products are being issued
+                    ready = for_the_warp(bar_test(bar(bFull + nr.at), nr.lap));         // asked for while this block's products are being issued
                     // (past the last column of a forward product the codes are the copy's zeros, times a scale, and the activations zeros)
                     if (!wait.lost) mma_block(d, tmem + a_base + ar.at * 32u, desc0 + ((ar.at * xstage) >> 4), idesc, i, bar(bEmpty + ar.at));
                     ar = nr;

@@ -139,14 +139,11 @@ __global__ void __launch_bounds__(most_threads(BT), 1) gated_rows_kernel(const R
         if (++load_chunk == chunks) { load_chunk = 0; load_tile++; }
     };
     auto wait = [&](uint32_t bar, uint32_t parity) {
-        if (bar_try(bar, parity)) return;
+        if (for_the_warp(bar_test(bar, parity))) return;
         const long long t0 = clock64();
-        while (!bar_try(bar, parity)) {
-            if (clock64() - t0 <= a.limit && !gave_up) continue;
-            gave_up = true;                        // (of all lanes or none: the loop is left together, below)
-            break;
-        }
-        gave_up = __any_sync(0xffffffffu, gave_up);
+        bool late = a.limit == 0;                  // no patience at all: what is not there has run out
+        while (!late && !bar_try(bar, parity)) late = clock64() - t0 > a.limit;
+        gave_up = __any_sync(0xffffffffu, late);
         if (gave_up && lane == 0) {
             asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(mark), "r"(1u) : "memory");
             *reinterpret_cast<volatile uint32_t *>(a.status) = 1u;
@@ -391,10 +388,10 @@ gated_many_rows_kernel(const ManyArgs a, const __grid_constant__ CUtensorMap gma
 
     bool gave_up = false;
     auto wait = [&](uint32_t bar, uint32_t parity) {
-        if (bar_try(bar, parity)) return;
+        if (for_the_warp(bar_test(bar, parity))) return;
         const long long t0 = clock64();
-        bool late = false;
-        while (!late && !bar_try(bar, parity)) late = clock64() - t0 > a.limit || gave_up;
+        bool late = a.limit == 0 || gave_up;
+        while (!late && !bar_try(bar, parity)) late = clock64() - t0 > a.limit;
         if (__any_sync(0xffffffffu, late)) {
             gave_up = true;
             if (lane == 0) {

@@ -26,6 +26,16 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity)
     asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok != 0;
 }
+// Whether a phase is over, without waiting (a try_wait, whose answer may take until it is, would keep the warp).
+__device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity)
+{
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+// A barrier answers each lane for itself, and where it completes meanwhile they are told different things.  One answer for the
+// warp, for waits behind which the lanes vote or elect together: a lane that had gone on alone would be missing there.
+__device__ __forceinline__ bool for_the_warp(bool yes) { return __all_sync(0xffffffffu, yes); }
 
 // The last uses of a ring of n barriers, of which `used` have been made: what the copy engine still has to bring is
 // there (or does not come for some ten milliseconds) before the CTA may leave its shared memory.
