@@ -386,12 +386,18 @@ gated_many_rows_kernel(const ManyArgs a, const __grid_constant__ CUtensorMap gma
     uint32_t tile0 = blockIdx.x * a.per + min(blockIdx.x, a.more);
     const uint32_t last = tile0 + a.per + (blockIdx.x < a.more);
 
+    // A warp that has given up, by itself or because another one of the CTA has, requests nothing and tells no barrier: a slice that it
+    // has not seen would be handed over, or written under those who still read it.
     bool gave_up = false;
     auto wait = [&](uint32_t bar, uint32_t parity) {
-        if (for_the_warp(bar_test(bar, parity))) return;
+        if (gave_up || for_the_warp(bar_test(bar, parity))) return;
         const long long t0 = clock64();
-        bool late = a.limit == 0 || gave_up;
-        while (!late && !bar_try(bar, parity)) late = clock64() - t0 > a.limit;
+        bool late = a.limit == 0;
+        while (!late && !bar_try(bar, parity)) {
+            uint32_t stop;
+            asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(stop) : "r"(mark) : "memory");
+            late = stop || clock64() - t0 > a.limit;
+        }
         if (__any_sync(0xffffffffu, late)) {
             gave_up = true;
             if (lane == 0) {
@@ -416,6 +422,7 @@ gated_many_rows_kernel(const ManyArgs a, const __grid_constant__ CUtensorMap gma
         for (uint32_t tiles_left = last - tile0; tiles_left; tiles_left -= min(tiles_left, a.most))
             for (uint32_t s = 0; s < slices; s++, r.next(2u)) {
                 wait(empty + 8u * r.at, r.lap ^ 1u);
+                if (gave_up) break;
                 const uint32_t c0 = s * a.slice, have = min(a.slice, chunks - c0);
                 uint4 *to = xs + r.at * a.slice * kPieces;
                 // 128 columns of two rows a warp and step: whole lines to read, and no two of a store's phase in one bank; eight steps under way
@@ -468,14 +475,17 @@ gated_many_rows_kernel(const ManyArgs a, const __grid_constant__ CUtensorMap gma
 #pragma unroll
                 for (int j = 0; j < 4; j++) tot[n][j] = 0.0f;
             uint32_t chunk = part;
+            // copies of this warp are under way, whichever wait runs out
+            auto wait_for = [&](uint32_t bar, uint32_t parity) {
+                if (gave_up) return;
+                wait(bar, parity);
+                if (gave_up) { lost = wr; owing = (requested - chunk) / a.split; }
+            };
             for (uint32_t s = 0; s < slices; s++, xr.next(2u)) {
-                wait(full + 8u * xr.at, xr.lap);
+                wait_for(full + 8u * xr.at, xr.lap);
                 const uint32_t end = work ? min(chunks, (s + 1) * a.slice) : 0u;
                 for (; chunk < end; chunk += a.split, wr.next(kSlots)) {
-                    if (!gave_up) {
-                        wait(mine + wr.at * 8u, wr.lap);
-                        if (gave_up) { lost = wr; owing = (requested - chunk) / a.split; }
-                    }
+                    wait_for(mine + wr.at * 8u, wr.lap);
                     uint32_t w = w0 + wr.at * kSlot, x = x0 + (xr.at * a.slice + chunk - s * a.slice) * (kPieces * 16u), at_scale = s0 + (EXACT ? chunk * (CH * kUnits * 2u) : 0u);
                     pin(w, x, at_scale);
                     uint32_t sc[2][kScales] = {};
@@ -559,7 +569,7 @@ gated_many_rows_kernel(const ManyArgs a, const __grid_constant__ CUtensorMap gma
                     request(wr.at);
                 }
                 __syncwarp();
-                if (lane == 0) bar_arrive(empty + 8u * xr.at);
+                if (lane == 0 && !gave_up) bar_arrive(empty + 8u * xr.at);
             }
             if (owing) {                               // no copy may be under way when its place is used otherwise
                 const long long t0 = clock64();

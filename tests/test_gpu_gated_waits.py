@@ -36,8 +36,10 @@ def _runs_out(call, patience, times=30):
         return call()
     want = call()
     assert want.isfinite().all() and lib.eoq_b200_linear_status() == 0
-    patience(0)
-    late = [late_call() for _ in range(times)]
+    late = []
+    for us in (1, 0):
+        patience(us)
+        late += [late_call() for _ in range(times)]
     patience(2000000)
     again = call()
     assert torch.equal(again, want)
@@ -54,7 +56,15 @@ def test_few_rows(m, n, k, group, patience):
     _runs_out(lambda: gated.gated_packed(pg, sg, pu, su, n, k, 4, group, x), patience)
 
 
-@pytest.mark.parametrize("m", [1, 8])
+# slices of activations and codes that do not come; several tiles a warp; several rounds of tiles a CTA
+@pytest.mark.parametrize("m,n,k,group", [(24, 11008, 4096, 128), (32, 3000, 4096, 64), (9, 30000, 1024, 128), (17, 700, 8192, 128)])
+def test_up_to_32_rows(m, n, k, group, patience):
+    """A warp that gives up for want of activations has copies of codes under way, which end before the warp's ring holds its sums and
+    before the CTA does."""
+    test_few_rows(m, n, k, group, patience)
+
+
+@pytest.mark.parametrize("m", [1, 8, 24])
 def test_a_slow_kernel_in_front_does_not_count(m, patience):
     lib = L.lib()
     n, k = 700, 1024
