@@ -152,8 +152,9 @@ struct Patience {
             uint32_t stop, alone;
             asm volatile("ld.volatile.shared.v2.u32 {%0, %1}, [%2];" : "=r"(stop), "=r"(alone) : "r"(mark) : "memory");
             if (!alone && limit) t0 = now;
-            // once a launch has given up, the others of a grid of many rounds wait an eighth as long
-            gave_up = stop || now - t0 > limit || (now - t0 > limit / 8 && *reinterpret_cast<volatile uint32_t *>(&g_gated_status));
+            // (all CTAs are there at the same time, so that their waits run out together: the status word, which stays set until it is asked
+            // for, is nobody's reason to give up)
+            gave_up = stop || now - t0 > limit;
         }
         gave_up = __any_sync(0xffffffffu, gave_up);
         if (gave_up) {

@@ -508,7 +508,8 @@ eoq_error_t eoq_b200_weight_linear(eoq_b200_weight_t *w, const void *x, int x_dt
 /* 0, or nonzero if a bounded wait of one of the two kernels above eoq_b200_weight_linear, or of the gated block's or the packed
  * gradient's below, has run out on the current device since the last call (synchronises; what a weight's own products meet is in
  * its eoq_b200_weight_status).  The results of
- * such a launch are NaN; the launches after it are not affected. */
+ * such a launch are NaN.  The launches after it are not affected, but that those of the two kernels above give a wait an eighth of
+ * its time until this has been called. */
 uint32_t eoq_b200_linear_status(void);
 
 /* y = x @ W.T (+ bias) straight from PolarLinear's in-memory form (kernels/polar_engine.py:144-360: one centroid index

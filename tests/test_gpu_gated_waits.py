@@ -82,3 +82,31 @@ def test_a_slow_kernel_in_front_does_not_count(m, patience):
     finally:
         torch.cuda.synchronize()
         lib.eoq_b200_gather_destroy(g)
+
+
+def test_a_call_that_gave_up_takes_no_patience_from_later_ones(patience):
+    """A product whose last sums take two milliseconds, with eight to wait for them, while the status says that another call's
+    waits have run out."""
+    (pg, sg, _), (pu, su, _) = weight(11008, 4096, 4, 128, 1), weight(11008, 4096, 4, 128, 2)
+    few = torch.ones(1, 4096, dtype=F16, device="cuda")
+    # a tile of 256 columns for each of up to 74 pairs of SMs, its sums over half a million rows
+    n, k, m = 1 << 19, 74 * 256, 256
+    packed = torch.randint(0, 15, (n, k // 2), dtype=torch.uint8, device="cuda")
+    scales = torch.full((n,), 2.0 ** -10, dtype=F16, device="cuda")
+    dy = torch.randn(m, n, device="cuda").to(F16)
+    call = lambda: gated.packed_input_grad(packed, scales, n, k, 4, k, dy)  # noqa: E731
+    want = call()
+    assert want.isfinite().all() and L.lib().eoq_b200_linear_status() == 0
+    _give_up(lambda: gated.gated_packed(pg, sg, pu, su, 11008, 4096, 4, 128, few), patience)
+    patience(8000)
+    assert torch.equal(call(), want) and L.lib().eoq_b200_linear_status() == 1
+
+
+def _give_up(call, patience):
+    """The call without patience, its codes not in the L2, and the status not asked for."""
+    patience(0)
+    cache = torch.empty(512 << 20, dtype=torch.uint8, device="cuda")
+    for _ in range(20):
+        cache.zero_()
+        late = call()
+    assert late.isnan().any()
