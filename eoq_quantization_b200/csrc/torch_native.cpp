@@ -133,10 +133,11 @@ struct Activations {
     std::optional<c10::cuda::CUDAGuard> guard;
 };
 
-bool resident(const Tensor *t, const Tensor &x, at::ScalarType type)
+bool beside(const Tensor *t, const Tensor &x, at::ScalarType type)
 {
-    return t && t->is_cuda() && t->get_device() == x.get_device() && t->scalar_type() == type && t->is_contiguous();
+    return t && t->is_cuda() && t->get_device() == x.get_device() && t->layout() == at::kStrided && t->scalar_type() == type;
 }
+bool resident(const Tensor *t, const Tensor &x, at::ScalarType type) { return beside(t, x, type) && t->is_contiguous(); }
 
 // A parameter of the module beside x in the type that the kernels read, converted for this call where a cast of the module
 // (half(), to(bfloat16), float(), double()) left it in another one: for this call only, since nothing that a copy could be
@@ -176,8 +177,8 @@ struct Bias {
     Parameter value;
 };
 
-// While this lives the library launches its kernels one behind the other: they read scales before the kernel in front of them
-// has ended, which may be the one that is writing the converted copy.
+// While this lives the library launches its kernels one behind the other: they read codes and scales before the kernel in front of
+// them has ended, which may be the one that is writing the converted copy.
 struct Ordered {
     explicit Ordered(bool on) : was(on ? eoq_b200_ordered_launches(1) : -1) {}
     ~Ordered() { if (was >= 0) eoq_b200_ordered_launches(was); }
@@ -390,8 +391,8 @@ PyObject *polar_linear(PyObject *, PyObject *const *a, Py_ssize_t n)
 
 // -- the gated block on packed weights ------------------------------------------
 
-// A packed weight beside x: codes in the layout of `bits`, scales that cover the flattened matrix, converted to fp16 where a cast
-// of the module left them in another type.
+// A packed weight beside x: codes in the layout of `bits`, copied where they are strided, scales that cover the flattened matrix,
+// converted to fp16 where a cast of the module left them in another type.
 struct Packed {
     const uint8_t *codes = nullptr;
     const uint16_t *scales = nullptr;
@@ -401,17 +402,25 @@ struct Packed {
         const Tensor *pk = tensor_of(codes_);
         const int64_t row_bytes = bits == 4 ? (K + 1) / 2 : bits == 2 ? (K + 3) / 4 : K;
         if (N < 1 || N > 0x7fffffff || K < 1 || K > 0x7fffffff || bits < 2 || bits > 8 || group < 1 || group > 0x7fffffff ||
-            !resident(pk, x, bits == 4 || bits == 2 ? at::kByte : at::kChar) || pk->numel() != N * row_bytes || !sc.open(scales_, x, at::kHalf) ||
+            !beside(pk, x, bits == 4 || bits == 2 ? at::kByte : at::kChar) || pk->numel() != N * row_bytes || !sc.open(scales_, x, at::kHalf) ||
             sc.t->numel() < (N * K + group - 1) / group)
             return false;
+        converted = sc.converted;
+        if (!pk->is_contiguous()) {
+            if (kind_of(*pk) != kPlain) return false;
+            at::AutoDispatchBelowADInplaceOrView below;
+            held = pk->contiguous();
+            pk = &held;
+            converted = true;
+        }
         codes = static_cast<const uint8_t *>(pk->data_ptr());
         scales = static_cast<const uint16_t *>(sc.t->data_ptr());
-        converted = sc.converted;
         return true;
     }
 
   private:
     Parameter sc;
+    Tensor held;
 };
 
 Tensor bytes_beside(const Tensor &x, size_t n) { return at::detail::empty_cuda({(int64_t)n}, at::kByte, x.device(), std::nullopt); }

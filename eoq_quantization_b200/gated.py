@@ -143,7 +143,6 @@ def gated_packed(gate: torch.Tensor, gate_scales: torch.Tensor, up: torch.Tensor
     if dt is not None:
         with torch.autocast("cuda", enabled=False):
             return gated_packed(gate, gate_scales, up, up_scales, rows, cols, bits, group, x.to(dt), gate_bias, up_bias, activation=activation, saved=saved)
-    gate, up = gate.contiguous(), up.contiguous()
     kind = call_kind(x, gate_bias, up_bias)
     if kind == WATCHED:                      # transforms, tangents, modes: torch's own operations on dequantised copies
         g, u = (F.linear(x, dequant_packed(w, s, rows, cols, bits, group).to(x.dtype), None if b is None else b.to(x.dtype))
@@ -173,7 +172,7 @@ def packed_input_grad(packed: torch.Tensor, scales: torch.Tensor, rows: int, col
         if grad.numel() == 0:
             return grad.new_zeros(*grad.shape[:-1], cols)
         with torch.autocast("cuda", enabled=False):
-            dx = _lib.native().input_grad(packed.contiguous(), scales, rows, cols, bits, group, grad)
+            dx = _lib.native().input_grad(packed, scales, rows, cols, bits, group, grad)
     if dx is None:
         raise RuntimeError(f"{what}: the call is not supported")
     return dx

@@ -1,0 +1,53 @@
+"""Calls of the gated block and of the packed gradient out of the ordinary."""
+import pytest
+import torch
+
+from eoq_quantization_b200 import gated
+from gated_reference import weight
+
+pytestmark = pytest.mark.gpu
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+
+
+def _layers(n, k, bits, group, seed):
+    return weight(n, k, bits, group, seed), weight(n, k, bits, group, seed + 100)
+
+
+def _inputs(m, k, dtype, seed, spread=1.0):
+    return (torch.randn(m, k, generator=torch.Generator().manual_seed(seed)) * spread).to(dtype).cuda()
+
+
+@pytest.mark.parametrize("m", [1, 12, 40])
+@pytest.mark.parametrize("bits", [2, 4, 8])
+def test_strided_codes(m, bits):
+    """Copied in front of kernels that read codes early: these are launched behind the copy, and in a recording, too."""
+    n, k = 2816, 4096
+    (pg, sg, _), (pu, su, _) = _layers(n, k, bits, 128, 1)
+    wide = lambda t: torch.stack([t, t + 1], 1)[:, 0]  # noqa: E731
+    x, dh = _inputs(m, k, BF16, 2), _inputs(m, n, BF16, 3)
+    want = gated.gated_packed(pg, sg, pu, su, n, k, bits, 128, x), gated.packed_input_grad(pg, sg, n, k, bits, 128, dh)
+    leaf = x.clone().requires_grad_()
+    dx, = torch.autograd.grad(gated.gated_packed(pg, sg, pu, su, n, k, bits, 128, leaf), leaf, dh)
+    sg_, su_ = torch.stack([sg, sg], 1)[:, 0], torch.stack([su, su], 1)[:, 0]
+    pg_, pu_ = wide(pg), wide(pu)
+    assert not pg_.is_contiguous() and not sg_.is_contiguous()
+
+    def calls():
+        h = gated.gated_packed(pg_, sg_, pu_, su_, n, k, bits, 128, leaf)
+        return (gated.gated_packed(pg_, sg_, pu, su, n, k, bits, 128, x), gated.packed_input_grad(pg_, sg_, n, k, bits, 128, dh), h.detach(),
+                torch.autograd.grad(h, leaf, dh)[0])
+    for got in (calls(), calls()):
+        assert all(torch.equal(a, b) for a, b in zip(got, (*want, want[0], dx)))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        calls()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = calls()
+    for _ in range(3):
+        for t in got:
+            t.zero_()
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, (*want, want[0], dx)))
