@@ -12,6 +12,7 @@ from typing import Optional
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.nn.modules import module as _modules
 
 from . import _lib
 from .core.quantized_linear import QuantizedLinear
@@ -235,11 +236,20 @@ def store_8bit(x: torch.Tensor) -> Stored8:
     return Stored8(*out, x.dtype)
 
 
+def _only_products(*layers: nn.Module) -> bool:
+    """Whether calling the layers comes to their products with packed weights: nothing hooked on, put in their place or in their
+    ``forward``'s."""
+    if _modules._global_forward_hooks or _modules._global_forward_pre_hooks or _modules._global_backward_hooks or _modules._global_backward_pre_hooks:
+        return False
+    return all(type(m) is QuantizedLinear and not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks) and
+               "forward" not in m.__dict__ for m in layers)
+
+
 class QuantizedGatedMLP(nn.Module):
     """down(act(gate(x)) * up(x)) of three ``QuantizedLinear`` layers, gate and up in one kernel.
 
     With gradients, gate's and up's results are kept as `saved` says ("full" or "8bit"), and the gradients go back through the
-    codes: no projection is dequantised."""
+    codes: no projection is dequantised.  Layers with hooks, or that something else has taken the place of, are called as they are."""
 
     def __init__(self, gate: QuantizedLinear, up: QuantizedLinear, down: QuantizedLinear, activation: str = "silu", saved: str = "full"):
         super().__init__()
@@ -263,9 +273,12 @@ class QuantizedGatedMLP(nn.Module):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         g, u, d = self.gate, self.up, self.down
-        h = gated_packed(g.packed_weight, g.scales, u.packed_weight, u.scales, g.out_features, g.in_features, g.bits, g.block_size, x, g.bias_param,
-                         u.bias_param, activation=self.activation, saved=self.saved)
-        if autocast_dtype(h) is None and h.dtype in _DTYPES and h.numel() and call_kind(h, d.bias_param) == GRADIENT:
+        if _only_products(g, u):
+            h = gated_packed(g.packed_weight, g.scales, u.packed_weight, u.scales, g.out_features, g.in_features, g.bits, g.block_size, x, g.bias_param,
+                             u.bias_param, activation=self.activation, saved=self.saved)
+        else:
+            h = _TORCH_ACTIVATIONS[self.activation](g(x)) * u(x)
+        if _only_products(d) and autocast_dtype(h) is None and h.dtype in _DTYPES and h.numel() and call_kind(h, d.bias_param) == GRADIENT:
             return _InputGradProduct.apply(h, d.bias_param, d, d.packed_weight, d.scales)
         return d(h)
 

@@ -51,3 +51,28 @@ def test_strided_codes(m, bits):
             t.zero_()
         graph.replay()
         assert all(torch.equal(a, b) for a, b in zip(got, (*want, want[0], dx)))
+
+
+@pytest.mark.parametrize("where", ["gate", "up", "down"])
+@pytest.mark.parametrize("m,dtype", [(3, F32), (40, F16)])
+def test_adapters_hooked_on(where, m, dtype):
+    """An adapter's output added by a hook counts, in the value, in its own gradient and in that of the activations."""
+    torch.manual_seed(1)
+    mlp = gated.QuantizedGatedMLP.from_float(*(torch.nn.Linear(*s).cuda() for s in ((256, 320), (256, 320), (320, 256))), block_size=64)
+    layer = getattr(mlp, where)
+    adapter = torch.nn.Linear(layer.in_features, layer.out_features, bias=False).cuda().to(dtype)
+    handle = layer.register_forward_hook(lambda module, args, out: out + adapter(args[0]))
+    x, dy = _inputs(m, 256, dtype, 2), _inputs(m, 256, dtype, 3)
+    got = []
+    for call in (mlp, lambda t: mlp.down(torch.nn.functional.silu(mlp.gate(t)) * mlp.up(t))):
+        leaf = x.clone().requires_grad_()
+        y = call(leaf)
+        got.append([y.detach(), *torch.autograd.grad(y, (leaf, adapter.weight), dy)])
+    handle.remove()
+    # the fused half rounds h once where the layers round gate, up, their product and h: half steps, weighed by what follows
+    tol = 12 * torch.finfo(dtype).eps / 2 + 2.0 ** -10 * (dtype != F32) + 2.0 ** -16
+    for a, b in zip(*got):
+        assert (a - b).double().norm() <= tol * b.double().norm()
+    leaf = x.clone().requires_grad_()
+    y = mlp(leaf)
+    assert (y.detach() - got[0][0]).double().norm() > 0.05 * y.double().norm()
