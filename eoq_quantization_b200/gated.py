@@ -249,7 +249,8 @@ class QuantizedGatedMLP(nn.Module):
     """down(act(gate(x)) * up(x)) of three ``QuantizedLinear`` layers, gate and up in one kernel.
 
     With gradients, gate's and up's results are kept as `saved` says ("full" or "8bit"), and the gradients go back through the
-    codes: no projection is dequantised.  Layers with hooks, or that something else has taken the place of, are called as they are."""
+    codes: no projection is dequantised.  Layers with hooks, or that something else has taken the place of, are called as they are, and so
+    are all of them for types that the kernels do not take (fp64)."""
 
     def __init__(self, gate: QuantizedLinear, up: QuantizedLinear, down: QuantizedLinear, activation: str = "silu", saved: str = "full"):
         super().__init__()
@@ -273,7 +274,7 @@ class QuantizedGatedMLP(nn.Module):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         g, u, d = self.gate, self.up, self.down
-        if _only_products(g, u):
+        if _only_products(g, u) and x.dtype in _DTYPES:
             h = gated_packed(g.packed_weight, g.scales, u.packed_weight, u.scales, g.out_features, g.in_features, g.bits, g.block_size, x, g.bias_param,
                              u.bias_param, activation=self.activation, saved=self.saved)
         else:

@@ -76,3 +76,16 @@ def test_adapters_hooked_on(where, m, dtype):
     leaf = x.clone().requires_grad_()
     y = mlp(leaf)
     assert (y.detach() - got[0][0]).double().norm() > 0.05 * y.double().norm()
+
+
+def test_module_takes_what_its_layers_take():
+    torch.manual_seed(1)
+    mlp = gated.QuantizedGatedMLP.from_float(*(torch.nn.Linear(*s).cuda() for s in ((256, 320), (256, 320), (320, 256))), block_size=64, activation="gelu")
+    x = _inputs(5, 256, F32, 2).double()
+    got = []
+    for call in (mlp, lambda t: mlp.down(torch.nn.functional.gelu(mlp.gate(t)) * mlp.up(t))):
+        leaf = x.clone().requires_grad_()
+        y = call(leaf)
+        got.append((call(x), y.detach(), *torch.autograd.grad(y, leaf, x)))
+    for a, b in zip(*got):
+        assert a.dtype == torch.float64 and torch.equal(a, b)
