@@ -403,7 +403,7 @@ struct Packed {
         const int64_t row_bytes = bits == 4 ? (K + 1) / 2 : bits == 2 ? (K + 3) / 4 : K;
         if (N < 1 || N > 0x7fffffff || K < 1 || K > 0x7fffffff || bits < 2 || bits > 8 || group < 1 || group > 0x7fffffff ||
             !beside(pk, x, bits == 4 || bits == 2 ? at::kByte : at::kChar) || pk->numel() != N * row_bytes || !sc.open(scales_, x, at::kHalf) ||
-            sc.t->numel() < (N * K + group - 1) / group)
+            sc.t->numel() < (N * K + group - 1) / group || kind_of(*tensor_of(scales_)) != kPlain)       // (no gradients for scales: refused by the caller)
             return false;
         converted = sc.converted;
         if (!pk->is_contiguous()) {

@@ -117,7 +117,7 @@ def gated_packed(gate: torch.Tensor, gate_scales: torch.Tensor, up: torch.Tensor
     Both weights are ``QuantizedLinear`` buffers of one shape: (rows, cols) codes of `bits` bits and fp16 scales, one for `group`
     codes of the flattened matrix.  `activation`: "silu", "gelu" (exact) or "gelu_tanh".  Differentiable once with respect to x
     and the biases; `saved` says what is kept for that, both projections' results in x.dtype ("full") or in 8 bits ("8bit": as
-    ``store_8bit`` keeps them, 8.5 bits a value); without gradients nothing is.  Sums in fp32."""
+    ``store_8bit`` keeps them, 8.5 bits a value); without gradients nothing is.  Scales that want gradients are refused.  Sums in fp32."""
     code = ACTIVATIONS.get(activation)
     if code is not None and saved in ("full", "8bit"):
         h = _lib.native().gated_packed(gate, gate_scales, up, up_scales, rows, cols, bits, group, x, gate_bias, up_bias, code, 0)

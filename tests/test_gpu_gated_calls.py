@@ -89,3 +89,20 @@ def test_module_takes_what_its_layers_take():
         got.append((call(x), y.detach(), *torch.autograd.grad(y, leaf, x)))
     for a, b in zip(*got):
         assert a.dtype == torch.float64 and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("wants", [False, True])
+def test_scales_that_want_gradients(which, wants):
+    """Refused, whether or not the activations want some too; without gradients the call is what it is for any scales."""
+    n, k = 64, 128
+    (pg, sg, _), (pu, su, _) = _layers(n, k, 4, 128, 1)
+    x = _inputs(3, k, F16, 2)
+    want = gated.gated_packed(pg, sg, pu, su, n, k, 4, 128, x)
+    (sg, su)[which].requires_grad_()
+    with pytest.raises(ValueError, match="no gradients for scales"):
+        gated.gated_packed(pg, sg, pu, su, n, k, 4, 128, x.clone().requires_grad_(wants))
+    with torch.no_grad():
+        assert torch.equal(gated.gated_packed(pg, sg, pu, su, n, k, 4, 128, x), want)
+        dx = gated.packed_input_grad(pg, sg, n, k, 4, 128, want)
+    assert torch.equal(gated.packed_input_grad(pg, sg.detach(), n, k, 4, 128, want), dx)
