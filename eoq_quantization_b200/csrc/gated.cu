@@ -314,9 +314,9 @@ __global__ void __launch_bounds__(256) gate_apply_kernel(const float *__restrict
 }
 
 // The same to fp16 where rows are multiples of eight values and aligned: a row's inputs are read once and stay in registers, as they
-// came (KEEP8: with their scales), eight values a thread ROUNDS times.  The row's power of two comes from a bound of its largest
-// gradient that takes no exponential, |dh| max(1.13 |u|, |g|): a slope is below 1.13 in magnitude and |act(g)| is at most |g|.  It
-// can be some bits above the largest, of which fp16 has enough (a row's largest is at 2^14, the smallest normal number at 2^-14).
+// came (KEEP8: with their scales), eight values a thread ROUNDS times; the gradients are computed twice.  (A bound of the largest that takes no
+// exponential, |dh| max(1.13 |u|, |g|), is any number of bits above it where all gates that dh meets are closed: at silu(-25) it left
+// the row's gradients four bits.)
 template <int DTYPE, bool KEEP8, int ROUNDS>
 __global__ void __launch_bounds__(512) gate_grad_rows_kernel(const GateGradArgs a)
 {
@@ -343,6 +343,20 @@ __global__ void __launch_bounds__(512) gate_grad_rows_kernel(const GateGradArgs 
             values_of<DTYPE>(k.v, f);
         }
     };
+    // eight values of both gradients
+    auto gradients = [&](const Raw8<DTYPE> &rd, const K &rg, const K &ru, float (&g)[8], float (&u)[8]) {
+        float d[8];
+        values_of<DTYPE>(rd, d);
+        kept_values(rg, g);
+        kept_values(ru, u);
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            float value, slope;
+            activation_and_slope(g[j], a.act, value, slope);
+            g[j] = d[j] * u[j] * slope;
+            u[j] = d[j] * value;
+        }
+    };
     for (uint32_t m = blockIdx.x; m < a.M; m += gridDim.x) {
         Raw8<DTYPE> rd[ROUNDS];
         K rg[ROUNDS], ru[ROUNDS];
@@ -359,12 +373,10 @@ __global__ void __launch_bounds__(512) gate_grad_rows_kernel(const GateGradArgs 
         for (int r = 0; r < ROUNDS; r++) {
             const uint32_t n = (r * 512u + threadIdx.x) * 8u;
             if (n >= a.N) continue;
-            float d[8], g[8], u[8];
-            values_of<DTYPE>(rd[r], d);
-            kept_values(rg[r], g);
-            kept_values(ru[r], u);
+            float g[8], u[8];
+            gradients(rd[r], rg[r], ru[r], g, u);
 #pragma unroll
-            for (int j = 0; j < 8; j++) most = fmaxf(most, finite_magnitude(d[j] * fmaxf(1.13f * fabsf(u[j]), fabsf(g[j]))));
+            for (int j = 0; j < 8; j++) most = fmaxf(most, fmaxf(finite_magnitude(g[j]), finite_magnitude(u[j])));
         }
         const int e = half_exponent(largest_of(most, part));
         const float up = power_of_two(e);
@@ -373,17 +385,10 @@ __global__ void __launch_bounds__(512) gate_grad_rows_kernel(const GateGradArgs 
         for (int r = 0; r < ROUNDS; r++) {
             const uint32_t n = (r * 512u + threadIdx.x) * 8u;
             if (n >= a.N) continue;
-            float d[8], g[8], u[8];
-            values_of<DTYPE>(rd[r], d);
-            kept_values(rg[r], g);
-            kept_values(ru[r], u);
+            float g[8], u[8];
+            gradients(rd[r], rg[r], ru[r], g, u);
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                float value, slope;
-                activation_and_slope(g[j], a.act, value, slope);
-                g[j] = d[j] * u[j] * slope * up;
-                u[j] = d[j] * value * up;
-            }
+            for (int j = 0; j < 8; j++) { g[j] *= up; u[j] *= up; }
             store8<EOQ_B200_F16>(a.half, (size_t)m * a.pitch + n, g);
             store8<EOQ_B200_F16>(a.half, ((size_t)a.M + m) * a.pitch + n, u);
         }

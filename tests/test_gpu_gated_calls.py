@@ -106,3 +106,38 @@ def test_scales_that_want_gradients(which, wants):
         assert torch.equal(gated.gated_packed(pg, sg, pu, su, n, k, 4, 128, x), want)
         dx = gated.packed_input_grad(pg, sg, n, k, 4, 128, want)
     assert torch.equal(gated.packed_input_grad(pg, sg.detach(), n, k, 4, 128, want), dx)
+
+
+@pytest.mark.parametrize("n", [61, 64, 8200, 16384])
+@pytest.mark.parametrize("form", ["full", "8bit"])
+def test_gradients_through_closed_gates(n, form):
+    """A row's gradients that meet closed gates alone, from what the forward pass has kept: eleven bits of each, whatever the width.
+    The slopes and values of silu down to -30 are some 2^-17 off in fp32 (the exponential 37 units, the division 2)."""
+    from eoq_quantization_b200 import _lib
+    k = 128
+    (pg, sg, wg), (pu, su, wu) = _layers(n, k, 4, 128, 1)
+    gates = torch.tensor([-2.0, -10.0, -15.0, -20.0, -25.0, -30.0], device="cuda")
+    m = len(gates)
+    u = _inputs(m, n, BF16, 2)
+    dh = torch.zeros(m, n, dtype=BF16, device="cuda")
+    at = torch.arange(m, device="cuda")
+    dh[at, 9 * at] = torch.tensor([1.0, -3.0, 2e-3, 5.0, 100.0, 7.0], dtype=BF16, device="cuda")
+    if form == "full":
+        kept = (gates[:, None].to(BF16).expand(m, n).contiguous(), u, None, None)
+        g, u = kept[0].double(), u.double()
+    else:
+        s = gated.store_8bit(u)
+        scale = (gates.abs() / 127)[:, None].expand(m, -(-n // 64)).contiguous()
+        kept = (torch.full((m, n), -127, dtype=torch.int8, device="cuda"), s.codes, scale, s.scales)
+        g, u = (-127 * scale[:, :1]).double().expand(m, n), s.dequantize(F32).double()
+    dx, dbg, dbu = _lib.native().gated_grad(pg, sg, pu, su, n, k, 4, 128, gated.ACTIVATIONS["silu"], dh, *kept, True, True, True, _lib.F32)
+    d, sig = dh.double(), torch.sigmoid(g)
+    dg, du = d * u * sig * (1 + g * (1 - sig)), d * g * sig
+    most = torch.maximum(dg.abs(), du.abs()).amax(1, keepdim=True) * 2.0 ** -38
+    eg, eu = ((2.0 ** -16 + 2.0 ** -11) * v.abs() + (d != 0) * most for v in (dg, du))
+    # (a bias's gradient has one term, or one beside zeros)
+    for got, v, e in ((dbg, dg, eg), (dbu, du, eu)):
+        assert ((got.double() - v.sum(0)).abs() <= e.sum(0) + 2.0 ** -23 * v.abs().sum(0)).all()
+    off = eg @ wg.abs() + eu @ wu.abs() + 2.0 ** -10.9 * (dg.abs() @ wg.abs() + du.abs() @ wu.abs())
+    want = dg @ wg + du @ wu
+    assert ((dx.double() - want).abs() <= off + 2.0 ** -8 * (want.abs() + off)).all()
