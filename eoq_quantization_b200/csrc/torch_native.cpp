@@ -459,7 +459,8 @@ PyObject *gated_packed(PyObject *, PyObject *const *a, Py_ssize_t n)
     if (n != 13) { PyErr_SetString(PyExc_TypeError, "gated_packed takes 13 arguments"); return nullptr; }
     GUARD_BEGIN
     const int64_t N = PyLong_AsLongLong(a[4]), K = PyLong_AsLongLong(a[5]), bits = PyLong_AsLongLong(a[6]), group = PyLong_AsLongLong(a[7]);
-    const int form = (int)PyLong_AsLong(a[12]);
+    const int activation = (int)PyLong_AsLong(a[11]), form = (int)PyLong_AsLong(a[12]);
+    if (PyErr_Occurred()) return nullptr;
     Activations act;
     Packed gate, up;
     Bias bias[2];
@@ -473,8 +474,7 @@ PyObject *gated_packed(PyObject *, PyObject *const *a, Py_ssize_t n)
     const Tensor &x = *act.x;
     const Ordered ordered(gate.converted || up.converted);
     const eoq_b200_gated_t w = {gate.codes, up.codes, gate.scales, up.scales, bias[0].p, bias[1].p, (uint32_t)N, (uint32_t)K, (uint32_t)bits, (uint32_t)group,
-                                (int)PyLong_AsLong(a[11]), dtype_code(bias_type)};
-    if (PyErr_Occurred()) return nullptr;
+                                activation, dtype_code(bias_type)};
     KeptTensors kept(form, x, act.rows, N);
     Tensor h = result(x, N, x.scalar_type()), scratch;
     if (const size_t bytes = eoq_b200_gated_scratch(&w, &kept.c, act.code, (uint32_t)act.rows)) scratch = bytes_beside(x, bytes);
@@ -499,6 +499,8 @@ PyObject *gated_grad(PyObject *, PyObject *const *a, Py_ssize_t n)
     if (n != 18) { PyErr_SetString(PyExc_TypeError, "gated_grad takes 18 arguments"); return nullptr; }
     GUARD_BEGIN
     const int64_t N = PyLong_AsLongLong(a[4]), K = PyLong_AsLongLong(a[5]), bits = PyLong_AsLongLong(a[6]), group = PyLong_AsLongLong(a[7]);
+    const int activation = (int)PyLong_AsLong(a[8]), type_of_bias = (int)PyLong_AsLong(a[17]);
+    if (PyErr_Occurred()) return nullptr;
     Activations act;
     Packed gate, up;
     if (!act.open(a[9], N) || !gate.open(a[0], a[1], *act.x, N, K, bits, group) || !up.open(a[2], a[3], *act.x, N, K, bits, group)) Py_RETURN_NONE;
@@ -517,7 +519,7 @@ PyObject *gated_grad(PyObject *, PyObject *const *a, Py_ssize_t n)
     }
     const Ordered ordered(gate.converted || up.converted);
     const eoq_b200_gated_t w = {gate.codes, up.codes, gate.scales, up.scales, nullptr, nullptr, (uint32_t)N, (uint32_t)K, (uint32_t)bits, (uint32_t)group,
-                                (int)PyLong_AsLong(a[8]), (int)PyLong_AsLong(a[17])};
+                                activation, type_of_bias};
     const at::ScalarType bias_type = w.bias_dtype == EOQ_B200_F16 ? at::kHalf : w.bias_dtype == EOQ_B200_BF16 ? at::kBFloat16 : at::kFloat;
     const bool want[3] = {PyObject_IsTrue(a[14]) == 1, PyObject_IsTrue(a[15]) == 1, PyObject_IsTrue(a[16]) == 1};
     if (PyErr_Occurred()) return nullptr;
@@ -544,6 +546,7 @@ PyObject *input_grad(PyObject *, PyObject *const *a, Py_ssize_t n)
     if (n != 7) { PyErr_SetString(PyExc_TypeError, "input_grad takes 7 arguments"); return nullptr; }
     GUARD_BEGIN
     const int64_t N = PyLong_AsLongLong(a[2]), K = PyLong_AsLongLong(a[3]), bits = PyLong_AsLongLong(a[4]), group = PyLong_AsLongLong(a[5]);
+    if (PyErr_Occurred()) return nullptr;
     Activations act;
     Packed w;
     if (!act.open(a[6], N) || !w.open(a[0], a[1], *act.x, N, K, bits, group)) Py_RETURN_NONE;
