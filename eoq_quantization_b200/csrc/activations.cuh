@@ -33,7 +33,7 @@ __device__ __forceinline__ void activation_and_slope(float g, int act, float &va
     } else {
         const float t = tanhf(0.79788456f * (g + 0.044715f * g * g * g)), p = 0.5f * (1.0f + t);
         value = g * p;
-        slope = p + g * 0.5f * (1.0f - t * t) * 0.79788456f * (1.0f + 0.134145f * g * g);
+        slope = p + g * 0.5f * (1.0f - t * t) * 0.79788456f * (1.0f + 0.134145f * fminf(g * g, 1e30f));      // (not zero times infinity)
     }
 }
 

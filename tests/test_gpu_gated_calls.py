@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from eoq_quantization_b200 import gated
-from gated_reference import weight
+from gated_reference import Gated, inside, weight
 
 pytestmark = pytest.mark.gpu
 F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
@@ -141,3 +141,16 @@ def test_gradients_through_closed_gates(n, form):
     off = eg @ wg.abs() + eu @ wu.abs() + 2.0 ** -10.9 * (dg.abs() @ wg.abs() + du.abs() @ wu.abs())
     want = dg @ wg + du @ wu
     assert ((dx.double() - want).abs() <= off + 2.0 ** -8 * (want.abs() + off)).all()
+
+
+@pytest.mark.parametrize("kind", list(gated.ACTIVATIONS))
+@pytest.mark.parametrize("m,n,dtype", [(4, 64, BF16), (40, 61, BF16), (3, 64, F32)])
+def test_gradients_of_huge_activations(kind, m, n, dtype):
+    """Gates whose squares are beyond fp32."""
+    k = 256
+    (pg, sg, wg), (pu, su, wu) = _layers(n, k, 4, 128, 1)
+    x, dh = _inputs(m, k, dtype, 2, 1e21).requires_grad_(), _inputs(m, n, dtype, 3, 1e-30)
+    dx, = torch.autograd.grad(gated.gated_packed(pg, sg, pu, su, n, k, 4, 128, x, activation=kind), x, dh)
+    (want, off), *_ = Gated(x.detach(), wg, wu, kind).gradients(dh, "full")
+    assert (Gated(x.detach(), wg, wu, kind).g.abs() > 1e20).any()
+    inside(dx, want, off, "dx")
