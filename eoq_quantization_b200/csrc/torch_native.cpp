@@ -389,6 +389,36 @@ PyObject *polar_linear(PyObject *, PyObject *const *a, Py_ssize_t n)
     GUARD_END
 }
 
+// dequant_packed(packed, scales or None, N, K, bits, group, row_lo, row_hi, type): rows of the dense weight, 0 fp16, 1 bf16, 2 fp32, or
+// 3 the codes.  A tensor of its own whatever watches the call: to a function transform or a recording it is a constant.  (Of
+// torch.empty a transform makes a tensor without memory, and a recording a step that leaves anything.)
+PyObject *dequant_packed(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    if (n != 9) { PyErr_SetString(PyExc_TypeError, "dequant_packed takes 9 arguments"); return nullptr; }
+    GUARD_BEGIN
+    int64_t v[7];
+    for (int i = 0; i < 7; i++) v[i] = PyLong_AsLongLong(a[2 + i]);
+    if (PyErr_Occurred()) return nullptr;
+    const int64_t K = v[1], lo = v[4], hi = v[5];
+    const int type = (int)v[6];
+    const Tensor *pk = tensor_of(a[0]);
+    for (int i = 0; i < 6; i++) if (v[i] < 0 || v[i] > 0x7fffffff) Py_RETURN_NONE;
+    if (!pk || !pk->is_cuda() || pk->layout() != at::kStrided || kind_of(*pk) != kPlain || lo > hi || type < 0 || type > EOQ_B200_I8) Py_RETURN_NONE;
+    const c10::impl::ExcludeDispatchKeyGuard alone(c10::DispatchKeySet({c10::DispatchKey::FuncTorchDynamicLayerFrontMode, c10::DispatchKey::FuncTorchDynamicLayerBackMode,
+        c10::DispatchKey::FuncTorchVmapMode, c10::DispatchKey::VmapMode, c10::DispatchKey::Tracer, c10::DispatchKey::Python, c10::DispatchKey::PythonTLSSnapshot}));
+    at::AutoDispatchBelowADInplaceOrView below;
+    const c10::cuda::CUDAGuard guard(pk->device());
+    Parameter sc;
+    if (a[1] != Py_None && !sc.open(a[1], *pk, at::kHalf)) Py_RETURN_NONE;
+    const Tensor codes = pk->contiguous();
+    Tensor dense = at::detail::empty_cuda({hi - lo, K}, type == EOQ_B200_F16 ? at::kHalf : type == EOQ_B200_BF16 ? at::kBFloat16 : type == EOQ_B200_F32 ? at::kFloat : at::kChar,
+                                          pk->device(), std::nullopt);
+    return done(eoq_b200_dequant_packed(static_cast<const uint8_t *>(codes.data_ptr()), sc.t ? static_cast<const uint16_t *>(sc.t->data_ptr()) : nullptr, (uint32_t)v[0],
+                                        (uint32_t)K, (uint32_t)v[2], (uint32_t)v[3], (uint32_t)lo, (uint32_t)hi, dense.data_ptr(), type, stream_of(*pk)),
+                std::move(dense), "eoq_b200_dequant_packed");
+    GUARD_END
+}
+
 // -- the gated block on packed weights ------------------------------------------
 
 // A packed weight beside x: codes in the layout of `bits`, copied where they are strided, scales that cover the flattened matrix,
@@ -826,6 +856,7 @@ PyMethodDef methods[] = {
     {"weight_linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(weight_linear)), METH_FASTCALL, nullptr},
     {"packed_linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(packed_linear)), METH_FASTCALL, nullptr},
     {"polar_linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(polar_linear)), METH_FASTCALL, nullptr},
+    {"dequant_packed", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(dequant_packed)), METH_FASTCALL, nullptr},
     {"gated_packed", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(gated_packed)), METH_FASTCALL, nullptr},
     {"gated_grad", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(gated_grad)), METH_FASTCALL, nullptr},
     {"input_grad", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(input_grad)), METH_FASTCALL, nullptr},

@@ -354,10 +354,13 @@ def dequant_packed(packed: torch.Tensor, scales: torch.Tensor, rows: int, cols: 
     dtype torch.int8 the signed codes themselves (scales may then be None)."""
     require_cuda(packed, "dequant_packed")
     row_hi = rows if row_hi is None else row_hi
+    code = _I8 if dtype == torch.int8 else _DTYPES[dtype]
+    out = _lib.native().dequant_packed(packed, scales, rows, cols, bits, group, row_lo, row_hi, code)
+    if out is not None:
+        return out
     pk = packed.contiguous()
     sc = None if scales is None else scales.to(device=packed.device, dtype=torch.float16).contiguous()
     out = torch.empty((row_hi - row_lo, cols), dtype=dtype, device=packed.device)
-    code = _I8 if dtype == torch.int8 else _DTYPES[dtype]
     with torch.cuda.device(packed.device):
         _lib.check(_lib.lib().eoq_b200_dequant_packed(pk.data_ptr(), sc.data_ptr() if sc is not None else None, rows, cols, bits, group,
                                                       row_lo, row_hi, out.data_ptr(), code, _stream_ptr()), "eoq_b200_dequant_packed")

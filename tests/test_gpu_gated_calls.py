@@ -154,3 +154,40 @@ def test_gradients_of_huge_activations(kind, m, n, dtype):
     (want, off), *_ = Gated(x.detach(), wg, wu, kind).gradients(dh, "full")
     assert (Gated(x.detach(), wg, wu, kind).g.abs() > 1e20).any()
     inside(dx, want, off, "dx")
+
+
+def _module(saved="full"):
+    torch.manual_seed(1)
+    return gated.QuantizedGatedMLP.from_float(*(torch.nn.Linear(*s).cuda() for s in ((256, 320), (256, 320), (320, 256))), block_size=64, saved=saved)
+
+
+def _dense(layer):
+    return layer._dequantize_weight().double()
+
+
+def _exact_module(mlp, x):
+    """The module in 64 bits, in torch's own operations."""
+    f = lambda layer, t: t @ _dense(layer).T + layer.bias_param.double()  # noqa: E731
+    return f(mlp.down, torch.nn.functional.silu(f(mlp.gate, x)) * f(mlp.up, x))
+
+
+@pytest.mark.parametrize("m", [1, 40])
+@pytest.mark.parametrize("which", ["layer", "block"])
+def test_function_transforms_and_recordings(m, which):
+    """torch.func's derivatives and torch.jit.trace of the block and of a layer alone, fp32: ten roundings and sums of 320 terms at most."""
+    mlp = _module()
+    f, exact = (mlp, lambda t: _exact_module(mlp, t)) if which == "block" else \
+        (mlp.gate, lambda t: t @ _dense(mlp.gate).T + mlp.gate.bias_param.double())
+    x, v = _inputs(m, 256, F32, 2), _inputs(m, 256, F32, 3)
+    near = lambda a, b: (a.double() - b).norm() <= (10 * 2.0 ** -24 + 320 * 2.0 ** -23) * b.norm()  # noqa: E731
+    leaf = x.double().requires_grad_()
+    want, = torch.autograd.grad(exact(leaf).square().sum(), leaf)
+    assert near(torch.func.grad(lambda t: f(t).square().sum())(x), want)
+    _, tangent = torch.func.jvp(f, (x,), (v,))
+    assert near(tangent, torch.func.jvp(exact, (x.double(),), (v.double(),))[1])
+    assert near(torch.func.jacrev(f)(x[:1]), torch.func.jacrev(exact)(x[:1].double()))
+    assert near(torch.func.vmap(torch.func.grad(lambda t: f(t).square().sum()))(x), want)
+    traced = torch.jit.trace(f, (x,))
+    for _ in range(3):
+        torch.full((320, 256), float("nan"), device="cuda")         # what memory may hold that nobody has written
+        assert near(traced(v), exact(v.double()))
