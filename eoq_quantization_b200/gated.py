@@ -22,6 +22,8 @@ ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
 KEEP = {"none": 0, "full": 1, "8bit": 2}
 STORE_BLOCK = 64                        # values of a row that share a scale in 8-bit storage
 _TYPES = {0: torch.float16, 1: torch.bfloat16, 2: torch.float32}
+# torch's own operations, for calls that something watches: the activations, and their gradients (of what follows, at g)
+_TORCH_BACKWARD = {0: torch.ops.aten.silu_backward, 1: torch.ops.aten.gelu_backward, 2: lambda d, g: torch.ops.aten.gelu_backward(d, g, approximate="tanh")}
 _TORCH_ACTIVATIONS = {"silu": F.silu, "gelu": F.gelu, "gelu_tanh": lambda g: F.gelu(g, approximate="tanh")}
 
 
@@ -75,18 +77,34 @@ class _Gated(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dh):
         gate, gate_scales, up, up_scales, *kept = ctx.saved_tensors          # an error if the weights have been written since
+        if call_kind(dh) == WATCHED:             # several gradients at once (is_grads_batched)
+            with _without_autocast():
+                return _Gated._backward_watched(ctx, dh, gate, gate_scales, up, up_scales, kept)
         if ctx.form == KEEP["full"]:
             kept += [None, None]
         types = {t for t in ctx.bias_dtypes if t is not None}          # of one type: written in it; else cast below
         bias_type = _DTYPES.get(next(iter(types)), _lib.F32) if len(types) == 1 else _lib.F32
         with _without_autocast():
-            out = _lib.native().gated_grad(gate, gate_scales, up, up_scales, *ctx.shape, ctx.activation, dh.detach(), *kept, *ctx.needs_input_grad[:3], bias_type)
+            out = _lib.native().gated_grad(gate, gate_scales, up, up_scales, *ctx.shape, ctx.activation, dh, *kept, *ctx.needs_input_grad[:3], bias_type)
         if out is None:
             raise RuntimeError("gated_packed: the backward pass is not supported")
         dx, *db = out
         dx = None if dx is None else dx.view(ctx.x_shape)
         db = [b if b is None or b.dtype == t else b.to(t) for b, t in zip(db, ctx.bias_dtypes)]
         return (dx, *db) + (None,) * 7
+
+    @staticmethod
+    def _backward_watched(ctx, dh, gate, gate_scales, up, up_scales, kept):
+        g, u = (v.float() for v in kept[:2])
+        if ctx.form == KEEP["8bit"]:
+            g, u = (v * s.repeat_interleave(STORE_BLOCK, 1)[:, :v.shape[1]] for v, s in ((g, kept[2]), (u, kept[3])))
+        d = dh.reshape(g.shape).float()
+        value = list(_TORCH_ACTIVATIONS.values())[ctx.activation](g)
+        dg, du = _TORCH_BACKWARD[ctx.activation](d * u, g), d * value
+        dx = None
+        if ctx.needs_input_grad[0]:
+            dx = (dg @ dequant_packed(gate, gate_scales, *ctx.shape) + du @ dequant_packed(up, up_scales, *ctx.shape)).to(dh.dtype).reshape(ctx.x_shape)
+        return (dx, *(v.sum(0).to(t) if wanted else None for v, t, wanted in zip((dg, du), ctx.bias_dtypes, ctx.needs_input_grad[1:3]))) + (None,) * 7
 
 
 class _InputGradProduct(torch.autograd.Function):
@@ -104,7 +122,9 @@ class _InputGradProduct(torch.autograd.Function):
     def backward(ctx, dy):
         packed, scales = ctx.saved_tensors
         with _without_autocast():
-            dx = packed_input_grad(packed, scales, *ctx.shape, dy.detach()) if ctx.needs_input_grad[0] else None
+            dx = None
+            if ctx.needs_input_grad[0]:
+                dx = packed_input_grad(packed, scales, *ctx.shape, dy) if call_kind(dy) != WATCHED else dy @ dequant_packed(packed, scales, *ctx.shape).to(dy.dtype)
             db = dy.reshape(-1, dy.shape[-1]).sum(0).to(ctx.bias_dtype) if ctx.needs_input_grad[1] else None
         return dx, db, None, None, None
 

@@ -191,3 +191,30 @@ def test_function_transforms_and_recordings(m, which):
     for _ in range(3):
         torch.full((320, 256), float("nan"), device="cuda")         # what memory may hold that nobody has written
         assert near(traced(v), exact(v.double()))
+
+
+@pytest.mark.parametrize("kind", list(gated.ACTIVATIONS))
+@pytest.mark.parametrize("saved", ["full", "8bit"])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_several_gradients_at_once(kind, saved, dtype):
+    """``is_grads_batched`` and what uses it: each gradient as by itself."""
+    n, k, m = 130, 256, 6
+    (pg, sg, wg), (pu, su, wu) = _layers(n, k, 4, 128, 1)
+    leaves = [_inputs(m, k, dtype, 2).view(2, 3, k), _inputs(1, n, F32, 3)[0], _inputs(1, n, dtype, 4)[0]]
+    want = Gated(leaves[0].view(m, k), wg, wu, kind, *leaves[1:])
+    leaves = [t.requires_grad_() for t in leaves]
+    h = gated.gated_packed(pg, sg, pu, su, n, k, 4, 128, *leaves, activation=kind, saved=saved)
+    dhs = torch.stack([_inputs(m, n, dtype, 5 + i).view(2, 3, n) for i in range(3)])
+    got = torch.autograd.grad(h, leaves, dhs, is_grads_batched=True)
+    for i, dh in enumerate(dhs):
+        (v, e), *db = want.gradients(dh.view(m, n), saved)
+        inside(got[0][i].reshape(m, k), v, e, f"dx {i}")
+        for t, (v, e) in zip(got[1:], db):
+            inside(t[i], v, e + torch.finfo(t.dtype).eps / 2 * (v.abs() + e), f"bias {i}")
+
+
+def test_jacobian_of_the_module():
+    mlp, x = _module(), _inputs(2, 256, F32, 2)
+    whole = torch.autograd.functional.jacobian(mlp, x, vectorize=True)
+    rows = torch.autograd.functional.jacobian(mlp, x)
+    assert (whole - rows).norm() <= 2.0 ** -16 * rows.norm()
