@@ -218,3 +218,21 @@ def test_jacobian_of_the_module():
     whole = torch.autograd.functional.jacobian(mlp, x, vectorize=True)
     rows = torch.autograd.functional.jacobian(mlp, x)
     assert (whole - rows).norm() <= 2.0 ** -16 * rows.norm()
+
+
+@pytest.mark.parametrize("bits", [3, 5, 6, 7])
+@pytest.mark.parametrize("m,n,k,group,dtype", [(1, 200, 256, 32, F16), (7, 96, 384, 96, BF16), (20, 130, 512, 128, F16), (33, 65, 320, 64, BF16),
+                                               (280, 200, 256, 32, F16), (5, 70, 256, 64, F32)])
+def test_other_widths(bits, m, n, k, group, dtype):
+    """One code a byte, at the tensor cores."""
+    (pg, sg, wg), (pu, su, wu) = _layers(n, k, bits, group, 1)
+    x, dh = _inputs(m, k, dtype, 2).requires_grad_(), _inputs(m, n, dtype, 3, 1e-3)
+    want = Gated(x.detach(), wg, wu, "gelu")
+    h = gated.gated_packed(pg, sg, pu, su, n, k, bits, group, x, activation="gelu", saved="8bit")
+    inside(h.detach(), want.h, want.h_bound(), "h")
+    inside(gated.gated_packed(pg, sg, pu, su, n, k, bits, group, x.detach(), activation="gelu"), want.h, want.h_bound(), "h")
+    (v, e), *_ = want.gradients(dh, "8bit")
+    inside(torch.autograd.grad(h, x, dh)[0], v, e, "dx")
+    d, half = dh.double(), torch.finfo(dtype).eps / 2
+    off = ((0 if dtype == F32 else 2.0 ** -11) + n * 2.0 ** -23 + 2.0 ** -37) * (d.abs() @ wg.abs())
+    inside(gated.packed_input_grad(pg, sg, n, k, bits, group, dh), d @ wg, off + half * ((d @ wg).abs() + off) + 2.0 ** -25, "dy W")
