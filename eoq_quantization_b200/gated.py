@@ -21,7 +21,6 @@ from .fused import _DTYPES, GRADIENT, WATCHED, autocast_dtype, call_kind, dequan
 ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
 KEEP = {"none": 0, "full": 1, "8bit": 2}
 STORE_BLOCK = 64                        # values of a row that share a scale in 8-bit storage
-_TYPES = {0: torch.float16, 1: torch.bfloat16, 2: torch.float32}
 # torch's own operations, for calls that something watches: the activations, and their gradients (of what follows, at g)
 _TORCH_BACKWARD = {0: torch.ops.aten.silu_backward, 1: torch.ops.aten.gelu_backward, 2: lambda d, g: torch.ops.aten.gelu_backward(d, g, approximate="tanh")}
 _TORCH_ACTIVATIONS = {"silu": F.silu, "gelu": F.gelu, "gelu_tanh": lambda g: F.gelu(g, approximate="tanh")}
@@ -60,6 +59,18 @@ def _without_autocast():
     return torch.autocast("cuda", enabled=False) if torch.is_autocast_enabled("cuda") else nullcontext()
 
 
+class _Once(torch.autograd.Function):
+    """A gradient that depends on what it was taken at, which nobody can differentiate again: an error instead of a zero."""
+
+    @staticmethod
+    def forward(ctx, value, wanted):
+        return value.view_as(value)
+
+    @staticmethod
+    def backward(ctx, _):
+        raise RuntimeError("gated_packed: differentiable once; there are no second derivatives")
+
+
 class _Gated(torch.autograd.Function):
     """h, and from what the forward pass kept of gate and up the gradients of x and the biases."""
 
@@ -74,12 +85,19 @@ class _Gated(torch.autograd.Function):
         return out[0]
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dh):
+        with torch.no_grad():
+            gradients = _Gated._gradients(ctx, dh)
+        if torch.is_grad_enabled():              # create_graph
+            gradients = [None if v is None else _Once.apply(v, torch.zeros((), requires_grad=True)) for v in gradients]
+        return (*gradients,) + (None,) * 7
+
+    @staticmethod
+    def _gradients(ctx, dh):
         gate, gate_scales, up, up_scales, *kept = ctx.saved_tensors          # an error if the weights have been written since
         if call_kind(dh) == WATCHED:             # several gradients at once (is_grads_batched)
             with _without_autocast():
-                return _Gated._backward_watched(ctx, dh, gate, gate_scales, up, up_scales, kept)
+                return _Gated._watched_gradients(ctx, dh, gate, gate_scales, up, up_scales, kept)
         if ctx.form == KEEP["full"]:
             kept += [None, None]
         types = {t for t in ctx.bias_dtypes if t is not None}          # of one type: written in it; else cast below
@@ -91,10 +109,10 @@ class _Gated(torch.autograd.Function):
         dx, *db = out
         dx = None if dx is None else dx.view(ctx.x_shape)
         db = [b if b is None or b.dtype == t else b.to(t) for b, t in zip(db, ctx.bias_dtypes)]
-        return (dx, *db) + (None,) * 7
+        return dx, *db
 
     @staticmethod
-    def _backward_watched(ctx, dh, gate, gate_scales, up, up_scales, kept):
+    def _watched_gradients(ctx, dh, gate, gate_scales, up, up_scales, kept):
         g, u = (v.float() for v in kept[:2])
         if ctx.form == KEEP["8bit"]:
             g, u = (v * s.repeat_interleave(STORE_BLOCK, 1)[:, :v.shape[1]] for v, s in ((g, kept[2]), (u, kept[3])))
@@ -104,7 +122,7 @@ class _Gated(torch.autograd.Function):
         dx = None
         if ctx.needs_input_grad[0]:
             dx = (dg @ dequant_packed(gate, gate_scales, *ctx.shape) + du @ dequant_packed(up, up_scales, *ctx.shape)).to(dh.dtype).reshape(ctx.x_shape)
-        return (dx, *(v.sum(0).to(t) if wanted else None for v, t, wanted in zip((dg, du), ctx.bias_dtypes, ctx.needs_input_grad[1:3]))) + (None,) * 7
+        return dx, *(v.sum(0).to(t) if wanted else None for v, t, wanted in zip((dg, du), ctx.bias_dtypes, ctx.needs_input_grad[1:3]))
 
 
 class _InputGradProduct(torch.autograd.Function):

@@ -236,3 +236,23 @@ def test_other_widths(bits, m, n, k, group, dtype):
     d, half = dh.double(), torch.finfo(dtype).eps / 2
     off = ((0 if dtype == F32 else 2.0 ** -11) + n * 2.0 ** -23 + 2.0 ** -37) * (d.abs() @ wg.abs())
     inside(gated.packed_input_grad(pg, sg, n, k, bits, group, dh), d @ wg, off + half * ((d @ wg).abs() + off) + 2.0 ** -25, "dy W")
+
+
+@pytest.mark.parametrize("what", ["block", "module"])
+def test_second_derivatives_are_errors(what):
+    """Also where the gradient of the result is a constant: the block's own depends on its activations."""
+    n, k = 320, 256
+    (pg, sg, _), (pu, su, _) = _layers(n, k, 4, 128, 1)
+    call = _module() if what == "module" else lambda t: gated.gated_packed(pg, sg, pu, su, n, k, 4, 128, t)
+    x = _inputs(12, k, F32, 2).requires_grad_()
+    plain, = torch.autograd.grad(call(x).sum(), x)
+    for loss in (lambda y: y.sum(), lambda y: y.square().sum()):
+        dx, = torch.autograd.grad(loss(call(x)), x, create_graph=True)
+        assert dx.requires_grad
+        with pytest.raises(RuntimeError):
+            (dx.square().sum() + x.sum()).backward()
+    dx, = torch.autograd.grad(call(x).sum(), x, create_graph=True)
+    assert torch.equal(dx.detach(), plain) and not plain.requires_grad
+    x.grad = None
+    call(x).sum().backward()
+    assert torch.equal(x.grad, plain) and not x.grad.requires_grad
