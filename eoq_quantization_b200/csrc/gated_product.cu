@@ -60,11 +60,13 @@ struct ProductArgs {
     const uint16_t *scales[2];   // [N][groups] fp16
     const void *bias[2];         // forward: [N] of bias_dtype, or null
     const float *factor;         // [M] or null
+    const uint8_t *codes[2];     // [N][row_bytes]
+    const uint16_t *x;           // fp16 [M][pitch] or, gradient, [weights][M][pitch]
     void *y;                     // [M][N] or, gradient, [M][K]
     Kept keep;                   // forward
     float *partial;              // [pairs][2][2][T][128]: sums of tiles that a pair's run begins (0) or ends (1) in the middle of
     uint32_t *count;             // [tiles][2], zero: parts of a tile that have arrived
-    uint32_t N, K, M, T, group, groups;
+    uint32_t N, K, M, T, group, groups, row_bytes, pitch;
     uint32_t tok_tiles, tiles, per_tile, per_weight, unit;         // of the grid of tiles; pieces of a tile's axis, of one weight's
     uint32_t nw, ns, nd;         // stages of packed weights and of operands, accumulators
     uint32_t at_x, at_out, at_bar;       // shared-memory offsets
@@ -223,9 +225,83 @@ __device__ __forceinline__ uint32_t place(uint32_t q, uint32_t p)
     return q * 32u + (p >> 4) * 16u + 2u * (p & 7u) + ((p >> 3) & 1u);
 }
 
+// Eight codes, BITS bytes, that lie together.
+template <int BITS>
+__device__ __forceinline__ void eight_codes(const uint8_t *from, float (&c)[8])
+{
+    if (BITS == 8) {
+        const uint2 w = __ldg(reinterpret_cast<const uint2 *>(from));
+#pragma unroll
+        for (int i = 0; i < 8; i++) c[i] = (float)(int8_t)((i < 4 ? w.x : w.y) >> (8 * (i & 3)));
+    } else {
+        const uint32_t w = BITS == 4 ? __ldg(reinterpret_cast<const uint32_t *>(from)) : __ldg(reinterpret_cast<const uint16_t *>(from));
+#pragma unroll
+        for (int i = 0; i < 8; i++) c[i] = (float)((int)((w >> (BITS * i)) & ((1u << BITS) - 1u)) - ((1 << (BITS - 1)) - 1));
+    }
+}
+
+// Sums of sixteen tokens again, in fp32 throughout, for weights that fp16 has no room for (beyond 65504, which takes scales above 511 for
+// byte codes, 8188 for four bits).  forward: of row n of a weight; gradient: of column n of all weights.
+template <bool GRAD, int BITS>
+__device__ __noinline__ void sums_in_fp32(const ProductArgs &a, uint32_t which, uint32_t n, uint32_t token, float (&v)[16])
+{
+#pragma unroll
+    for (int j = 0; j < 16; j++) v[j] = 0.0f;
+    auto add = [&](const uint16_t *x, const float (&w)[8]) {       // eight terms of each token
+#pragma unroll
+        for (uint32_t j = 0; j < 16; j++) {
+            const uint4 q = __ldg(reinterpret_cast<const uint4 *>(x + (size_t)min(token + j, a.M - 1u) * a.pitch));
+            const uint32_t p[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&p[i]));
+                v[j] = fmaf(w[2 * i + 1], f.y, fmaf(w[2 * i], f.x, v[j]));
+            }
+        }
+    };
+    if constexpr (!GRAD) {
+        for (uint32_t k = 0; k < a.K; k += 8u) {
+            float w[8];
+            eight_codes<BITS>(a.codes[which] + (size_t)n * a.row_bytes + k / 8u * BITS, w);
+            const float s = __half2float(__ushort_as_half(__ldg(a.scales[which] + (size_t)n * a.groups + k / a.group)));
+#pragma unroll
+            for (int i = 0; i < 8; i++) w[i] *= s;
+            add(a.x + k, w);
+        }
+    } else {
+        for (uint32_t weight = 0; weight * a.per_weight < a.per_tile; weight++)
+            for (uint32_t r = 0; r < a.N; r += 8u) {
+                float w[8];
+#pragma unroll
+                for (uint32_t i = 0; i < 8; i++) {
+                    w[i] = 0.0f;
+                    if (r + i >= a.N) continue;
+                    float c[8];
+                    eight_codes<BITS>(a.codes[weight] + (size_t)(r + i) * a.row_bytes + n / 8u * BITS, c);
+#pragma unroll
+                    for (uint32_t j = 0; j < 8; j++) if (j == n % 8u) w[i] = c[j];
+                    w[i] *= __half2float(__ushort_as_half(__ldg(a.scales[weight] + (size_t)(r + i) * a.groups + n / a.group)));
+                }
+                add(a.x + (size_t)weight * a.M * a.pitch + r, w);
+            }
+    }
+}
+
+// Whether a scale of weights [w0, w1), of rows r0, r0 + step .. before r1 and groups [g0, g1), is such that a code times it may be beyond fp16.
+template <int BITS>
+__device__ __noinline__ bool beyond_fp16(const ProductArgs &a, uint32_t w0, uint32_t w1, uint32_t r0, uint32_t r1, uint32_t step, uint32_t g0, uint32_t g1)
+{
+    constexpr uint32_t kMost = BITS == 8 ? 0x5FFFu : BITS == 4 ? 0x6FFFu : 0x77FFu;        // 65504 / 128, / 8, / 2
+    bool yes = false;
+    for (uint32_t w = w0; w < w1; w++)
+        for (uint32_t r = r0; r < r1; r += step)
+            for (uint32_t g = g0; g < g1; g++) yes |= (__ldg(a.scales[w] + (size_t)r * a.groups + g) & 0x7FFFu) > kMost;
+    return yes;
+}
+
 template <bool GRAD, int BITS>
 __global__ void __launch_bounds__(kThreads, 1)
-gated_product_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap gmap, const __grid_constant__ CUtensorMap umap, const __grid_constant__ CUtensorMap xmap)
+gated_product_kernel(const __grid_constant__ ProductArgs a, const __grid_constant__ CUtensorMap gmap, const __grid_constant__ CUtensorMap umap, const __grid_constant__ CUtensorMap xmap)
 {
     using P = Piece<GRAD, BITS>;
     extern __shared__ uint8_t raw[];
@@ -532,6 +608,13 @@ gated_product_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap gm
             }
         };
         uint32_t turn = 0;                                       // buffers of the exchange alternate
+        float spoilt = 0.0f;                                     // NaN once a sum of this tile is not finite
+        auto look_at = [&](const float (&v)[16]) {
+            uint64_t s = pack2(v[0], v[1]);
+#pragma unroll
+            for (int j = 2; j < 16; j += 2) s = add2(s, pack2(v[j], v[j + 1]));
+            spoilt = fmaf(low2(s) + high2(s), 0.0f, spoilt);
+        };
         // a tile, its rows' sums of sixteen tokens from `take`; `behind` is called when the last have been taken
         auto finish = [&](uint32_t tile, auto &&take, auto &&behind) {
             const uint32_t row0 = first_row(tile), tok0 = first_token(tile), tokens = min(a.T, a.M - tok0);
@@ -542,6 +625,7 @@ gated_product_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap gm
                     take(t0, v);
                     if (t0 + 16u >= a.T) behind();
                     if (t0 >= tokens || k >= a.K) continue;
+                    look_at(v);
                     if (a.factor) {
 #pragma unroll
                         for (uint32_t j = 0; j < 16; j++) v[j] *= __ldg(a.factor + min(tok0 + t0 + j, a.M - 1u));
@@ -568,6 +652,8 @@ gated_product_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap gm
                     for (uint32_t j = 0; j < 16; j++) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(u[j]) : "r"(other + j * 128u));
                     const uint32_t t = gate ? t0 : t0 + 16u;
                     const bool work = gate || two;
+                    look_at(g);
+                    look_at(u);
                     if (!gate) {
 #pragma unroll
                         for (uint32_t j = 0; j < 16; j++) { const float v = g[j]; g[j] = u[j]; u[j] = v; }
@@ -626,6 +712,27 @@ gated_product_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap gm
                 }
             }
         };
+        auto any_of_all = [&](bool yes) {                        // of the four warps
+            uint32_t r;
+            asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 5, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(r) : "r"((uint32_t)yes) : "memory");
+            return r != 0;
+        };
+        // a tile with sums that are not finite, and weights that may be why
+        auto made_good = [&](uint32_t tile) {
+            const bool yes = any_of_all(spoilt != 0.0f && !wait.lost);
+            spoilt = 0.0f;
+            const uint32_t first = first_row(tile), which = GRAD ? 0u : q >> 1, n = GRAD ? min(first + row, a.K - 1u) : min(first + (q & 1u) * 32u + lane, a.N - 1u);
+            if (!yes) return;
+            const bool mine = GRAD ? beyond_fp16<BITS>(a, 0u, a.per_tile / a.per_weight, tid, a.N, 128u, min(first, a.K - 1u) / a.group, min(first + 127u, a.K - 1u) / a.group + 1u)
+                                   : beyond_fp16<BITS>(a, which, which + 1u, n, n + 1u, 1u, 0u, a.groups);
+            if (!any_of_all(mine)) return;
+            finish(tile, [&](uint32_t t, float (&v)[16]) {
+#pragma unroll
+                for (int j = 0; j < 16; j++) v[j] = 0.0f;
+                if (t < a.T) sums_in_fp32<GRAD, BITS>(a, which, n, first_token(tile) + t, v);
+            }, [] {});
+            spoilt = 0.0f;
+        };
         auto partial_of = [&](uint32_t p, uint32_t begins) { return a.partial + ((size_t)(p * 2u + begins) * 2u + rank) * a.T * kRows + q * 32u + lane; };
         Ring dr;
         for (uint64_t at = head, left = run1 - run0; left; dr.next(a.nd)) {
@@ -648,6 +755,7 @@ gated_product_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap gm
             };
             if (s.p1 - s.p0 == a.per_tile) {
                 finish(s.tile, take, release);
+                made_good(s.tile);
                 continue;
             }
             // the tile's other parts are other pairs': the last to arrive adds them up, in the order of the pairs, its own (the same bits)
@@ -692,6 +800,7 @@ gated_product_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap gm
                     for (int j = 0; j < 16; j++) v[j] += o[j];
                 }
             }, [&]() { if (here) release(); });
+            made_good(s.tile);
         }
     }
     __syncwarp();
@@ -803,6 +912,8 @@ int run(ProductArgs a, const PackedPair &w, int nw, const void *x, uint32_t pitc
     a.nw = l.nw; a.ns = l.ns; a.nd = l.nd; a.at_x = l.at_x; a.at_out = l.at_out; a.at_bar = l.at_bar;
     a.count = static_cast<uint32_t *>(scratch);
     a.partial = reinterpret_cast<float *>(static_cast<uint8_t *>(scratch) + count_bytes(p));
+    a.x = static_cast<const uint16_t *>(x);
+    a.pitch = pitch;
     CUtensorMap maps[2], xmap;
     constexpr CUtensorMapSwizzle sw = P::kBytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : P::kBytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B;
     for (int i = 0; i < 2; i++)
@@ -829,7 +940,8 @@ int run(ProductArgs a, const PackedPair &w, int nw, const void *x, uint32_t pitc
 ProductArgs common(const PackedPair &w, const float *factor, uint32_t M, void *y, int dtype)
 {
     ProductArgs a = {};
-    a.scales[0] = w.scales[0]; a.scales[1] = w.scales[1];
+    for (int i = 0; i < 2; i++) { a.scales[i] = w.scales[i]; a.codes[i] = w.codes[i]; }
+    a.row_bytes = w.row_bytes;
     a.factor = factor; a.y = y; a.N = w.N; a.K = w.K; a.M = M; a.group = w.group; a.groups = w.K / w.group; a.dtype = dtype;
     a.inverse = (uint32_t)(((1ull << 32) + w.group / 16u - 1) / (w.group / 16u));
     a.limit = g_limit.load(std::memory_order_relaxed);

@@ -563,7 +563,8 @@ typedef struct eoq_b200_kept {
  * Up to 24 rows of 16-bit activations (32, where a weight has no more than 50 Mi values), codes and activations are exact there and
  * scales apply to the sums.  Beyond, activations go in as
  * fp16, bf16 ones times a power of two per row, which is exact for all but what is 2^-24 below the row's largest, and code x scale is
- * rounded to fp16 once.  Asynchronous. */
+ * rounded to fp16 once (tiles of weights that fp16 has no room for, beyond 65504, are computed again in fp32, slowly; so are the
+ * gradients' below).  Asynchronous. */
 size_t eoq_b200_gated_scratch(const eoq_b200_gated_t *w, const eoq_b200_kept_t *kept, int dtype, uint32_t batch);
 eoq_error_t eoq_b200_gated_packed(const eoq_b200_gated_t *w, const void *x, int dtype, uint32_t batch, void *d_scratch, void *h,
                                   const eoq_b200_kept_t *kept, void *stream);

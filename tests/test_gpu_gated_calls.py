@@ -256,3 +256,40 @@ def test_second_derivatives_are_errors(what):
     x.grad = None
     call(x).sum().backward()
     assert torch.equal(x.grad, plain) and not x.grad.requires_grad
+
+
+def _loud(n, k, bits, group, seed):
+    """A weight a hundredth of whose groups are beyond fp16 (some of their codes)."""
+    packed, scales, dense = weight(n, k, bits, group, seed)
+    codes = torch.round(dense.view(-1, group) / scales.double()[:, None])
+    qmax = (1 << (bits - 1)) - 1
+    loud = torch.rand(len(scales), generator=torch.Generator().manual_seed(seed + 7)) < 0.01
+    assert loud.any()
+    scales = torch.where(loud.cuda(), torch.tensor(3 * 65504.0 / qmax if bits > 2 else 60000.0).to(F16).cuda(), scales)
+    return packed, scales, (codes * scales.double()[:, None]).view(n, k)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("m,n,k,group", [(3, 130, 512, 128), (20, 130, 512, 64), (40, 130, 4096, 128), (300, 257, 320, 32), (150, 11000, 512, 64), (520, 64, 256, 128)])
+def test_weights_beyond_fp16(bits, m, n, k, group):
+    """Codes times scales above 65504, which bf16 and fp32 results have room for: right with any number of rows, by whichever kernel."""
+    (pg, sg, wg), (pu, su, wu) = _loud(n, k, bits, group, 1), _loud(n, k, bits, group, 2)
+    assert wg.abs().max() > 65504
+    x, dh = _inputs(m, k, BF16, 3, 1e-4).requires_grad_(), _inputs(m, n, BF16, 4, 1e-3)
+    x.data[0, 0] = float("inf")                # one row is not finite, and that stays
+    rest = slice(1, m)
+    for saved in ("full", "8bit"):
+        want = Gated(x.detach()[rest], wg, wu, "silu")
+        h = gated.gated_packed(pg, sg, pu, su, n, k, bits, group, x, saved=saved)
+        dx, = torch.autograd.grad(h, x, dh)
+        inside(h.detach()[rest], want.h, want.h_bound(), "h")
+        (v, e), *_ = want.gradients(dh[rest], saved)
+        inside(dx[rest], v, e, "dx")
+        assert not h[0].isfinite().any()
+    d = dh.double()
+    off = (2.0 ** -11 + n * 2.0 ** -23 + 2.0 ** -37) * (d.abs() @ wg.abs())
+    inside(gated.packed_input_grad(pg, sg, n, k, bits, group, dh), d @ wg, off + 2.0 ** -8 * ((d @ wg).abs() + off), "dy W")
+    half = _inputs(m, n, F16, 5, 1e-5)
+    want = half.double() @ wg
+    off = (2.0 ** -11 + n * 2.0 ** -23 + 2.0 ** -37) * (half.double().abs() @ wg.abs())
+    inside(gated.packed_input_grad(pg, sg, n, k, bits, group, half), want, off + 2.0 ** -11 * (want.abs() + off) + 2.0 ** -25, "fp16 dy W")
