@@ -81,6 +81,7 @@ class _Gated(torch.autograd.Function):
             raise _Unsupported("gated_packed: the call is not supported")
         ctx.shape, ctx.activation, ctx.form, ctx.x_shape = shape, activation, form, x.shape
         ctx.bias_dtypes = [None if b is None else b.dtype for b in (gate_bias, up_bias)]
+        ctx.bias_shapes = [None if b is None else b.shape for b in (gate_bias, up_bias)]
         ctx.save_for_backward(gate, gate_scales, up, up_scales, *out[1:])
         return out[0]
 
@@ -108,7 +109,7 @@ class _Gated(torch.autograd.Function):
             raise RuntimeError("gated_packed: the backward pass is not supported")
         dx, *db = out
         dx = None if dx is None else dx.view(ctx.x_shape)
-        db = [b if b is None or b.dtype == t else b.to(t) for b, t in zip(db, ctx.bias_dtypes)]
+        db = [b if b is None else b.to(t).view(s) for b, t, s in zip(db, ctx.bias_dtypes, ctx.bias_shapes)]
         return dx, *db
 
     @staticmethod
@@ -122,7 +123,7 @@ class _Gated(torch.autograd.Function):
         dx = None
         if ctx.needs_input_grad[0]:
             dx = (dg @ dequant_packed(gate, gate_scales, *ctx.shape) + du @ dequant_packed(up, up_scales, *ctx.shape)).to(dh.dtype).reshape(ctx.x_shape)
-        return dx, *(v.sum(0).to(t) if wanted else None for v, t, wanted in zip((dg, du), ctx.bias_dtypes, ctx.needs_input_grad[1:3]))
+        return dx, *(v.sum(0).to(t).reshape(s) if wanted else None for v, t, s, wanted in zip((dg, du), ctx.bias_dtypes, ctx.bias_shapes, ctx.needs_input_grad[1:3]))
 
 
 class _InputGradProduct(torch.autograd.Function):
@@ -184,7 +185,7 @@ def gated_packed(gate: torch.Tensor, gate_scales: torch.Tensor, up: torch.Tensor
             return gated_packed(gate, gate_scales, up, up_scales, rows, cols, bits, group, x.to(dt), gate_bias, up_bias, activation=activation, saved=saved)
     kind = call_kind(x, gate_bias, up_bias)
     if kind == WATCHED:                      # transforms, tangents, modes: torch's own operations on dequantised copies
-        g, u = (F.linear(x, dequant_packed(w, s, rows, cols, bits, group).to(x.dtype), None if b is None else b.to(x.dtype))
+        g, u = (F.linear(x, dequant_packed(w, s, rows, cols, bits, group).to(x.dtype), None if b is None else b.to(x.dtype).reshape(rows))
                 for w, s, b in ((gate, gate_scales, gate_bias), (up, up_scales, up_bias)))
         return _TORCH_ACTIVATIONS[activation](g) * u
     if x.numel() == 0:                       # no rows: nothing to launch, the graph as it would be

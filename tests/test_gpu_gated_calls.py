@@ -293,3 +293,19 @@ def test_weights_beyond_fp16(bits, m, n, k, group):
     want = half.double() @ wg
     off = (2.0 ** -11 + n * 2.0 ** -23 + 2.0 ** -37) * (half.double().abs() @ wg.abs())
     inside(gated.packed_input_grad(pg, sg, n, k, bits, group, half), want, off + 2.0 ** -11 * (want.abs() + off) + 2.0 ** -25, "fp16 dy W")
+
+
+@pytest.mark.parametrize("shape", [(1, 130), (130, 1), (2, 65)])
+@pytest.mark.parametrize("batched", [False, True])
+def test_biases_of_any_shape(shape, batched):
+    """A bias is as many values as the weight has rows; its gradient has its shape."""
+    n, k, m = 130, 256, 5
+    (pg, sg, _), (pu, su, _) = _layers(n, k, 4, 128, 1)
+    x, dh = _inputs(m, k, F32, 2), _inputs(m, n, F32, 3)
+    flat, shaped = ([b.view(s).requires_grad_() for b in (_inputs(1, n, F32, 4), _inputs(1, n, F32, 5))] for s in ((n,), shape))
+    (h, got), (want_h, want) = ((y.detach(), torch.autograd.grad(y, b, dh[None] if batched else dh, is_grads_batched=batched)) for b in (shaped, flat)
+                                for y in [gated.gated_packed(pg, sg, pu, su, n, k, 4, 128, x, *b)])
+    assert torch.equal(h, want_h)
+    assert all(g.shape == ((1, *shape) if batched else shape) and torch.equal(g.flatten(), w.flatten()) for g, w in zip(got, want))
+    watched = torch.func.vmap(lambda t: gated.gated_packed(pg, sg, pu, su, n, k, 4, 128, t, *(b.detach() for b in shaped)))(x)
+    assert (watched - h).norm() <= 2.0 ** -16 * h.norm()
