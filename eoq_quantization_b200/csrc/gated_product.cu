@@ -474,9 +474,10 @@ gated_product_kernel(const __grid_constant__ ProductArgs a, const __grid_constan
                     fence_after();
                     Ring nr = ar;
                     nr.next(a.ns);
-                    ready = for_the_warp(bar_test(bar(bFull + nr.at), nr.lap));         // asked for while this block's products are being issued
+                    const bool there = bar_test(bar(bFull + nr.at), nr.lap);         // asked for while this block's products are being issued
                     // (past the last column of a forward product the codes are the copy's zeros, times a scale, and the activations zeros)
                     if (!wait.lost) mma_block(d, tmem + a_base + ar.at * 32u, desc0 + ((ar.at * xstage) >> 4), idesc, i, bar(bEmpty + ar.at));
+                    ready = for_the_warp(there);
                     ar = nr;
                 }
                 if (!wait.lost) commit_pair(bar(bOutFull + dr.at));       // else the way out's waits run out too, in both CTAs
@@ -652,8 +653,6 @@ gated_product_kernel(const __grid_constant__ ProductArgs a, const __grid_constan
                     for (uint32_t j = 0; j < 16; j++) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(u[j]) : "r"(other + j * 128u));
                     const uint32_t t = gate ? t0 : t0 + 16u;
                     const bool work = gate || two;
-                    look_at(g);
-                    look_at(u);
                     if (!gate) {
 #pragma unroll
                         for (uint32_t j = 0; j < 16; j++) { const float v = g[j]; g[j] = u[j]; u[j] = v; }
@@ -678,6 +677,7 @@ gated_product_kernel(const __grid_constant__ ProductArgs a, const __grid_constan
 #pragma unroll
                             for (uint32_t j = 0; j < 16; j++) h[j] = activation(g[j], a.act) * u[j];
                         }
+                        look_at(h);                              // (not finite where g or u is not)
                         put(a.y, at, a.N, tokens - t, h);
                         if (a.keep.form == kKeepFull) {
                             put(a.keep.v[0], at, a.N, tokens - t, g);
