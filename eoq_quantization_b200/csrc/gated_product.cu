@@ -24,12 +24,16 @@
 // from one tile to the next while four warps bring the last one out; two accumulators take turns where tensor memory has room for them
 // (tiles of up to 160 tokens).
 //
-// Measured (4 bits, fp16, back to back, codes from HBM; in brackets the products at 1688 TFLOP/s): 11008 x 4096, forward 64 rows 35 us (7.5),
-// 256 61 (27), 777 126 (83), 2048 303 (219); gradient of one weight 512 rows 47 (27), 1024 69 (55), 2048 135 (109); 28672 x 8192, 2048 rows
-// 1490 (1140; long runs at full power meet 1422 TFLOP/s, 1353) and 734 (570).  What bounds it: with tiles of 256 tokens the tensor pipe (79 % of
-// active cycles for gradients of 1024 rows; 57 % forward at 777), beside it the producers' issue slots (69 % forward) and, where tensor memory
+// Measured (4 bits, fp16, back to back, codes from HBM; in brackets the products at 1688 TFLOP/s): 11008 x 4096, forward 64 rows 36 us (7.5),
+// 256 65 (27), 777 131 (83), 2048 313 (219); gradient of one weight 512 rows 48 (27), 1024 70 (55), 2048 137 (109); 28672 x 8192, 2048 rows
+// 1540 (1140; long runs at full power meet 1422 TFLOP/s, 1353) and 715 (570).  What bounds it: with tiles of 256 tokens the tensor pipe (79 % of
+// active cycles for gradients of 1024 rows; 56 % forward at 777), beside it the producers' issue slots (70 % forward) and, where tensor memory
 // holds one accumulator, the way out between two tiles; few rows: 430 clocks a block of 64, the producers' hand-over, whatever the tokens.
 // Six producer sets, because a set's block takes some 2500 clocks from its codes' arrival to its operand's: four gave 650 clocks a block.
+//
+// A product of code and scale that fp16 has no room for makes its sums infinities or NaN: the way out looks for such, and computes a tile
+// again in fp32 where the weights' scales can be why (11008 x 4096 with all scales at 20000: 64 rows 10 ms; 27 us for the look at the
+// scales of a gradient that has a NaN of its own).
 //
 // Waits are bounded, as in the product kernel for one weight (qmm.cu): one that runs out marks the CTA, whose results become NaN,
 // and sets a status word.
@@ -241,7 +245,7 @@ __device__ __forceinline__ void eight_codes(const uint8_t *from, float (&c)[8])
 }
 
 // Sums of sixteen tokens again, in fp32 throughout, for weights that fp16 has no room for (beyond 65504, which takes scales above 511 for
-// byte codes, 8188 for four bits).  forward: of row n of a weight; gradient: of column n of all weights.
+// byte codes, 8188 for four bits): a thread goes through all codes of its row.  forward: of row n of a weight; gradient: of column n of all weights.
 template <bool GRAD, int BITS>
 __device__ __noinline__ void sums_in_fp32(const ProductArgs &a, uint32_t which, uint32_t n, uint32_t token, float (&v)[16])
 {

@@ -1,4 +1,5 @@
-// The gated block for a few rows (up to eight of 16-bit activations): one pass over both weights' codes.
+// The gated block for a few rows of 16-bit activations, one pass over both weights' codes: up to eight rows here, up to 32 in the
+// second kernel below.
 //
 // Warp-level products, D[16 x 8] += A[16 x 16] B[16 x 8] (mma.sync m16n8k16), the codes exact and the scales applied to the sums in
 // fp32, with gate rows and up rows of the same features in one instruction: lane (g, t) takes gate row g as A's row g and up row g as
@@ -11,7 +12,7 @@
 // and what the warps left is added up in their order.  Each warp has a ring of chunks of its own, which TMA fills some chunks ahead:
 // what has to be under way to keep HBM busy (50 KB an SM) would not fit the registers.
 //   Measured (4 bits, groups of 128, fp16, back to back, codes from HBM; in brackets what both weights' bytes take at 6470 GB/s): 11008 x 4096
-// one row 13.0 us (7.2), eight 14.9; 28672 x 8192 one row 50.8 (37.4); 704 x 512 3.0; 11008 x 4096 of 8 bits 19.0 (14.2).  What bounds it at
+// one row 13.1 us (7.2), eight 15.0; 28672 x 8192 one row 51.0 (37.4); 704 x 512 3.0; 11008 x 4096 of 8 bits 19.1 (14.2).  What bounds it at
 // length is the issue slots (70 % of active cycles) and the integer pipe (51 %) of the unpacking, with HBM at 53 %; short calls are their start.
 //   Waits are bounded: a warp whose copy does not come marks the CTA, whose results become NaN, and sets the status word.
 #include "gated.h"
@@ -346,8 +347,9 @@ __global__ void __launch_bounds__(most_threads(BT), 1) gated_rows_kernel(const R
 // its tile, its sums in registers, through all slices; where a CTA has fewer tiles than warps, SPLIT warps take a tile's chunks in turn, and
 // what they have is added up in their order at the end.
 //   What bounds it: the warp-level tensor pipe (8 clocks a product and scheduler, 8 NT products of 128 columns), then the unpacking, and
-// with 20 warps an SM their waits for shared memory (28672 x 8192, 24 rows: tensor pipe 36 % of active cycles, shared memory's 61 %, slots 47 %).
-//   Measured as above: 11008 x 4096 16 rows 18.6 us, 24 rows 23.9 (7.3), 28672 x 8192 24 rows 119.
+// with few warps an SM their waits for shared memory (28672 x 8192, 24 rows: 13 of 20 warps work, for a tile takes whole warps and a CTA has
+// 25 tiles in two rounds of 13; tensor pipe 38 % of active cycles, slots 46 %).  11008 features are ten tiles a CTA, two warps each.
+//   Measured as above: 11008 x 4096 16 rows 18.2 us, 24 rows 22.9 (7.3), 28672 x 8192 24 rows 108 to 116.
 // ---------------------------------------------------------------------------
 constexpr uint32_t kManyWarps = 20, kStagers = 4;
 
@@ -689,7 +691,8 @@ static ManyRoom many_room(const PackedPair &w, uint32_t batch)
 
 // Rows of whole 128-byte lines, whole units a group, scales that can be loaded two at a time, activations that fit beside two chunks a warp.
 // 32 rows, or 24 of large weights, for which the products of pairs of SMs are quicker from there on (us, here at 32 rows and there at 33: 2816 x 1024
-// 7.9 and 10.9, 11008 x 4096 30.2 and 33.6, 14336 x 4096 40.8 and 37.2, 28672 x 8192 141 and 111; here at 24 rows 32.5 and 113 for the last two).
+// 7.9 and 10.9, 11008 x 4096 30.2 and 33.6, 14336 x 4096 40.8 and 37.2, 28672 x 8192 141 and 111; here at 24 rows 32.5 and 113 for the last two.
+// The large ones run 13 warps here; a size between with all 20 has not been measured).
 bool gated_rows_takes(const PackedPair &w, uint32_t batch)
 {
     const uint32_t most = (uint64_t)w.N * w.K > 50ull << 20 ? 24u : 32u;

@@ -560,8 +560,9 @@ typedef struct eoq_b200_kept {
 /* x [batch, cols] to h [batch, rows], both of type dtype (EOQ_B200_F16 / BF16 / F32), sums in fp32; kept may be NULL.  d_scratch:
  * eoq_b200_gated_scratch() bytes, 16-byte aligned (may be NULL where that is 0).  Any shape; 16-byte aligned pointers, whole
  * groups per row, groups that are multiples of 32 and packed rows that are multiples of 16 bytes take the tensor-core forms.
- * Up to 24 rows of 16-bit activations (32, where a weight has no more than 50 Mi values), codes and activations are exact there and
- * scales apply to the sums.  Beyond, activations go in as
+ * Up to 24 rows of 16-bit activations (32, where a weight has no more than 50 Mi values) of packed rows that are multiples of 128
+ * bytes (2 bits: in groups that are multiples of 64, too), codes and activations are exact there and scales apply to the sums, as long
+ * as the activations fit shared memory.  Other rows, and beyond, activations go in as
  * fp16, bf16 ones times a power of two per row, which is exact for all but what is 2^-24 below the row's largest, and code x scale is
  * rounded to fp16 once (tiles of weights that fp16 has no room for, beyond 65504, are computed again in fp32, slowly; so are the
  * gradients' below).  Asynchronous. */
