@@ -45,7 +45,7 @@ PackedPair pair_of(const eoq_b200_gated_t *w)
 }
 Kept kept_of(const eoq_b200_kept_t *k)
 {
-    if (!k) return Kept{kKeepNone, {nullptr, nullptr}, {nullptr, nullptr}};
+    if (!k || k->form == kKeepNone) return Kept{kKeepNone, {nullptr, nullptr}, {nullptr, nullptr}};
     return Kept{k->form, {k->gate, k->up}, {k->gate_scales, k->up_scales}};
 }
 size_t values(uint32_t batch, uint32_t n) { return (size_t)batch * n; }

@@ -553,7 +553,7 @@ typedef struct eoq_b200_kept {
     float *gate_scales, *up_scales;
 } eoq_b200_kept_t;
 
-#define EOQ_B200_KEEP_NONE 0
+#define EOQ_B200_KEEP_NONE 0   /* nothing, whatever the pointers are */
 #define EOQ_B200_KEEP_FULL 1
 #define EOQ_B200_KEEP_8BIT 2
 

@@ -309,3 +309,51 @@ def test_biases_of_any_shape(shape, batched):
     assert all(g.shape == ((1, *shape) if batched else shape) and torch.equal(g.flatten(), w.flatten()) for g, w in zip(got, want))
     watched = torch.func.vmap(lambda t: gated.gated_packed(pg, sg, pu, su, n, k, 4, 128, t, *(b.detach() for b in shaped)))(x)
     assert (watched - h).norm() <= 2.0 ** -16 * h.norm()
+
+
+@pytest.mark.parametrize("m", [1, 8, 20, 40])
+@pytest.mark.parametrize("dtype,k", [(F16, 256), (F32, 256), (BF16, 77)])
+def test_nothing_is_kept_where_nothing_is_to_be(m, dtype, k):
+    """The C entry with EOQ_B200_KEEP_NONE writes to none of the pointers beside it."""
+    import ctypes as C
+    from eoq_quantization_b200 import _lib as L
+    n = 64
+    (pg, sg, wg), (pu, su, wu) = _layers(n, k, 4, 64, 1)
+    x, h = _inputs(m, k, dtype, 2), torch.empty(m, n, dtype=dtype, device="cuda")
+    other = [torch.full((m, n), 7.0, device="cuda") for _ in range(4)]
+    w = L.Gated(pg.data_ptr(), pu.data_ptr(), sg.data_ptr(), su.data_ptr(), None, None, n, k, 4, 64, 0, L.F32)
+    kept = L.Kept(0, *(t.data_ptr() for t in other))
+    code = {F16: L.F16, BF16: L.BF16, F32: L.F32}[dtype]
+    lib = L.lib()
+    scratch = torch.empty(lib.eoq_b200_gated_scratch(C.byref(w), C.byref(kept), code, m) + 16, dtype=torch.uint8, device="cuda")
+    L.check(lib.eoq_b200_gated_packed(C.byref(w), x.data_ptr(), code, m, scratch.data_ptr(), h.data_ptr(), C.byref(kept), torch.cuda.current_stream().cuda_stream), "call")
+    want = Gated(x, wg, wu, "silu")
+    inside(h, want.h, want.h_bound(), "h")
+    assert all((t == 7).all() for t in other)
+
+
+@pytest.mark.parametrize("bits", [2, 4, 8])
+@pytest.mark.parametrize("m,dtype", [(1, F16), (20, BF16), (40, F16), (300, BF16), (5, F32)])
+def test_any_bytes(bits, m, dtype):
+    """Codes to the very ends of their bits (2, 8, -128), scales of either sign and of zero."""
+    n, k, group = 130, 512, 64
+
+    def layer(seed):
+        gen = torch.Generator().manual_seed(seed)
+        raw = torch.randint(0, 256, (n, k if bits == 8 else k * bits // 8), generator=gen)
+        scales = (torch.randn(n * k // group, generator=gen) * 0.01).to(F16)
+        scales[::7] = 0
+        if bits == 8:
+            packed = raw.to(torch.uint8).view(torch.int8)
+            codes = packed.double()
+        else:
+            packed = raw.to(torch.uint8)
+            codes = torch.stack([(raw >> s) & (2 ** bits - 1) for s in range(0, 8, bits)], -1).view(n, k).double() - (2 ** (bits - 1) - 1)
+        return packed.cuda(), scales.cuda(), (codes * scales.double().repeat_interleave(group).view(n, k)).cuda()
+    (pg, sg, wg), (pu, su, wu) = layer(1), layer(2)
+    x, dh = _inputs(m, k, dtype, 3).requires_grad_(), _inputs(m, n, dtype, 4)
+    want = Gated(x.detach(), wg, wu, "silu")
+    h = gated.gated_packed(pg, sg, pu, su, n, k, bits, group, x)
+    inside(h.detach(), want.h, want.h_bound(), "h")
+    (v, e), *_ = want.gradients(dh, "full")
+    inside(torch.autograd.grad(h, x, dh)[0], v, e, "dx")
