@@ -60,11 +60,12 @@ def _without_autocast():
 
 
 class _Once(torch.autograd.Function):
-    """A gradient that depends on what it was taken at, which nobody can differentiate again: an error instead of a zero."""
+    """A zero to be added to a gradient that depends on what it was taken at and that nobody can differentiate again: an error on the
+    way to whatever `tie` is made of, instead of a gradient that is a constant."""
 
     @staticmethod
-    def forward(ctx, value, wanted):
-        return value.view_as(value)
+    def forward(ctx, tie, dtype):
+        return tie.new_zeros((), dtype=dtype)
 
     @staticmethod
     def backward(ctx, _):
@@ -72,7 +73,8 @@ class _Once(torch.autograd.Function):
 
 
 class _Gated(torch.autograd.Function):
-    """h, and from what the forward pass kept of gate and up the gradients of x and the biases."""
+    """h, and from what the forward pass kept of gate and up the gradients of x and the biases.  Beside h an empty result, which
+    ties the gradients to x and the biases without holding them."""
 
     @staticmethod
     def forward(ctx, x, gate_bias, up_bias, gate, gate_scales, up, up_scales, shape, activation, form):
@@ -82,20 +84,25 @@ class _Gated(torch.autograd.Function):
         ctx.shape, ctx.activation, ctx.form, ctx.x_shape = shape, activation, form, x.shape
         ctx.bias_dtypes = [None if b is None else b.dtype for b in (gate_bias, up_bias)]
         ctx.bias_shapes = [None if b is None else b.shape for b in (gate_bias, up_bias)]
-        ctx.save_for_backward(gate, gate_scales, up, up_scales, *out[1:])
-        return out[0]
+        tie = torch.empty(0)
+        ctx.save_for_backward(gate, gate_scales, up, up_scales, tie, *out[1:])
+        ctx.set_materialize_grads(False)
+        return out[0], tie
 
     @staticmethod
-    def backward(ctx, dh):
+    def backward(ctx, dh, _):
+        if dh is None:
+            return (None,) * 10
+        saved = ctx.saved_tensors                # an error if the weights have been written since
         with torch.no_grad():
-            gradients = _Gated._gradients(ctx, dh)
+            gradients = _Gated._gradients(ctx, dh, saved)
         if torch.is_grad_enabled():              # create_graph
-            gradients = [None if v is None else _Once.apply(v, torch.zeros((), requires_grad=True)) for v in gradients]
+            gradients = [None if v is None else v + _Once.apply(saved[4], v.dtype) for v in gradients]
         return (*gradients,) + (None,) * 7
 
     @staticmethod
-    def _gradients(ctx, dh):
-        gate, gate_scales, up, up_scales, *kept = ctx.saved_tensors          # an error if the weights have been written since
+    def _gradients(ctx, dh, saved):
+        gate, gate_scales, up, up_scales, _, *kept = saved
         if call_kind(dh) == WATCHED:             # several gradients at once (is_grads_batched)
             with _without_autocast():
                 return _Gated._watched_gradients(ctx, dh, gate, gate_scales, up, up_scales, kept)
@@ -165,7 +172,7 @@ def gated_packed(gate: torch.Tensor, gate_scales: torch.Tensor, up: torch.Tensor
         # training: the checks below are for what this does not take
         if call_kind(x, gate_bias, up_bias) == GRADIENT and not torch.is_autocast_enabled("cuda") and not gate_scales.requires_grad and not up_scales.requires_grad:
             try:
-                return _Gated.apply(x, gate_bias, up_bias, gate, gate_scales, up, up_scales, (rows, cols, bits, group), code, KEEP[saved])
+                return _Gated.apply(x, gate_bias, up_bias, gate, gate_scales, up, up_scales, (rows, cols, bits, group), code, KEEP[saved])[0]
             except _Unsupported:
                 pass
     what = "gated_packed"
@@ -192,7 +199,7 @@ def gated_packed(gate: torch.Tensor, gate_scales: torch.Tensor, up: torch.Tensor
         h = x.new_zeros(*x.shape[:-1], rows) + x.sum() * 0
         return h if kind != GRADIENT else h + sum((b.sum() * 0).to(h.dtype) for b in (gate_bias, up_bias) if b is not None)
     if kind == GRADIENT:
-        return _Gated.apply(x, gate_bias, up_bias, gate, gate_scales, up, up_scales, (rows, cols, bits, group), code, KEEP[saved])
+        return _Gated.apply(x, gate_bias, up_bias, gate, gate_scales, up, up_scales, (rows, cols, bits, group), code, KEEP[saved])[0]
     h = _lib.native().gated_packed(gate, gate_scales, up, up_scales, rows, cols, bits, group, x, gate_bias, up_bias, code, 0)
     if h is None:
         raise RuntimeError(f"{what}: the call is not supported")

@@ -251,6 +251,11 @@ def test_second_derivatives_are_errors(what):
         assert dx.requires_grad
         with pytest.raises(RuntimeError):
             (dx.square().sum() + x.sum()).backward()
+    with pytest.raises(RuntimeError, match="differentiable once"):          # (which takes what is not reached for zeros)
+        torch.autograd.functional.hvp(lambda t: call(2 * t).sum(), x.detach(), x.detach())
+    whole = torch.autograd.functional.jacobian(call, x[:2].detach(), create_graph=True, vectorize=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        whole.sum().backward()
     dx, = torch.autograd.grad(call(x).sum(), x, create_graph=True)
     assert torch.equal(dx.detach(), plain) and not plain.requires_grad
     x.grad = None
