@@ -94,11 +94,11 @@ class _Gated(torch.autograd.Function):
         if dh is None:
             return (None,) * 10
         saved = ctx.saved_tensors                # an error if the weights have been written since
-        with torch.no_grad():
+        if not torch.is_grad_enabled():
+            return (*_Gated._gradients(ctx, dh, saved), *(None,) * 7)
+        with torch.no_grad():                    # create_graph
             gradients = _Gated._gradients(ctx, dh, saved)
-        if torch.is_grad_enabled():              # create_graph
-            gradients = [None if v is None else v + _Once.apply(saved[4], v.dtype) for v in gradients]
-        return (*gradients,) + (None,) * 7
+        return (*(None if v is None else v + _Once.apply(saved[4], v.dtype) for v in gradients), *(None,) * 7)
 
     @staticmethod
     def _gradients(ctx, dh, saved):
@@ -115,8 +115,11 @@ class _Gated(torch.autograd.Function):
         if out is None:
             raise RuntimeError("gated_packed: the backward pass is not supported")
         dx, *db = out
-        dx = None if dx is None else dx.view(ctx.x_shape)
-        db = [b if b is None else b.to(t).view(s) for b, t, s in zip(db, ctx.bias_dtypes, ctx.bias_shapes)]
+        if dx is not None and dx.shape != ctx.x_shape:
+            dx = dx.view(ctx.x_shape)
+        for i, b in enumerate(db):
+            if b is not None and (b.dtype != ctx.bias_dtypes[i] or b.shape != ctx.bias_shapes[i]):
+                db[i] = b.to(ctx.bias_dtypes[i]).view(ctx.bias_shapes[i])
         return dx, *db
 
     @staticmethod
