@@ -16,7 +16,7 @@ from torch.nn.modules import module as _modules
 
 from . import _lib
 from .core.quantized_linear import QuantizedLinear
-from .fused import _DTYPES, GRADIENT, WATCHED, autocast_dtype, call_kind, dequant_packed, require_cuda
+from .fused import _DTYPES, GRADIENT, PLAIN, WATCHED, autocast_dtype, call_kind, dequant_packed, require_cuda
 
 ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
 KEEP = {"none": 0, "full": 1, "8bit": 2}
@@ -147,13 +147,12 @@ class _InputGradProduct(torch.autograd.Function):
         return layer(x)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         packed, scales = ctx.saved_tensors
         with _without_autocast():
             dx = None
-            if ctx.needs_input_grad[0]:
-                dx = packed_input_grad(packed, scales, *ctx.shape, dy) if call_kind(dy) != WATCHED else dy @ dequant_packed(packed, scales, *ctx.shape).to(dy.dtype)
+            if ctx.needs_input_grad[0]:          # of several gradients at once, or to be differentiated again: torch's own product
+                dx = packed_input_grad(packed, scales, *ctx.shape, dy) if call_kind(dy) == PLAIN else dy @ dequant_packed(packed, scales, *ctx.shape).to(dy.dtype)
             db = dy.reshape(-1, dy.shape[-1]).sum(0).to(ctx.bias_dtype) if ctx.needs_input_grad[1] else None
         return dx, db, None, None, None
 

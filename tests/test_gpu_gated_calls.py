@@ -362,3 +362,18 @@ def test_any_bytes(bits, m, dtype):
     inside(h.detach(), want.h, want.h_bound(), "h")
     (v, e), *_ = want.gradients(dh, "full")
     inside(torch.autograd.grad(h, x, dh)[0], v, e, "dx")
+
+
+def test_second_derivatives_behind_hooked_layers():
+    """With gate and up called as layers, which can be differentiated again, down can, too."""
+    mlp = _module()
+    handle = mlp.gate.register_forward_hook(lambda module, args, out: out + 1)
+    x = _inputs(6, 256, F32, 2).requires_grad_()
+    got = []
+    for call in (mlp, lambda t: mlp.down(torch.nn.functional.silu(mlp.gate(t)) * mlp.up(t))):
+        for loss in (lambda y: y.sum(), lambda y: y.square().sum()):
+            dx, = torch.autograd.grad(loss(call(x)), x, create_graph=True)
+            got.append((dx.detach(), torch.autograd.grad(dx.square().sum(), x)[0]))
+    handle.remove()
+    for (a, b), (c, d) in zip(got[:2], got[2:]):
+        assert (a - c).norm() <= 2.0 ** -16 * c.norm() and (b - d).norm() <= 2.0 ** -16 * d.norm() and d.norm() > 0
